@@ -292,6 +292,146 @@ typedef struct starkv_prefill_args {
 
 int starkv_prefill_attention(const starkv_prefill_args* args, starkv_stream_t stream);
 
+/*
+ * Paged 4-bit key / value cache, for layers whose K / V projections are not
+ * factored (no counterpart in the reference, whose only cache of whole heads is
+ * transformers' DynamicCache).  A pool of pages of page_size tokens; a block table
+ * row names a sequence's pages in order, so position p of sequence b lives in page
+ * block_table[b][p / page_size], slot p % page_size.
+ *
+ * Quantiser (IEEE fp32, round-half-even), per token, KV head and group of 32
+ * channels, x clamped to +-65504:
+ *   s = fp16((max - min) / 15),  m = fp16(min + 8 s),  inv = s > 0 ? 1 / s : 0,
+ *   c = clamp(rint((x - m) * inv), -8, 7),  stored as c + 8;  value = s * c + m.
+ *   A group that holds a NaN reads back as NaN (m = NaN, s = 0).
+ *
+ * data: (num_pages, num_kv_heads, page_size / 16) tiles of 16 tokens, 2560 bytes:
+ *   [0, 1024)     key codes: channel d of token t is nibble d % 8 of the 32-bit word
+ *                 at t * 64 + (d % 32 / 8) * 16 + (d / 32) * 4
+ *   [1024, 2048)  value codes: nibble d % 4 of the 16-bit word at
+ *                 1024 + (t / 2) * 128 + (d % 32 / 4) * 16 + (d / 32) * 4 + (t % 2) * 2
+ *   [2048, 2304)  key parameters, fp16: s of group g at 2048 + t * 16 + g * 2, m 8 bytes on
+ *   [2304, 2560)  value parameters, fp16: s of group g at
+ *                 2304 + (t / 2) * 32 + g * 4 + (t % 2) * 2, m 16 bytes on
+ *   (the order in which the attention kernel's matrix instructions take them: one
+ *   16-byte load per thread and operand, no shuffles).
+ * bounds (nullable with bound_scales): int8 (num_pages, num_kv_heads, 2, 128), written
+ *   when a write fills a page's last slot, over the page's stored key values:
+ *   t = max|value| / 127 (bound_scales, fp32), up = min(ceil(max / t), 127),
+ *   lo = max(floor(min / t), -127) per channel (t = 0: codes 0).
+ */
+typedef struct starkv_kv4_cache {
+  void* data;               /* 16-byte aligned */
+  void* bounds;
+  float* bound_scales;
+  int32_t* error_word;      /* device int, set to a code when a kernel meets a bad page or position */
+  int32_t num_pages;
+  int32_t num_kv_heads;
+  int32_t page_size;        /* 16, 32, 64 or 128 */
+  int32_t head_dim;         /* 128 */
+} starkv_kv4_cache;
+
+/* Tokens in or out: k / v (B, num_tokens, Hkv, 128) of dtype with element strides
+ * (batch, token, head; multiples of 16 bytes, 16-byte aligned bases, channels
+ * contiguous).  Token i of sequence b is position start[b] + i; only the first
+ * count[b] (NULL: num_tokens) are touched.  Positions outside the block table, or
+ * whose page id is outside the pool, are skipped and set the error word. */
+typedef struct starkv_kv4_io_args {
+  void* k;
+  void* v;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+  const int32_t* block_table; /* (B, table_width), rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* start;       /* (B) */
+  const int32_t* count;       /* (B) or NULL */
+  int32_t dtype;
+  int32_t batch;
+  int32_t num_tokens;
+  int32_t table_width;
+} starkv_kv4_io_args;
+
+/* Quantise num_tokens tokens per sequence into their pages.  Two sequences must
+ * not write the same page in one call. */
+int starkv_kv4_write(const starkv_kv4_cache* cache, const starkv_kv4_io_args* args, starkv_stream_t stream);
+
+/* Read positions back as s * c + m (one fp32 rounding, then one to dtype); tokens
+ * past count[b] and skipped positions read as 0. */
+int starkv_kv4_read(const starkv_kv4_cache* cache, const starkv_kv4_io_args* args, starkv_stream_t stream);
+
+/*
+ * Attention of the newest num_queries tokens of each sequence over the cache:
+ * query i of sequence b sits at position lengths[b] - num_queries + i and attends
+ * to positions [0, that], within the pages of `pages` when given.  x = scaling *
+ * q.k + mask; out = softmax(x) V; lse = log(sum exp(x)).  A query that attends to
+ * nothing (no length, mask -inf everywhere) gets out = 0, lse = -inf; what the
+ * cache holds at positions past the length or masked by -inf does not matter.
+ */
+typedef struct starkv_kv4_attention_args {
+  const void* q;              /* (B, num_queries, Hq, 128), fp16 / bf16 */
+  void* out;                  /* same shape, out_dtype */
+  float* lse;                 /* (B, num_queries, Hq) contiguous, or NULL */
+  int64_t q_strides[3];       /* elements: batch, token, head (as for k / v) */
+  int64_t out_strides[3];
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;     /* (B) tokens in the cache, the queries' own included */
+  const float* mask;          /* additive, (B, mask_width), row b at b * mask_stride (positions past it: 0), or NULL */
+  int64_t mask_stride;
+  int64_t mask_width;
+  const int32_t* pages;       /* (B, Hkv, num_selected) page ordinals of the sequence, each once, -1 = none, or NULL */
+  void* workspace;            /* starkv_kv4_workspace_size bytes, zeroed before its first use; each call leaves it ready
+                                 for the next.  One call at a time may use it. */
+  size_t workspace_bytes;
+  float scaling;
+  int32_t num_selected;
+  int32_t q_dtype;
+  int32_t out_dtype;
+  int32_t batch;
+  int32_t num_queries;
+  int32_t num_q_heads;
+  int32_t table_width;
+} starkv_kv4_attention_args;
+
+int starkv_kv4_workspace_size(size_t* bytes);
+int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attention_args* args,
+                         starkv_stream_t stream);
+
+/*
+ * The pages worth attending to, per (sequence, KV head): the first num_first and
+ * the last num_last pages of the sequence (the last may be part full), and the
+ * full pages of the highest score among the others, num_selected in all (all pages
+ * when there are no more).  Score of a page over the query columns j of the KV
+ * head (all its query heads and query tokens), with the query's int8 codes
+ * a_j = rint(q_j / u_j), u_j = max|q_j| / 127:
+ *   max_j (u_j * sum_d (a_jd > 0 ? a_jd * up_d : a_jd * lo_d)) * t
+ * (an upper bound of q.k over the page, up to the rounding of q), products rounded
+ * in that order in fp32; the sums are exact integers.  Ties go to the lower page.
+ * pages_out: int32 (B, Hkv, num_selected), ascending, then -1.
+ */
+typedef struct starkv_kv4_select_args {
+  const void* q;
+  int64_t q_strides[3];
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  int32_t* pages_out;
+  float* scores;              /* scratch, (B, Hkv, table_width) */
+  int32_t q_dtype;
+  int32_t batch;
+  int32_t num_queries;
+  int32_t num_q_heads;
+  int32_t table_width;
+  int32_t num_selected;
+  int32_t num_first;
+  int32_t num_last;           /* >= 1 */
+} starkv_kv4_select_args;
+
+int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* args, starkv_stream_t stream);
+
+/* sizeof of the four structs above, in order (ABI check for bindings). */
+size_t starkv_kv4_struct_size(int32_t which);
+
 /* Last CUDA error string seen by the library on this thread (for diagnostics). */
 const char* starkv_last_error(void);
 

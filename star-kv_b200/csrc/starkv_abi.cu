@@ -10,6 +10,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "host.hpp"
 #include "k_logits.cuh"
 #include "prefill.cuh"
 #include "quant.cuh"
@@ -466,6 +467,18 @@ int launch_pa(const starkv_layout& l, const void* hidden, int H, const void* vs_
 }
 
 }  // namespace
+
+namespace starkv {
+
+int host_error(int code, const char* msg) { return set_error(code, msg); }
+int host_launch_status() { return fail_launch(); }
+int host_device(int* sms) {
+  const int rc = check_device();
+  if (!rc && sms) *sms = device_sm_count(nullptr);
+  return rc;
+}
+
+}  // namespace starkv
 
 extern "C" {
 

@@ -63,6 +63,51 @@ class PrefillArgs(C.Structure):
     ]
 
 
+class KV4Cache(C.Structure):
+    """Mirror of ``starkv_kv4_cache``."""
+
+    _fields_ = [
+        ("data", C.c_void_p), ("bounds", C.c_void_p), ("bound_scales", C.c_void_p), ("error_word", C.c_void_p),
+        ("num_pages", C.c_int32), ("num_kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
+class KV4IoArgs(C.Structure):
+    """Mirror of ``starkv_kv4_io_args``."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("start", C.c_void_p), ("count", C.c_void_p),
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("num_tokens", C.c_int32), ("table_width", C.c_int32),
+    ]
+
+
+class KV4AttentionArgs(C.Structure):
+    """Mirror of ``starkv_kv4_attention_args``."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("q_strides", C.c_int64 * 3), ("out_strides", C.c_int64 * 3),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("lengths", C.c_void_p),
+        ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("mask_width", C.c_int64), ("pages", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("scaling", C.c_float), ("num_selected", C.c_int32), ("q_dtype", C.c_int32), ("out_dtype", C.c_int32),
+        ("batch", C.c_int32), ("num_queries", C.c_int32), ("num_q_heads", C.c_int32), ("table_width", C.c_int32),
+    ]
+
+
+class KV4SelectArgs(C.Structure):
+    """Mirror of ``starkv_kv4_select_args``."""
+
+    _fields_ = [
+        ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("lengths", C.c_void_p),
+        ("pages_out", C.c_void_p), ("scores", C.c_void_p),
+        ("q_dtype", C.c_int32), ("batch", C.c_int32), ("num_queries", C.c_int32), ("num_q_heads", C.c_int32),
+        ("table_width", C.c_int32), ("num_selected", C.c_int32), ("num_first", C.c_int32), ("num_last", C.c_int32),
+    ]
+
+
 # (name, restype, argtypes) of every exported symbol; tests check the header declares exactly these.
 SIGNATURES = [
     ("starkv_layout_size", C.c_size_t, []),
@@ -88,6 +133,13 @@ SIGNATURES = [
     ("starkv_static_read_device_error", C.c_int, [C.POINTER(C.c_int), C.c_void_p]),
     ("starkv_read_device_error", C.c_int, [C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
     ("starkv_prefill_attention", C.c_int, [C.POINTER(PrefillArgs), C.c_void_p]),
+    # the kv4 argument blocks travel as packed bytes (starkv.kv4), so as void pointers
+    ("starkv_kv4_struct_size", C.c_size_t, [C.c_int32]),
+    ("starkv_kv4_write", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("starkv_kv4_read", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("starkv_kv4_workspace_size", C.c_int, [C.POINTER(C.c_size_t)]),
+    ("starkv_kv4_attention", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("starkv_kv4_select", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("starkv_last_error", C.c_char_p, []),
 ]
 
@@ -112,6 +164,9 @@ def load(path: str = LIB_PATH):
         fn.argtypes = args
     if lib.starkv_layout_size() != C.sizeof(Layout):
         raise StarKVError("starkv_layout size mismatch between libstarkv.so and the Python binding")
+    for i, mirror in enumerate((KV4Cache, KV4IoArgs, KV4AttentionArgs, KV4SelectArgs)):
+        if lib.starkv_kv4_struct_size(i) != C.sizeof(mirror):
+            raise StarKVError(f"{mirror.__name__} size mismatch between libstarkv.so and the Python binding")
     _lib = lib
     return lib
 

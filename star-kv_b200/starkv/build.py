@@ -19,11 +19,12 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
+    "--threads", "0",
 ]
 
 
 def sources():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")))
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".hpp")))
 
 
 def nvcc() -> str:
@@ -34,12 +35,12 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/starkv_abi.cu into starkv/libstarkv.so unless it is newer than every source."""
+    """Compile csrc/*.cu into starkv/libstarkv.so unless it is newer than every source."""
     srcs = sources() + [os.path.join(INCLUDE, "starkv.h")]
     if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(s) for s in srcs):
         return OUT
     tmp = OUT + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-o", tmp, os.path.join(CSRC, "starkv_abi.cu")]
+    cmd = [nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-o", tmp, *(s for s in srcs if s.endswith(".cu"))]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), file=sys.stderr)

@@ -1,0 +1,284 @@
+"""Paged 4-bit key / value cache for layers whose K / V projections are not factored.
+
+The latent cache (``ops.LatentCache``) pays off where a layer's learned ranks are
+small; a layer whose ranks stay near the head dimension keeps its whole heads
+here instead, 5 bits a value (4-bit codes, fp16 scale and centre per 32 channels),
+in pages that sequences of a batch share a pool of:
+
+    cache = KV4Cache(num_pages, num_kv_heads, page_size=64)
+    cache.write(k, v, block_table, start)                       # prompt or newest tokens, quantised
+    out = cache.attend(q, block_table, lengths, scaling)        # newest 1..n queries, dense
+    pages = cache.select(q, block_table, lengths, 64)           # pages a score bound keeps
+    out = cache.attend(q, block_table, lengths, scaling, pages=pages)
+    k, v = cache.read(block_table, start, num_tokens)           # back to whole heads
+
+Every op launches on the current torch stream, takes its positions, lengths and
+page lists from the GPU (so a step can be captured in a CUDA graph) and goes
+through ``libstarkv.so`` (``starkv_kv4_*`` in ``include/starkv.h``, which specifies
+the layout and the arithmetic); there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import struct
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import StarKVError, check, load
+from .ops import _DT
+
+# Argument blocks (the mirrors of _lib, packed in one call: a ctypes structure
+# costs several microseconds to fill field by field).
+_CACHE = struct.Struct("4P4i")
+_IO = struct.Struct("2P3q3qPq2P4i")
+_ATTENTION = struct.Struct("3P3q3qPqPP2qPPNf7i")
+_SELECT = struct.Struct("P3qPq3P8i")
+
+_TOKEN_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+_QUERY_DTYPES = (torch.float16, torch.bfloat16)
+
+
+def _ints(t: torch.Tensor, name: str, shape, device):
+    if t.dtype != torch.int32 or t.device != device:
+        raise StarKVError(f"{name} must be an int32 tensor on {device}")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        raise StarKVError(f"{name} must be contiguous of shape {shape}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, shape, dtypes, device):
+    """Checks a (B, tokens, heads, 128) tensor; returns its element strides."""
+    if t.device != device:
+        raise StarKVError(f"{name} must be on {device}")
+    if t.dtype not in dtypes:
+        raise StarKVError(f"{name} must be one of {dtypes}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise StarKVError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    st = t.stride()
+    if st[3] != 1:
+        raise StarKVError(f"{name} channels must be contiguous")
+    if 1 in shape:                       # the stride of a dimension of one is never used
+        st = tuple(0 if n == 1 else s for n, s in zip(shape, st))
+    return st
+
+
+def _output(t: torch.Tensor, name: str):
+    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+        raise StarKVError(f"{name} must not repeat elements (stride 0)")
+
+
+class _on:
+    """The tensors' device made current (nothing where it is already)."""
+
+    def __init__(self, device):
+        self.index, self.before = device.index, None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if now != self.index:
+            self.before = now
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
+_WORKSPACES = {}
+_workspace_bytes = 0
+
+
+def workspace(device: torch.device, stream: int) -> torch.Tensor:
+    """Attention scratch of one stream (zeroed once; every call leaves it zeroed
+    where the next needs it).  A call under graph capture gets its own, zeroed by the
+    graph, so replays never share one with eager calls."""
+    global _workspace_bytes
+    key = (device.index, stream)
+    ws = _WORKSPACES.get(key)
+    if ws is not None and not torch.cuda.is_current_stream_capturing():
+        return ws
+    if not _workspace_bytes:
+        n = C.c_size_t(0)
+        check(load().starkv_kv4_workspace_size(C.byref(n)), "starkv_kv4_workspace_size")
+        _workspace_bytes = int(n.value)
+    ws = torch.zeros(_workspace_bytes, dtype=torch.uint8, device=device)
+    if not torch.cuda.is_current_stream_capturing():
+        _WORKSPACES[key] = ws
+    return ws
+
+
+class KV4Cache:
+    """A pool of ``num_pages`` pages of ``page_size`` tokens (16, 32, 64 or 128) for
+    ``num_kv_heads`` KV heads of dimension 128.
+
+    ``data``: uint8 (num_pages, num_kv_heads, page_size / 16, 2560).  With
+    ``page_bounds`` each full page also carries int8 bounds of its keys
+    (``bounds``, ``bound_scales``), which ``select`` scores.  Which pages belong to
+    which sequence is the caller's: ``block_table`` (B, W) int32 names sequence b's
+    pages in order."""
+
+    def __init__(self, num_pages: int, num_kv_heads: int, page_size: int = 64, device="cuda",
+                 page_bounds: bool = True):
+        if page_size not in (16, 32, 64, 128):
+            raise StarKVError(f"page_size must be 16, 32, 64 or 128, got {page_size}")
+        if num_pages <= 0 or num_kv_heads <= 0:
+            raise StarKVError("KV4Cache needs at least one page and one KV head")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise StarKVError("KV4Cache lives on a CUDA device")
+        self.num_pages, self.num_kv_heads, self.page_size = int(num_pages), int(num_kv_heads), int(page_size)
+        self.data = torch.zeros(num_pages, num_kv_heads, page_size // 16, 2560, dtype=torch.uint8, device=dev)
+        self.device = self.data.device
+        self.bounds = self.bound_scales = None
+        if page_bounds:
+            self.bounds = torch.zeros(num_pages, num_kv_heads, 2, 128, dtype=torch.int8, device=dev)
+            self.bound_scales = torch.zeros(num_pages, num_kv_heads, dtype=torch.float32, device=dev)
+        self.error_word = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._block = _CACHE.pack(self.data.data_ptr(), self.bounds.data_ptr() if page_bounds else 0,
+                                  self.bound_scales.data_ptr() if page_bounds else 0, self.error_word.data_ptr(),
+                                  self.num_pages, self.num_kv_heads, self.page_size, 128)
+        self._lib = load()
+
+    def nbytes(self) -> int:
+        """Device bytes of the pool (codes, parameters and bounds)."""
+        return sum(t.numel() * t.element_size() for t in (self.data, self.bounds, self.bound_scales) if t is not None)
+
+    def _table(self, t: torch.Tensor):
+        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 2 or t.shape[1] == 0:
+            raise StarKVError(f"block_table must be an int32 (B, W) tensor on {self.device}, W > 0")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise StarKVError("block_table rows must be contiguous")
+        return t.shape[0], t.shape[1], t.data_ptr(), t.stride(0)
+
+    def _io(self, fn, what, k, v, ks, vs, table, start, count):
+        B, W, tp, ts = self._table(table)
+        n = k.shape[1]
+        a = _IO.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], tp, ts,
+                     _ints(start, "start", (B,), self.device),
+                     0 if count is None else _ints(count, "count", (B,), self.device), _DT[k.dtype], B, n, W)
+        with _on(self.device) as stream:
+            check(fn(self._block, a, stream), what)
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
+              count: Optional[torch.Tensor] = None) -> None:
+        """Quantise k / v (B, T, num_kv_heads, 128; fp32, fp16 or bf16, rows of any
+        stride that is a multiple of 16 bytes) into positions start[b] .. start[b] +
+        count[b] - 1 (count: int32 (B,), T when None).  Filling a page's last slot
+        writes the page's bounds."""
+        shape = (block_table.shape[0], k.shape[1] if k.dim() == 4 else -1, self.num_kv_heads, 128)
+        ks = _rows(k, "k", shape, _TOKEN_DTYPES, self.device)
+        vs = _rows(v, "v", shape, (k.dtype,), self.device)
+        self._io(self._lib.starkv_kv4_write, "starkv_kv4_write", k, v, ks, vs, block_table, start, count)
+
+    def read(self, block_table: torch.Tensor, start: torch.Tensor, num_tokens: int,
+             count: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
+             out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Positions start[b] .. start[b] + num_tokens - 1 as (k, v), each (B,
+        num_tokens, num_kv_heads, 128) of ``dtype`` (or into ``out``); rows past count[b]
+        are 0."""
+        shape = (block_table.shape[0], int(num_tokens), self.num_kv_heads, 128)
+        if out is None:
+            if num_tokens < 0:
+                raise StarKVError("num_tokens must not be negative")
+            out = (torch.empty(shape, dtype=dtype, device=self.device),
+                   torch.empty(shape, dtype=dtype, device=self.device))
+        k, v = out
+        ks = _rows(k, "out[0]", shape, _TOKEN_DTYPES, self.device)
+        vs = _rows(v, "out[1]", shape, (k.dtype,), self.device)
+        _output(k, "out[0]")
+        _output(v, "out[1]")
+        self._io(self._lib.starkv_kv4_read, "starkv_kv4_read", k, v, ks, vs, block_table, start, count)
+        return k, v
+
+    def _queries(self, q: torch.Tensor, batch: int):
+        """q as (B, Q, Hq, 128) and its strides; a (B, Hq, 128) q is one query token."""
+        q4 = q.unsqueeze(1) if q.dim() == 3 else q
+        if q4.dim() != 4 or q4.shape[2] == 0 or q4.shape[2] % self.num_kv_heads:
+            raise StarKVError(f"q must be (B, Hq, 128) or (B, Q, Hq, 128), Hq a multiple of {self.num_kv_heads}")
+        return q4, _rows(q4, "q", (batch, q4.shape[1], q4.shape[2], 128), _QUERY_DTYPES, self.device)
+
+    def attend(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scaling: float,
+               mask: Optional[torch.Tensor] = None, pages: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, return_lse: bool = False,
+               ws: Optional[torch.Tensor] = None):
+        """Attention of each sequence's newest Q tokens, q (B, Q, Hq, 128) or (B, Hq,
+        128), over its first lengths[b] positions (the queries' own included, written
+        before): query i attends to positions up to lengths[b] - Q + i.
+
+        mask: additive fp32 (B, L), -inf excludes a position.  pages: int32 (B,
+        num_kv_heads, n) page ordinals to attend within (``select``).  Returns out of
+        q's shape and dtype (or in ``out``), and with ``return_lse`` the fp32 log-sum-exp
+        (q's shape without the channels); a query with nothing to attend to gets 0 and
+        -inf."""
+        B, W, tp, ts = self._table(block_table)
+        q4, qs = self._queries(q, B)
+        Q, Hq = q4.shape[1], q4.shape[2]
+        lp = _ints(lengths, "lengths", (B,), self.device)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        o4 = out.unsqueeze(1) if q.dim() == 3 and out.dim() == 3 else out
+        os_ = _rows(o4, "out", tuple(q4.shape), _TOKEN_DTYPES, self.device)
+        _output(o4, "out")
+        mp = mstride = mwidth = 0
+        if mask is not None:
+            if mask.dtype != torch.float32 or mask.device != self.device or mask.dim() != 2 or mask.shape[0] != B:
+                raise StarKVError(f"mask must be an fp32 (B, L) tensor on {self.device}")
+            if mask.shape[1] > 1 and mask.stride(1) != 1:
+                raise StarKVError("mask rows must be contiguous")
+            mp, mstride, mwidth = mask.data_ptr(), mask.stride(0), mask.shape[1]
+        pp = n = 0
+        if pages is not None:
+            if pages.dim() != 3 or pages.shape[2] == 0:
+                raise StarKVError("pages must be (B, num_kv_heads, n), n > 0")
+            n = pages.shape[2]
+            pp = _ints(pages, "pages", (B, self.num_kv_heads, n), self.device)
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+        with _on(self.device) as stream:
+            if ws is None:
+                ws = workspace(self.device, stream)
+            a = _ATTENTION.pack(q4.data_ptr(), o4.data_ptr(), lse.data_ptr() if return_lse else 0,
+                                qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], tp, ts, lp, mp, mstride, mwidth, pp,
+                                ws.data_ptr(), ws.numel(), scaling, n, _DT[q.dtype], _DT[out.dtype], B, Q, Hq, W)
+            check(self._lib.starkv_kv4_attention(self._block, a, stream), "starkv_kv4_attention")
+        return (out, lse) if return_lse else out
+
+    def select(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, num_pages: int,
+               first: int = 1, last: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Page ordinals to attend to, int32 (B, num_kv_heads, num_pages) ascending, then
+        -1: the sequence's first ``first`` and last ``last`` pages and, among the others,
+        those whose bound on q.k (over the KV head's query heads and tokens) is
+        highest; every page where there are no more than ``num_pages``."""
+        if self.bounds is None:
+            raise StarKVError("this KV4Cache was made without page_bounds")
+        B, W, tp, ts = self._table(block_table)
+        q4, qs = self._queries(q, B)
+        lp = _ints(lengths, "lengths", (B,), self.device)
+        shape = (B, self.num_kv_heads, int(num_pages))
+        if out is None:
+            if num_pages <= 0:
+                raise StarKVError("num_pages must be positive")
+            out = torch.empty(shape, dtype=torch.int32, device=self.device)
+        op = _ints(out, "out", shape, self.device)
+        scores = torch.empty(B * self.num_kv_heads * W, dtype=torch.float32, device=self.device)
+        a = _SELECT.pack(q4.data_ptr(), qs[0], qs[1], qs[2], tp, ts, lp, op, scores.data_ptr(), _DT[q.dtype], B,
+                         q4.shape[1], q4.shape[2], W, num_pages, first, last)
+        with _on(self.device) as stream:
+            check(self._lib.starkv_kv4_select(self._block, a, stream), "starkv_kv4_select")
+        return out
+
+    def read_error(self) -> int:
+        """Read and clear the pool's device error word (synchronises): 0, or a code of
+        ``ERRORS``."""
+        code = int(self.error_word.item())
+        if code:
+            self.error_word.zero_()
+        return code
+
+
+#: Codes of the device error word.
+ERRORS = {0x101: "a bulk copy never completed", 0x201: "a block table names a page outside the pool",
+          0x202: "a position or length lies outside the block table"}

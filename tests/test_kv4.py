@@ -1,0 +1,85 @@
+"""The paged 4-bit cache on a machine without a GPU: the argument blocks match the
+library's structs, the host checks refuse, and the oracle's quantiser has the
+properties its specification states."""
+
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_oracle as O
+from starkv import _lib, kv4
+
+
+@pytest.mark.parametrize("which,mirror,packed", [(0, _lib.KV4Cache, kv4._CACHE), (1, _lib.KV4IoArgs, kv4._IO),
+                                                 (2, _lib.KV4AttentionArgs, kv4._ATTENTION),
+                                                 (3, _lib.KV4SelectArgs, kv4._SELECT)])
+def test_argument_blocks(which, mirror, packed):
+    assert _lib.load().starkv_kv4_struct_size(which) == C.sizeof(mirror) == packed.size
+    # packed in field order, arrays spread out
+    n = sum(f[1]._length_ if hasattr(f[1], "_length_") else 1 for f in mirror._fields_)
+    got = mirror.from_buffer_copy(packed.pack(*range(1, n + 1)))
+    flat = []
+    for name, *_ in mirror._fields_:
+        v = getattr(got, name)
+        flat += list(v) if hasattr(v, "_length_") else [v]
+    assert [int(x) for x in flat] == list(range(1, n + 1))
+
+
+def test_no_cpu_path():
+    with pytest.raises(_lib.StarKVError):
+        kv4.KV4Cache(4, 2, device="cpu")
+    lib = _lib.load()
+    z = b"\0" * 256
+    for fn in (lib.starkv_kv4_write, lib.starkv_kv4_read, lib.starkv_kv4_attention, lib.starkv_kv4_select):
+        assert fn(z, z, None) == 1                              # null cache: refused before any CUDA call
+
+
+@pytest.mark.parametrize("field,value,status", [("head_dim", 64, 2), ("page_size", 48, 2), ("num_pages", 0, 1),
+                                                ("num_kv_heads", 0, 1), ("data", 8, 1), ("bounds", 0, 1)])
+def test_pool_checks(field, value, status):
+    c = _lib.KV4Cache(data=256, bounds=256, bound_scales=256, error_word=256, num_pages=4, num_kv_heads=2,
+                      page_size=64, head_dim=128)
+    setattr(c, field, value)
+    a = _lib.KV4IoArgs()
+    assert _lib.load().starkv_kv4_write(C.byref(c), C.byref(a), None) == status
+
+
+def test_oracle_quantiser():
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((50, 128)) * 10.0 ** rng.uniform(-3, 3, (50, 1))
+    x = x.astype(np.float16).astype(np.float64)
+    c, s, m = O.quantise(x)
+    assert c.min() == -8 and c.max() == 7
+    g = x.reshape(50, 4, 32)
+    # half a step, plus what rounding the centre to fp16 may cut off at an end
+    room = 0.5 * s + np.abs(m) * 2.0 ** -11 + np.abs(s) * 16 * 2.0 ** -11 + 2.0 ** -24
+    assert (np.abs(O.values(x).reshape(50, 4, 32) - g) <= room[..., None] * 1.01).all()
+    assert (O.values(np.full((1, 128), 0.1)) == np.float64(np.float16(0.1))).all()
+
+
+def test_oracle_bounds_hold():
+    """A page's score is not below q.k of any of its tokens by more than the rounding of q."""
+    rng = np.random.default_rng(1)
+    page = O.values(rng.standard_normal((32, 128)))
+    up, lo, t = O.bounds(page)
+    assert (up * t >= page.max(0) - 1e-5).all() and (lo * t <= page.min(0) + 1e-5).all()
+    q = rng.standard_normal((3, 128))
+    u = np.abs(q).max(-1) / 127
+    a = np.rint(q / u[:, None])
+    score = (np.where(a > 0, a * up, a * lo).sum(-1) * u * t)
+    slack = 0.5 * u * np.abs(page).sum(-1).max()
+    assert (score >= (q @ page.T).max(-1) - slack - 1e-3).all()
+
+
+def test_oracle_attention_is_softmax():
+    rng = np.random.default_rng(2)
+    q, k, v = rng.standard_normal((2, 3, 128)), rng.standard_normal((9, 128)), rng.standard_normal((9, 128))
+    out, lse, w = O.attend(q, k, v, 0.1)
+    x = torch.from_numpy(q[1] @ k.T * 0.1)
+    assert np.allclose(out[1], (torch.softmax(x, -1) @ torch.from_numpy(v)).numpy())
+    assert np.allclose(lse[1], torch.logsumexp(x, -1).numpy())
+    assert (w[0][:, 8] == 0).all() and np.allclose(w.sum(-1), 1)
+    out, lse, _ = O.attend(q, k[:1], v[:1], 0.1)                # one token, two queries: the first sees nothing
+    assert (out[0] == 0).all() and np.isneginf(lse[0]).all() and np.allclose(out[1], v[:1])
