@@ -3,6 +3,7 @@
 // memory or synchronises.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "host.hpp"
@@ -72,6 +73,23 @@ int io_params(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, Kv4IoP
   return STARKV_OK;
 }
 
+template <int NT, bool MASK>
+int launch_attn(const Kv4AttnParams& p, int grid, cudaStream_t st) {
+  auto kern = kv4_attn_kernel<NT, MASK>;
+  const size_t smem = sizeof(Kv4AttnSmem<NT>);
+  static_assert(sizeof(Kv4AttnSmem<NT>) <= 227 * 1024, "shared memory of one SM");
+  static std::atomic<uint64_t> raised{0};                      // one bit a device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return host_launch_status();
+  if (dev >= 64 || !(raised.load(std::memory_order_relaxed) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return host_launch_status();
+    if (dev < 64) raised.fetch_or(1ull << dev);
+  }
+  kern<<<grid, kKv4Warps * 32, smem, st>>>(p);
+  return host_launch_status();
+}
+
 }  // namespace
 
 extern "C" {
@@ -128,7 +146,7 @@ int starkv_kv4_read(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, 
 
 int starkv_kv4_workspace_size(size_t* bytes) {
   if (!bytes) return host_error(STARKV_ERR_INVALID, "null argument");
-  *bytes = 256;
+  *bytes = kKv4CounterBytes + (size_t)kKv4MaxGrid * 2 * kKv4PartFloats * sizeof(float);
   return STARKV_OK;
 }
 
@@ -177,13 +195,25 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   p.width = a->table_width;
   const int64_t cols = (int64_t)p.group * p.queries;
   if (cols > 65536) return host_error(STARKV_ERR_UNSUPPORTED, "too many query columns");
-  const dim3 grid((unsigned)cols, (unsigned)p.pool.heads, (unsigned)p.batch);
+  // up to 8 columns one n-tile of the matrix instructions, more in blocks of 16
+  const int nt = cols <= 8 ? 1 : 2;
+  p.q_dtype = a->q_dtype;
+  p.col_blocks = (int)((cols + nt * 8 - 1) / (nt * 8));
+  if ((int64_t)p.pool.heads * p.col_blocks > (1 << 24))
+    return host_error(STARKV_ERR_UNSUPPORTED, "too many query columns");
+  if (((int64_t)a->table_width << p.pool.page_shift) > 0x7fffff00)
+    return host_error(STARKV_ERR_UNSUPPORTED, "block table of 2^31 positions or more");
+  if (a->pages && (int64_t)a->num_selected * p.pool.page_tiles > 0x7fffff00)
+    return host_error(STARKV_ERR_UNSUPPORTED, "too many selected pages");
+  int sms = 0;
+  if ((rc = host_device(&sms))) return rc;
+  const int grid = sms < kKv4MaxGrid ? sms : kKv4MaxGrid;
+  p.counters = (int*)a->workspace;
+  p.parts = (float*)((uint8_t*)a->workspace + kKv4CounterBytes);
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->q_dtype == STARKV_F16)
-    kv4_attn_kernel<__half><<<grid, 128, 0, st>>>(p);
-  else
-    kv4_attn_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p);
-  return host_launch_status();
+  if (nt == 1)
+    return p.mask ? launch_attn<1, true>(p, grid, st) : launch_attn<1, false>(p, grid, st);
+  return p.mask ? launch_attn<2, true>(p, grid, st) : launch_attn<2, false>(p, grid, st);
 }
 
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* a, starkv_stream_t stream) {
