@@ -73,11 +73,11 @@ int io_params(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, Kv4IoP
   return STARKV_OK;
 }
 
-template <int NT, bool MASK>
+template <int NT, int W, bool MASK>
 int launch_attn(const Kv4AttnParams& p, int grid, cudaStream_t st) {
-  auto kern = kv4_attn_kernel<NT, MASK>;
-  const size_t smem = sizeof(Kv4AttnSmem<NT>);
-  static_assert(sizeof(Kv4AttnSmem<NT>) <= 227 * 1024, "shared memory of one SM");
+  auto kern = kv4_attn_kernel<NT, W, MASK>;
+  const size_t smem = sizeof(Kv4AttnSmem<NT, W>);
+  static_assert(sizeof(Kv4AttnSmem<NT, W>) <= 227 * 1024, "shared memory of one SM");
   static std::atomic<uint64_t> raised{0};                      // one bit a device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return host_launch_status();
@@ -86,7 +86,7 @@ int launch_attn(const Kv4AttnParams& p, int grid, cudaStream_t st) {
       return host_launch_status();
     if (dev < 64) raised.fetch_or(1ull << dev);
   }
-  kern<<<grid, kKv4Warps * 32, smem, st>>>(p);
+  kern<<<grid, W * 32, smem, st>>>(p);
   return host_launch_status();
 }
 
@@ -203,8 +203,9 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
     return host_error(STARKV_ERR_UNSUPPORTED, "too many query columns");
   if (((int64_t)a->table_width << p.pool.page_shift) > 0x7fffff00)
     return host_error(STARKV_ERR_UNSUPPORTED, "block table of 2^31 positions or more");
-  if (a->pages && (int64_t)a->num_selected * p.pool.page_tiles > 0x7fffff00)
-    return host_error(STARKV_ERR_UNSUPPORTED, "too many selected pages");
+  const int64_t tiles = (a->pages ? (int64_t)a->num_selected : (int64_t)a->table_width) * p.pool.page_tiles;
+  if ((double)tiles * p.pool.heads * p.col_blocks * a->batch > 2.0e9)
+    return host_error(STARKV_ERR_UNSUPPORTED, "batch * KV heads * tiles of a block table row must stay below 2e9");
   int sms = 0;
   if ((rc = host_device(&sms))) return rc;
   const int grid = sms < kKv4MaxGrid ? sms : kKv4MaxGrid;
@@ -212,8 +213,8 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   p.parts = (float*)((uint8_t*)a->workspace + kKv4CounterBytes);
   cudaStream_t st = (cudaStream_t)stream;
   if (nt == 1)
-    return p.mask ? launch_attn<1, true>(p, grid, st) : launch_attn<1, false>(p, grid, st);
-  return p.mask ? launch_attn<2, true>(p, grid, st) : launch_attn<2, false>(p, grid, st);
+    return p.mask ? launch_attn<1, 16, true>(p, grid, st) : launch_attn<1, 16, false>(p, grid, st);
+  return p.mask ? launch_attn<2, 8, true>(p, grid, st) : launch_attn<2, 8, false>(p, grid, st);
 }
 
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* a, starkv_stream_t stream) {
