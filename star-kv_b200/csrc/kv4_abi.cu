@@ -86,7 +86,7 @@ int launch_attn(const Kv4AttnParams& p, int grid, cudaStream_t st) {
       return host_launch_status();
     if (dev < 64) raised.fetch_or(1ull << dev);
   }
-  kern<<<grid, W * 32, smem, st>>>(p);
+  kern<<<grid, (W + 1) * 32, smem, st>>>(p);
   return host_launch_status();
 }
 
@@ -213,8 +213,8 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   p.parts = (float*)((uint8_t*)a->workspace + kKv4CounterBytes);
   cudaStream_t st = (cudaStream_t)stream;
   if (nt == 1)
-    return p.mask ? launch_attn<1, 16, true>(p, grid, st) : launch_attn<1, 16, false>(p, grid, st);
-  return p.mask ? launch_attn<2, 8, true>(p, grid, st) : launch_attn<2, 8, false>(p, grid, st);
+    return p.mask ? launch_attn<1, 15, true>(p, grid, st) : launch_attn<1, 15, false>(p, grid, st);
+  return p.mask ? launch_attn<2, 7, true>(p, grid, st) : launch_attn<2, 7, false>(p, grid, st);
 }
 
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* a, starkv_stream_t stream) {

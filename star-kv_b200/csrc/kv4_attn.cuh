@@ -93,10 +93,6 @@ __device__ __forceinline__ uint32_t kv4_hmul2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t kv4_hmax2(uint32_t a, uint32_t b) {
-  const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ float2 kv4_float2(uint32_t a) {
   return __half22float2(*reinterpret_cast<const __half2*>(&a));
 }
@@ -186,20 +182,20 @@ struct Kv4Piece {
 template <int NT, int W>
 struct Kv4AttnSmem {
   static constexpr int kCols = NT * 8;
-  static constexpr int kRing = 64 / W;      // tile slots of a warp
-  alignas(128) uint8_t ring[W][kRing][kKv4TileBytes];
+  static constexpr int kRing = 32 / W;      // stages of a warp, two tiles each
+  alignas(128) uint8_t ring[W][kRing][2][kKv4TileBytes];
   alignas(16) float head[W][kCols * 130];
-  alignas(8) uint64_t bar[W][kRing];
-  int pos[W][kRing];                        // position of a slot's first token, -1: nothing to attend to
+  alignas(8) uint64_t full[W][kRing], empty[W][kRing];
+  int pos[W][kRing][2];                     // position of a tile's first token, -1: nothing to attend to
   Kv4Piece piece[2 * W];
-  int scan[W];
+  int scan[W + 1];
   int base[W];                              // first tile of the warp's first sequence
   int first[W];                             // that sequence
   int last;
   // piece i: o (cols, 128), base (cols), l (cols).  The first piece of a warp has its own space,
   // the second lies over the warp's ring.
   __device__ __forceinline__ float* part(int i) {
-    return i & 1 ? reinterpret_cast<float*>(ring[i >> 1][0]) : head[i >> 1];
+    return i & 1 ? reinterpret_cast<float*>(ring[i >> 1][0][0]) : head[i >> 1];
   }
 };
 
@@ -385,16 +381,15 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos
     ta.x &= la, ta.y &= la, ta.z &= la, ta.w &= la, ma &= la;
     tb.x &= lb, tb.y &= lb, tb.z &= lb, tb.w &= lb, mb &= lb;
   }
-  const uint32_t big = kv4_hmax2(kv4_hmax2(kv4_hmax2(ta.x, ta.y), kv4_hmax2(ta.z, ta.w)),
-                                 kv4_hmax2(kv4_hmax2(tb.x, tb.y), kv4_hmax2(tb.z, tb.w)));
   // an s above 2^e in either half (the bits of positive fp16 numbers order like integers)
-  const uint32_t lim = (uint32_t)(15 + s.e) << 10;
-  over |= (big & 0xffffu) > lim;
-  over |= big > (lim << 16 | 0xffffu);
+  const uint32_t lim = (uint32_t)(15 + s.e) * 0x04000400u;
+  const uint32_t big = __vimax3_u16x2(__vimax3_u16x2(ta.x, ta.y, ta.z), __vimax3_u16x2(ta.w, tb.x, tb.y),
+                                      __vimax3_u16x2(tb.z, tb.w, lim));
+  over |= big != lim;
   // ---- a score or an s that the base does not cover
   if (__any_sync(0xffffffffu, over)) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
-    const int e_new = max(s.e, (int)((top + 0x3ffu) >> 10) - 15);
+    const int e_new = (int)((top + 0x3ffu) >> 10) - 15;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -452,12 +447,12 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos
   for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma, 0u, mb, 0u, p0[nt], p1[nt]);
 }
 
-// NT: n-tiles of 8 columns.  W: warps of the CTA.  Up to 8 columns 16 warps of at most 128
-// registers (4 a scheduler: enough to hide the latencies of a tile's dependent steps;
-// 8 warps that took 4 tiles a step ran at 37 % of the issue slots, 2.5 TB/s);
-// 16 columns need twice the accumulators and take 8 warps.
+// NT: n-tiles of 8 columns.  W: warps that compute; one more starts the copies, its lanes 2 w
+// and 2 w + 1 the two tiles of each stage of warp w.  Up to 8 columns 16 warps (4 a scheduler: enough to hide the
+// latencies of a tile's dependent steps; 8 warps that took 4 tiles a step ran at 37 % of the
+// issue slots, 2.5 TB/s); 16 columns need twice the accumulators and take 8 warps.
 template <int NT, int W, bool MASK>
-__global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams p) {
+__global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using Smem = Kv4AttnSmem<NT, W>;
   constexpr int kCols = Smem::kCols, kRing = Smem::kRing;
@@ -466,7 +461,8 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
   const int HC = p.pool.heads * p.col_blocks;
 
   // ---- the line of tiles: total, this CTA's stretch, the warps' first sequences
-  const int per_thread = (p.batch + W * 32 - 1) / (W * 32);
+  constexpr int kThreads = (W + 1) * 32;
+  const int per_thread = (p.batch + kThreads - 1) / kThreads;
   const int b_lo = tid * per_thread, b_hi = min(b_lo + per_thread, p.batch);
   int mine = 0;
   for (int b = b_lo; b < b_hi; ++b) mine += kv4_tiles(p, kv4_length(p, b)) * HC;
@@ -477,13 +473,15 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
     if (lane >= o) upto += y;
   }
   if (lane == 31) sm.scan[warp] = upto;
-  if (lane < kRing) mbar_init(&sm.bar[warp][lane], 1);
-  if (lane < 2) sm.piece[2 * warp + lane].start = -1;
+  if (warp < W) {
+    if (lane < kRing) mbar_init(&sm.full[warp][lane], 1), mbar_init(&sm.empty[warp][lane], 1);
+    if (lane < 2) sm.piece[2 * warp + lane].start = -1;
+  }
   fence_mbar_init();
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
+  for (int w = 0; w <= W; ++w) {
     if (w < warp) upto += sm.scan[w];
     total += sm.scan[w];
   }
@@ -506,56 +504,80 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
   }
   __syncthreads();
 
-  const int g0 = c0 + (int)((int64_t)width * warp / W), stretch = c0 + (int)((int64_t)width * (warp + 1) / W) - g0;
-  if (stretch > 0) {
-    Kv4Cursor use, get;
-    use.b = sm.first[warp];
+  // a warp's stretch; the last warp's lanes have the stretches of the warps they serve
+  const int who = min(warp < W ? warp : lane >> 1, W - 1);
+  const int g0 = c0 + (int)((int64_t)width * who / W), stretch = c0 + (int)((int64_t)width * (who + 1) / W) - g0;
+  Kv4Cursor use;
+  int seg_start = g0;                       // first tile of the segment at hand
+  use.left = 0;
+  if (stretch > 0 && (warp < W || lane < 2 * W)) {
+    use.b = sm.first[who];
     use.len = (int)kv4_length(p, use.b);
     use.tiles = kv4_tiles(p, use.len);
-    const unsigned off = g0 - sm.base[warp];
+    const unsigned off = g0 - sm.base[who];
     use.hc = use.tiles ? (int)(off / (unsigned)use.tiles) : 0;
     use.t = (int)(off - (unsigned)(use.hc * use.tiles));
     use.left = use.tiles ? stretch : 0;
-    get = use;
-    int seg_start = g0 - use.t;             // the segment's first tile on the line
-
-    // The copies run kRing tiles ahead.  `run` tiles are left of the page at hand: its next tile
-    // is at `src` (null: no such page), position `at` (a selected page may end before `stop`, the length).
-    const uint8_t* src = nullptr;
-    int at = 0, run = 0, stop = 0;
-    auto fetch = [&](int slot) {
-      if (run == 0) {                       // the next page
-        if (get.left <= 0) return;
-        const int in_page = get.t & (p.pool.page_tiles - 1), head = get.hc / p.col_blocks;
-        int ord = get.t >> (p.pool.page_shift - 4);
-        if (p.pages) ord = __ldg(p.pages + ((int64_t)get.b * p.pool.heads + head) * p.num_selected + ord);
-        src = nullptr;
-        if (ord >= 0 && (int64_t)ord << p.pool.page_shift < get.len) {
-          const int page = kv4_page(p.pool, p.table + get.b * p.table_stride, ord, p.width);
-          if (page >= 0) src = p.pool.tile(page, head, in_page);
-          at = (ord << p.pool.page_shift) + in_page * kKv4Tile;
-        }
-        run = min(p.pool.page_tiles - in_page, get.here());
-        stop = get.len;
-        get.advance(p, run);
-      }
-      --run;
-      if (lane == 0) {
-        const bool there = src != nullptr && at < stop;
-        sm.pos[warp][slot] = there ? at : -1;
-        if (there) {
-          mbar_arrive_expect_tx(&sm.bar[warp][slot], kKv4TileBytes);
-          bulk_g2s(sm.ring[warp][slot], src, kKv4TileBytes, &sm.bar[warp][slot]);
-        } else {
-          mbar_arrive(&sm.bar[warp][slot]);
+    seg_start -= use.t;
+  }
+  if (warp == W) {
+    // ---- copies.  The page of a lane's next tile is looked up a stage ahead, so that the block
+    // table's latency is not waited for.
+    static_assert(2 * W <= 32, "two lanes a warp");
+    const int q = lane & 1;
+    int slot = 0, parity = 1, at = 0, page = 0, tile = 0, head = 0;
+    bool more = false, there = false;       // a stage to issue; this lane's tile of it has tokens
+    auto look = [&]() {
+      more = use.left > 0;
+      there = false;
+      if (!more) return;
+      const int n = min(2, use.here()), t = use.t + q;
+      head = use.hc / p.col_blocks;
+      tile = t & (p.pool.page_tiles - 1);
+      if (q < n) {
+        int ord = t >> (p.pool.page_shift - 4);
+        if (p.pages) ord = __ldg(p.pages + ((int64_t)use.b * p.pool.heads + head) * p.num_selected + ord);
+        const int64_t pos = ((int64_t)ord << p.pool.page_shift) + tile * kKv4Tile;
+        if (ord >= 0 && pos < use.len) {    // a selected page may lie past the length, or end before it
+          at = (int)pos;
+          page = __ldg(p.table + use.b * p.table_stride + ord);
+          there = true;
         }
       }
-      src += src ? kKv4TileBytes : 0;
-      at += kKv4Tile;
+      use.advance(p, n);
     };
-#pragma unroll
-    for (int i = 0; i < kRing; ++i) fetch(i);
-
+    look();
+    unsigned long long idle_since = 0;
+    while (__any_sync(0xffffffffu, more)) {
+      bool go = more && q == 0 && mbar_test_wait(&sm.empty[who][slot], parity);
+      go = __shfl_sync(0xffffffffu, go, lane & 30);
+      if (!__any_sync(0xffffffffu, go)) {
+        const unsigned long long now = global_timer_ns();
+        if (idle_since == 0) idle_since = now;
+        if (now - idle_since > kWaitLimitNs) {
+          if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
+          break;
+        }
+        __nanosleep(40);
+        continue;
+      }
+      idle_since = 0;
+      if (go && there && (unsigned)page >= (unsigned)p.pool.num_pages) {
+        record_error(p.pool.err, kDevBadPage);
+        there = false;
+      }
+      const unsigned copies = __ballot_sync(0xffffffffu, go && there) >> (lane & 30) & 3u;
+      if (go) sm.pos[who][slot][q] = there ? at : -1;
+      __syncwarp();
+      if (go && q == 0) mbar_arrive_expect_tx(&sm.full[who][slot], __popc(copies) * kKv4TileBytes);
+      __syncwarp();
+      if (go) {
+        if (there) bulk_g2s(sm.ring[who][slot][q], p.pool.tile(page, head, tile), kKv4TileBytes, &sm.full[who][slot]);
+        if (++slot == kRing) slot = 0, parity ^= 1;
+        look();
+      }
+    }
+  } else if (use.left > 0) {
     Kv4Columns<NT> s;
     int slot = 0, parity = 0, npieces = 0;
     bool ok = true;
@@ -564,22 +586,24 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
       kv4_begin<NT>(p, s, use.b, use.hc, use.len, lane);
       const float* mrow = MASK ? p.mask + use.b * p.mask_stride : nullptr;
 #pragma unroll 1
-      for (int i = 0; i < n; ++i) {
+      for (int i = 0; i < n; i += 2) {
         // a wait that runs out is recorded; what follows waits briefly and computes on what is there
-        if (!mbar_wait(&sm.bar[warp][slot], parity, ok ? kWaitLimitNs : 1000000ull)) {
+        if (!mbar_wait(&sm.full[warp][slot], parity, ok ? kWaitLimitNs : 1000000ull)) {
           ok = false;
           if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
         }
-        const uint32_t tl = smem_u32(sm.ring[warp][slot]);
-        const int pos = sm.pos[warp][slot];
-        if (pos >= 0) {
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) {
+          const int pos = sm.pos[warp][slot][j];
+          if (pos < 0) continue;
+          const uint32_t tl = smem_u32(sm.ring[warp][slot][j]);
           if (pos + kKv4Tile > use.len - p.queries + 1)
             kv4_tile<NT, MASK, true>(s, tl, pos, use.len, mrow, p.mask_width, lane);
           else
             kv4_tile<NT, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, lane);
         }
-        __syncwarp();                       // the slot is read: its next copy may land
-        fetch(slot);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.empty[warp][slot]);   // the stage is read: its next copies may land
         if (++slot == kRing) slot = 0, parity ^= 1;
       }
 
@@ -637,7 +661,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
   // sequences without a tile: nothing to attend to
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (kv4_length(p, b) == 0)
-      for (int i = tid; i < HC * kCols * 32; i += W * 32) {
+      for (int i = tid; i < HC * kCols * 32; i += kThreads) {
         int64_t lse_at;
         const int64_t row = kv4_out_row(p, b, i / (kCols * 32), i / 32 % kCols, kCols, &lse_at);
         if (row < 0) continue;
@@ -658,7 +682,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
     todo &= ~members;
     const bool whole = pc.start >= c0 && pc.start + pc.tiles <= c1;
     float* part = p.parts + (blockIdx.x * 2 + (pc.start <= c0 ? 0 : 1)) * kKv4PartFloats;
-    for (int col = warp; col < kCols; col += W) {
+    for (int col = warp; col < kCols; col += W + 1) {
       const bool in = members >> lane & 1;
       const float base = in ? sm.part(lane)[kCols * 128 + col] : -INFINITY;
       float mx = base;
@@ -703,7 +727,7 @@ __global__ void __launch_bounds__(W * 32, 1) kv4_attn_kernel(const Kv4AttnParams
       if (tid == 0) p.counters[first] = 0;
       // the segment's piece of CTA k is its first one, but for the CTA in whose middle it starts
       const int skip = pc.start > first * per ? 1 : 0;
-      for (int col = warp; col < kCols; col += W) {
+      for (int col = warp; col < kCols; col += W + 1) {
         float mx = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k0 = 0; k0 < n; k0 += 32) {
