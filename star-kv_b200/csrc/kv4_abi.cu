@@ -253,12 +253,19 @@ int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_arg
   p.first = a->num_first;
   p.last = a->num_last;
   if ((int64_t)p.group * p.queries > 65536) return host_error(STARKV_ERR_UNSUPPORTED, "too many query columns");
-  const dim3 grid((unsigned)p.pool.heads, (unsigned)p.batch);
+  p.q_dtype = a->q_dtype;
+  if (((int64_t)a->table_width << p.pool.page_shift) > 0x7fffff00)
+    return host_error(STARKV_ERR_UNSUPPORTED, "block table of 2^31 positions or more");
   cudaStream_t st = (cudaStream_t)stream;
-  if (a->q_dtype == STARKV_F16)
-    kv4_select_kernel<__half><<<grid, 256, 0, st>>>(p);
+  const dim3 grid((unsigned)p.pool.heads, (unsigned)p.batch);
+  if (p.width > p.keep) {                   // else no sequence has pages to drop
+    const int chunk = kKv4ScoreWarps * kKv4ScorePages;
+    kv4_score_kernel<<<dim3((unsigned)((p.width + chunk - 1) / chunk), grid.x, grid.y), kKv4ScoreWarps * 32, 0, st>>>(p);
+  }
+  if (p.width <= kKv4SelThreads * kKv4SelRegs)
+    kv4_select_kernel<true><<<grid, kKv4SelThreads, 0, st>>>(p);
   else
-    kv4_select_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+    kv4_select_kernel<false><<<grid, kKv4SelThreads, 0, st>>>(p);
   return host_launch_status();
 }
 

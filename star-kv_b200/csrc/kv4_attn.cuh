@@ -776,8 +776,19 @@ struct Kv4SelectParams {
   const int* lengths;
   int* out;
   float* scores;
-  int batch, queries, q_heads, group, width, keep, first, last;
+  int q_dtype, batch, queries, q_heads, group, width, keep, first, last;
 };
+
+// Pages of a sequence, within the block table.
+__device__ __forceinline__ int kv4_pages(const Kv4SelectParams& p, int b) {
+  const int64_t cap = (int64_t)p.width << p.pool.page_shift;
+  int64_t len = __ldg(p.lengths + b);
+  if (len > cap) {
+    record_error(p.pool.err, kDevBadPosition);
+    len = cap;
+  }
+  return len <= 0 ? 0 : (int)((len + (1 << p.pool.page_shift) - 1) >> p.pool.page_shift);
+}
 
 // Order-preserving integer of a score (larger score, larger key; -0 equals 0).
 __device__ __forceinline__ uint32_t kv4_key_of(float s) {
@@ -785,93 +796,171 @@ __device__ __forceinline__ uint32_t kv4_key_of(float s) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One CTA of 256 threads per (KV head, sequence): scores, then the keep-th largest
-// key by bits, then the list in page order.
-template <typename T>
-__global__ void __launch_bounds__(256) kv4_select_kernel(const Kv4SelectParams p) {
-  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, cols = p.queries * p.group;
-  __shared__ int cnt[8];
-  __shared__ uint32_t qp[32], qn[32];
-  __shared__ float unit;
-  const int64_t cap = (int64_t)p.width << p.pool.page_shift;
-  int64_t len = p.lengths[b];
-  len = len < 0 ? 0 : len > cap ? cap : len;
-  const int n = (int)((len + (1 << p.pool.page_shift) - 1) >> p.pool.page_shift);
-  const int64_t seg = (int64_t)b * p.pool.heads + head;
-  int* out = p.out + seg * p.keep;
-  if (n <= p.keep) {
-    for (int i = tid; i < p.keep; i += 256) out[i] = i < n ? i : -1;
-    return;
+// ---- page scores: a warp takes 8 pages, a lane 4 channels of their bounds.  Per page and
+// column two dp4a (the positive codes against the upper bounds, the negative ones
+// against the lower) and one warp sum; bound by the bounds' bytes (256 a page and head).
+constexpr int kKv4ScoreWarps = 8, kKv4ScorePages = 8, kKv4ScoreCols = 16;
+
+__global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv4SelectParams p) {
+  __shared__ int pos[kKv4ScoreCols][32], neg[kKv4ScoreCols][32];
+  __shared__ float unit[kKv4ScoreCols];
+  const int head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = kv4_pages(p, b), lo = p.first, hi = n - p.last;   // the pages to score
+  const int p0 = lo + (blockIdx.x * kKv4ScoreWarps + warp) * kKv4ScorePages;
+  if (n <= p.keep || lo + (int)blockIdx.x * kKv4ScoreWarps * kKv4ScorePages >= hi) return;
+  // the pages' bounds, all in flight together
+  int page = -1;
+  if (lane < kKv4ScorePages && p0 + lane < hi) page = kv4_page(p.pool, p.table + b * p.table_stride, p0 + lane, p.width);
+  int up[kKv4ScorePages], dn[kKv4ScorePages];
+#pragma unroll
+  for (int i = 0; i < kKv4ScorePages; ++i) {
+    const int pg = __shfl_sync(0xffffffffu, page, i);
+    up[i] = dn[i] = 0;
+    if (pg >= 0) {
+      const int* bd = reinterpret_cast<const int*>(p.pool.bounds + ((int64_t)pg * p.pool.heads + head) * 256);
+      up[i] = __ldg(bd + lane);
+      dn[i] = __ldg(bd + 32 + lane);
+    }
   }
-  float* sc = p.scores + seg * p.width;
-  const int* row = p.table + b * p.table_stride;
-  for (int col = 0; col < cols; ++col) {
-    __syncthreads();
-    if (tid < 32) {
-      const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + (col / p.group) * p.qs[1] +
-                   (head * p.group + col % p.group) * p.qs[2] + tid * 4;
-      float x[4], a = 0.f;
-      for (int i = 0; i < 4; ++i) x[i] = to_f32(q[i]), a = fmaxf(a, fabsf(x[i]));
+  const float scale = page >= 0 ? __ldg(p.pool.bound_scales + (int64_t)page * p.pool.heads + head) : 0.f;
+  float best[kKv4ScorePages];
+#pragma unroll
+  for (int i = 0; i < kKv4ScorePages; ++i) best[i] = -INFINITY;
+  const int cols = p.queries * p.group;
+  for (int c0 = 0; c0 < cols; c0 += kKv4ScoreCols) {
+    const int nc = min(kKv4ScoreCols, cols - c0);
+    if (c0) __syncthreads();
+    for (int col = warp; col < nc; col += kKv4ScoreWarps) {
+      const int gc = c0 + col;
+      const int64_t at = b * p.qs[0] + (gc / p.group) * p.qs[1] + (head * p.group + gc % p.group) * p.qs[2] + lane * 4;
+      const uint2 raw = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.q) + at));
+      float x[4];
+      if (p.q_dtype == STARKV_F16) {
+        const float2 f0 = kv4_float2(raw.x), f1 = kv4_float2(raw.y);
+        x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
+      } else {
+        x[0] = __uint_as_float(raw.x << 16), x[1] = __uint_as_float(raw.x & 0xffff0000u);
+        x[2] = __uint_as_float(raw.y << 16), x[3] = __uint_as_float(raw.y & 0xffff0000u);
+      }
+      float a = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
       for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
       const float u = __fdiv_rn(a, 127.f);
       uint32_t wp = 0, wn = 0;
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = u > 0.f ? (int)rintf(__fdiv_rn(x[i], u)) : 0;
-        wp |= (uint32_t)(c > 0 ? c : 0) << (8 * i);
-        wn |= (uint32_t)((c < 0 ? c : 0) & 255) << (8 * i);
+        wp |= (uint32_t)max(c, 0) << (8 * i);
+        wn |= (uint32_t)(min(c, 0) & 255) << (8 * i);
       }
-      qp[tid] = wp;
-      qn[tid] = wn;
-      if (tid == 0) unit = u;
+      pos[col][lane] = (int)wp;
+      neg[col][lane] = (int)wn;
+      if (lane == 0) unit[col] = u;
     }
     __syncthreads();
-    for (int i = tid; i < n; i += 256) {
-      float s = -INFINITY;
-      if (i < p.first || i >= n - p.last) {
-        s = INFINITY;
-      } else {
-        const int page = kv4_page(p.pool, row, i, p.width);
-        if (page >= 0) {
-          const int* bd = reinterpret_cast<const int*>(p.pool.bounds + ((int64_t)page * p.pool.heads + head) * 256);
-          int dot = 0;
-          for (int j = 0; j < 32; ++j) dot = __dp4a((int)qp[j], bd[j], __dp4a((int)qn[j], bd[32 + j], dot));
-          s = __fmul_rn((float)dot, unit);
-          if (col > 0) s = fmaxf(s, sc[i]);
-          if (col < cols - 1) {
-            sc[i] = s;
-            continue;
-          }
-          s = __fmul_rn(s, p.pool.bound_scales[(int64_t)page * p.pool.heads + head]);
-        }
+    for (int col = 0; col < nc; ++col) {
+      const int wp = pos[col][lane], wn = neg[col][lane];
+      const float u = unit[col];
+#pragma unroll
+      for (int i = 0; i < kKv4ScorePages; ++i) {
+        const int dot = __reduce_add_sync(0xffffffffu, __dp4a(wp, up[i], __dp4a(wn, dn[i], 0)));
+        best[i] = fmaxf(best[i], __fmul_rn((float)dot, u));
       }
-      sc[i] = s;
     }
+  }
+  float mine = 0.f;
+#pragma unroll
+  for (int i = 0; i < kKv4ScorePages; ++i)
+    if (lane == i) mine = best[i];
+  if (lane < kKv4ScorePages && p0 + lane < hi)
+    p.scores[((int64_t)b * p.pool.heads + head) * p.width + p0 + lane] = page >= 0 ? __fmul_rn(mine, scale) : -INFINITY;
+}
+
+// ---- the pages kept: one CTA per (KV head, sequence).  Thread t holds the keys of the
+// pages [t * per, (t + 1) * per) (in registers up to 8 of them), the keep-th largest key is
+// found bit by bit, and two scans put the kept pages in order.
+constexpr int kKv4SelThreads = 1024, kKv4SelRegs = 8;
+
+// Sum over the threads before this one; total: over all of them.
+__device__ __forceinline__ int kv4_scan(int x, int* warps, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int y = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
   }
   __syncthreads();
-  // largest key with at least `keep` scores at or above it
-  uint32_t key = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  if (lane == 31) warps[warp] = y;
+  __syncthreads();
+  int w = warps[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += z;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  return y - x + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
+}
+
+template <bool REGS>
+__global__ void __launch_bounds__(kKv4SelThreads) kv4_select_kernel(const Kv4SelectParams p) {
+  __shared__ int count[32], warps[32];
+  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int n = kv4_pages(p, b);
+  const int64_t seg = (int64_t)b * p.pool.heads + head;
+  int* out = p.out + seg * p.keep;
+  if (n <= p.keep) {
+    for (int i = tid; i < p.keep; i += kKv4SelThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float* sc = p.scores + seg * p.width;
+  const int per = (n + kKv4SelThreads - 1) / kKv4SelThreads, i0 = min(tid * per, n), mine = min(per, n - i0);
+  auto key_at = [&](int i) { return i < p.first || i >= n - p.last ? 0xffffffffu : kv4_key_of(__ldcg(sc + i)); };
+  uint32_t held[kKv4SelRegs];
+  if (REGS) {
+#pragma unroll
+    for (int i = 0; i < kKv4SelRegs; ++i) held[i] = i < mine ? key_at(i0 + i) : 0;
+  }
+  // f(i, key) over this thread's pages
+  auto each = [&](auto f) {
+    if (REGS) {
+#pragma unroll
+      for (int i = 0; i < kKv4SelRegs; ++i)
+        if (i < mine) f(i0 + i, held[i]);
+    } else {
+      for (int i = 0; i < mine; ++i) f(i0 + i, key_at(i0 + i));
+    }
+  };
+  if (tid < 32) count[tid] = 0;
+  __syncthreads();
+  uint32_t key = 0;                         // the largest key with at least `keep` keys >= it
+  bool exact = false;                       // exactly `keep`
+  for (int bit = 31; bit >= 0 && !exact; --bit) {
     const uint32_t trial = key | (1u << bit);
     int c = 0;
-    for (int i = tid; i < n; i += 256) c += kv4_key_of(sc[i]) >= trial;
+    each([&](int, uint32_t k) { c += k >= trial; });
     c = __reduce_add_sync(0xffffffffu, c);
-    if ((tid & 31) == 0) cnt[tid >> 5] = c;
+    if ((tid & 31) == 0 && c) atomicAdd(&count[bit], c);
     __syncthreads();
-    c = 0;
-    for (int i = 0; i < 8; ++i) c += cnt[i];
+    c = count[bit];
     if (c >= p.keep) key = trial;
-    __syncthreads();
+    exact = c == p.keep;
   }
-  if (tid == 0) {
-    int above = 0, at = 0;
-    for (int i = 0; i < n; ++i) above += kv4_key_of(sc[i]) > key;
-    int equal = p.keep - above;
-    for (int i = 0; i < n && at < p.keep; ++i) {
-      const uint32_t k = kv4_key_of(sc[i]);
-      if (k > key || (k == key && equal-- > 0)) out[at++] = i;
-    }
-    for (; at < p.keep; ++at) out[at] = -1;
+  int above = 0, equal = 0, total = 0;
+  each([&](int, uint32_t k) { above += k > key, equal += k == key; });
+  int ties = 0x7fffffff, taken = 0;         // equal keys still to take, and those of earlier threads
+  if (!exact) {
+    taken = kv4_scan(equal, warps, &total);
+    int all_above;
+    kv4_scan(above, warps, &all_above);
+    ties = p.keep - all_above;
   }
+  const int left = max(0, min(equal, ties - taken));
+  int at = kv4_scan(above + left, warps, &total), use = left;
+  each([&](int i, uint32_t k) {
+    if (k > key || (k == key && use-- > 0)) out[at++] = i;
+  });
 }
 
 }  // namespace starkv
