@@ -189,9 +189,8 @@ struct Kv4AttnSmem {
   int pos[W][kRing][2];                     // position of a tile's first token, -1: nothing to attend to
   Kv4Piece piece[2 * W];
   int scan[W + 1];
-  int base[W];                              // first tile of the warp's first sequence
-  int first[W];                             // that sequence
-  int last;
+  int upto[(W + 1) * 32];                   // tiles of the sequences up to and with a thread's
+  int last[2];
   // piece i: o (cols, 128), base (cols), l (cols).  The first piece of a warp has its own space,
   // the second lies over the warp's ring.
   __device__ __forceinline__ float* part(int i) {
@@ -297,19 +296,28 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
   s.e = 0;
 }
 
-// One tile at shared address tl.  MASK: an additive mask (mrow, its row).  EDGE: some of the
-// tile's positions are beyond what a column attends to, or beyond the length.
-template <int NT, bool MASK, bool EDGE>
-__device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos, int len, const float* mrow,
-                                         int64_t mask_width, int lane) {
+// TILES consecutive tiles at shared address tl.  MASK: an additive mask (mrow, its row).  EDGE:
+// some of their positions are beyond what a column attends to, or beyond the length.
+template <int NT, int TILES, bool MASK, bool EDGE>
+__device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, int pos, int len, const float* mrow,
+                                               int64_t mask_width, int lane) {
   const int r = lane >> 2, c = lane & 3;
-  const uint4 ka = kv4_lds128(tl + r * 64 + c * 16), kb = kv4_lds128(tl + r * 64 + c * 16 + 512);
-  const uint4 pa = kv4_lds128(tl + kKv4KParams + r * 16), pb = kv4_lds128(tl + kKv4KParams + r * 16 + 128);
-  const uint4 va = kv4_lds128(tl + kKv4VCodes + c * 128 + r * 16), vb = kv4_lds128(tl + kKv4VCodes + c * 128 + r * 16 + 512);
-  uint4 ta = kv4_lds128(tl + kKv4VParams + c * 32), tb = kv4_lds128(tl + kKv4VParams + c * 32 + 128);
-  // ---- scores
-  float x[NT][4];
-  {
+  float x[TILES][NT][4];
+  uint4 ta[TILES], tb[TILES];
+  uint32_t keep_a[TILES], keep_b[TILES];    // halves of the value parameters that count
+  bool over = false;
+  // an s above 2^e (the bits of positive fp16 numbers order like integers)
+  const uint32_t lim = (uint32_t)(15 + s.e) * 0x04000400u;
+  uint32_t big = lim;
+#pragma unroll
+  for (int h = 0; h < TILES; ++h) {
+    const uint32_t at = tl + h * kKv4TileBytes;
+    const int p0 = pos + h * kKv4Tile;
+    // ---- scores
+    const uint4 ka = kv4_lds128(at + r * 64 + c * 16), kb = kv4_lds128(at + r * 64 + c * 16 + 512);
+    const uint4 pa = kv4_lds128(at + kKv4KParams + r * 16), pb = kv4_lds128(at + kKv4KParams + r * 16 + 128);
+    ta[h] = kv4_lds128(at + kKv4VParams + c * 32);
+    tb[h] = kv4_lds128(at + kKv4VParams + c * 32 + 128);
     const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
     const float2 sa01 = kv4_float2(pa.x), sa23 = kv4_float2(pa.y), sb01 = kv4_float2(pb.x), sb23 = kv4_float2(pb.y);
     const float sa[4] = {sa01.x, sa01.y, sa23.x, sa23.y}, sb[4] = {sb01.x, sb01.y, sb23.x, sb23.y};
@@ -322,70 +330,69 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos
         kv4_mma0(d, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, s.qb[nt][j][0],
                  s.qb[nt][j][1]);
         kv4_mma(d, ua & 0x000f000fu, ub & 0x000f000fu, ua & 0x00f000f0u, ub & 0x00f000f0u, s.qb[nt][j][2], s.qb[nt][j][3]);
-        x[nt][0] = j ? fmaf(sa[j], d[0], x[nt][0]) : sa[j] * d[0];
-        x[nt][1] = j ? fmaf(sa[j], d[1], x[nt][1]) : sa[j] * d[1];
-        x[nt][2] = j ? fmaf(sb[j], d[2], x[nt][2]) : sb[j] * d[2];
-        x[nt][3] = j ? fmaf(sb[j], d[3], x[nt][3]) : sb[j] * d[3];
+        x[h][nt][0] = j ? fmaf(sa[j], d[0], x[h][nt][0]) : sa[j] * d[0];
+        x[h][nt][1] = j ? fmaf(sa[j], d[1], x[h][nt][1]) : sa[j] * d[1];
+        x[h][nt][2] = j ? fmaf(sb[j], d[2], x[h][nt][2]) : sb[j] * d[2];
+        x[h][nt][3] = j ? fmaf(sb[j], d[3], x[h][nt][3]) : sb[j] * d[3];
       }
     }
-  }
-  unsigned live = 0xffffu;                  // MASK: tokens that are not masked out
-  float add0 = 0.f, add1 = 0.f;
-  if (MASK) {
-    const int t0 = pos + r, t1 = t0 + 8;
-    if (t0 < len && t0 < mask_width) add0 = __ldg(mrow + t0);
-    if (t1 < len && t1 < mask_width) add1 = __ldg(mrow + t1);
-    // one bit a token: lanes c = 0 and c = 1 of row r hold tokens r and r + 8
-    const unsigned votes = __ballot_sync(0xffffffffu, (c == 0 ? add0 : add1) != -INFINITY);
-    live = 0;
-#pragma unroll
-    for (int t = 0; t < 16; ++t) live |= ((votes >> (4 * (t & 7) + (t >> 3))) & 1u) << t;
-    // beyond -2.3e38 the sum would leave fp32 in the log2 domain
-    add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
-    add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
-  }
-  const uint32_t m0 = c & 1 ? pa.w : pa.z, m1 = c & 1 ? pb.w : pb.z, s0 = c & 1 ? pa.y : pa.x, s1 = c & 1 ? pb.y : pb.x;
-  bool over = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float d[4];
-    kv4_mma0(d, m0, m1, s0, s1, s.qc[nt][0], s.qc[nt][1]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float y = fmaf(x[nt][u], 0x1p17f, d[u]);    // an eighth of the column's score
-      if (MASK) {
-        const float add = u & 2 ? add1 : add0;
-        y = add == -INFINITY ? -INFINITY : fmaf(y, s.cs[nt][u & 1], add);
-      }
-      if (EDGE && pos + r + (u & 2 ? 8 : 0) >= s.end[nt][u & 1]) y = -INFINITY;
-      x[nt][u] = y;
-    }
-    over |= fmaxf(x[nt][0], x[nt][2]) > s.thr[nt][0];
-    over |= fmaxf(x[nt][1], x[nt][3]) > s.thr[nt][1];
-  }
-  // ---- value parameters
-  uint32_t ma = 0, mb = 0;
-  if (r < 4) {
-    ma = kv4_lds32(tl + kKv4VParams + 16 + c * 32 + r * 4);
-    mb = kv4_lds32(tl + kKv4VParams + 16 + c * 32 + r * 4 + 128);
-  }
-  if (MASK || EDGE) {                       // tokens that do not count may hold anything
-    const int t = pos + 2 * c;
-    uint32_t la = (t < len ? 0xffffu : 0u) | (t + 1 < len ? 0xffff0000u : 0u);
-    uint32_t lb = (t + 8 < len ? 0xffffu : 0u) | (t + 9 < len ? 0xffff0000u : 0u);
+    unsigned live = 0xffffu;                // MASK: tokens that are not masked out
+    float add0 = 0.f, add1 = 0.f;
     if (MASK) {
-      const unsigned ba = live >> (2 * c), bb = live >> (2 * c + 8);
-      la &= (ba & 1 ? 0xffffu : 0u) | (ba & 2 ? 0xffff0000u : 0u);
-      lb &= (bb & 1 ? 0xffffu : 0u) | (bb & 2 ? 0xffff0000u : 0u);
+      const int t0 = p0 + r, t1 = t0 + 8;
+      if (t0 < len && t0 < mask_width) add0 = __ldg(mrow + t0);
+      if (t1 < len && t1 < mask_width) add1 = __ldg(mrow + t1);
+      // one bit a token: lanes c = 0 and c = 1 of row r hold tokens r and r + 8
+      const unsigned votes = __ballot_sync(0xffffffffu, (c == 0 ? add0 : add1) != -INFINITY);
+      live = 0;
+#pragma unroll
+      for (int t = 0; t < 16; ++t) live |= ((votes >> (4 * (t & 7) + (t >> 3))) & 1u) << t;
+      // beyond -2.3e38 the sum would leave fp32 in the log2 domain
+      add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
+      add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
     }
-    ta.x &= la, ta.y &= la, ta.z &= la, ta.w &= la, ma &= la;
-    tb.x &= lb, tb.y &= lb, tb.z &= lb, tb.w &= lb, mb &= lb;
+    const uint32_t m0 = c & 1 ? pa.w : pa.z, m1 = c & 1 ? pb.w : pb.z, s0 = c & 1 ? pa.y : pa.x, s1 = c & 1 ? pb.y : pb.x;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float d[4];
+      kv4_mma0(d, m0, m1, s0, s1, s.qc[nt][0], s.qc[nt][1]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float y = fmaf(x[h][nt][u], 0x1p17f, d[u]);   // an eighth of the column's score
+        if (MASK) {
+          const float add = u & 2 ? add1 : add0;
+          y = add == -INFINITY ? -INFINITY : fmaf(y, s.cs[nt][u & 1], add);
+        }
+        if (EDGE && p0 + r + (u & 2 ? 8 : 0) >= s.end[nt][u & 1]) y = -INFINITY;
+        x[h][nt][u] = y;
+      }
+    }
+    if (MASK || EDGE) {                     // tokens that do not count may hold anything
+      const int t = p0 + 2 * c;
+      uint32_t la = (t < len ? 0xffffu : 0u) | (t + 1 < len ? 0xffff0000u : 0u);
+      uint32_t lb = (t + 8 < len ? 0xffffu : 0u) | (t + 9 < len ? 0xffff0000u : 0u);
+      if (MASK) {
+        const unsigned ba = live >> (2 * c), bb = live >> (2 * c + 8);
+        la &= (ba & 1 ? 0xffffu : 0u) | (ba & 2 ? 0xffff0000u : 0u);
+        lb &= (bb & 1 ? 0xffffu : 0u) | (bb & 2 ? 0xffff0000u : 0u);
+      }
+      ta[h].x &= la, ta[h].y &= la, ta[h].z &= la, ta[h].w &= la;
+      tb[h].x &= lb, tb[h].y &= lb, tb[h].z &= lb, tb[h].w &= lb;
+      keep_a[h] = la;
+      keep_b[h] = lb;
+    }
+    big = __vimax3_u16x2(big, __vimax3_u16x2(ta[h].x, ta[h].y, ta[h].z),
+                         __vimax3_u16x2(ta[h].w, tb[h].x, __vimax3_u16x2(tb[h].y, tb[h].z, tb[h].w)));
   }
-  // an s above 2^e in either half (the bits of positive fp16 numbers order like integers)
-  const uint32_t lim = (uint32_t)(15 + s.e) * 0x04000400u;
-  const uint32_t big = __vimax3_u16x2(__vimax3_u16x2(ta.x, ta.y, ta.z), __vimax3_u16x2(ta.w, tb.x, tb.y),
-                                      __vimax3_u16x2(tb.z, tb.w, lim));
-  over |= big != lim;
+  over = big != lim;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float t = fmaxf(x[0][nt][u], x[0][nt][u + 2]);
+      if (TILES == 2) t = fmaxf(t, fmaxf(x[TILES - 1][nt][u], x[TILES - 1][nt][u + 2]));
+      over |= t > s.thr[nt][u];
+    }
   // ---- a score or an s that the base does not cover
   if (__any_sync(0xffffffffu, over)) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
@@ -394,7 +401,8 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float t = fmaxf(x[nt][u], x[nt][u + 2]);
+        float t = fmaxf(x[0][nt][u], x[0][nt][u + 2]);
+        if (TILES == 2) t = fmaxf(t, fmaxf(x[TILES - 1][nt][u], x[TILES - 1][nt][u + 2]));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
@@ -416,35 +424,46 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, uint32_t tl, int pos
     s.e = e_new;
   }
   // ---- weights and values
-  uint32_t p0[NT], p1[NT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    float w[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      w[u] = kv4_exp2(MASK ? x[nt][u] - s.base[nt][u & 1] : fmaf(x[nt][u], s.cs[nt][u & 1], -s.base[nt][u & 1]));
-    s.l[nt][0] += w[0] + w[2];
-    s.l[nt][1] += w[1] + w[3];
-    p0[nt] = kv4_transpose(kv4_half2(w[0], w[1]));
-    p1[nt] = kv4_transpose(kv4_half2(w[2], w[3]));
-  }
-  const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-  const uint32_t sa[4] = {ta.x, ta.y, ta.z, ta.w}, sb[4] = {tb.x, tb.y, tb.z, tb.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t ua = wa[j] >> 8, ub = wb[j] >> 8;
+  for (int h = 0; h < TILES; ++h) {
+    const uint32_t at = tl + h * kKv4TileBytes;
+    const uint4 va = kv4_lds128(at + kKv4VCodes + c * 128 + r * 16), vb = kv4_lds128(at + kKv4VCodes + c * 128 + r * 16 + 512);
+    uint32_t ma = 0, mb = 0;
+    if (r < 4) {
+      ma = kv4_lds32(at + kKv4VParams + 16 + c * 32 + r * 4);
+      mb = kv4_lds32(at + kKv4VParams + 16 + c * 32 + r * 4 + 128);
+    }
+    if (MASK || EDGE) ma &= keep_a[h], mb &= keep_b[h];
+    uint32_t p0[NT], p1[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t b0 = kv4_hmul2(p0[nt], sa[j]), b1 = kv4_hmul2(p1[nt], sb[j]);
-      kv4_mma(s.o[2 * j][nt], wa[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x000f000fu, wb[j] & 0x00f000f0u, b0, b1);
-      kv4_mma(s.o[2 * j + 1][nt], ua & 0x000f000fu, ua & 0x00f000f0u, ub & 0x000f000fu, ub & 0x00f000f0u, b0, b1);
-      // -8 * 2^-24 in rows r, -8 * 2^-20 in rows r + 8
-      kv4_mma(s.o[2 * j][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-      kv4_mma(s.o[2 * j + 1][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-    }
-  }
+      float w[4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma, 0u, mb, 0u, p0[nt], p1[nt]);
+      for (int u = 0; u < 4; ++u)
+        w[u] = kv4_exp2(MASK ? x[h][nt][u] - s.base[nt][u & 1] : fmaf(x[h][nt][u], s.cs[nt][u & 1], -s.base[nt][u & 1]));
+      s.l[nt][0] += w[0] + w[2];
+      s.l[nt][1] += w[1] + w[3];
+      p0[nt] = kv4_transpose(kv4_half2(w[0], w[1]));
+      p1[nt] = kv4_transpose(kv4_half2(w[2], w[3]));
+    }
+    const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+    const uint32_t sa[4] = {ta[h].x, ta[h].y, ta[h].z, ta[h].w}, sb[4] = {tb[h].x, tb[h].y, tb[h].z, tb[h].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t ua = wa[j] >> 8, ub = wb[j] >> 8;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t b0 = kv4_hmul2(p0[nt], sa[j]), b1 = kv4_hmul2(p1[nt], sb[j]);
+        kv4_mma(s.o[2 * j][nt], wa[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x000f000fu, wb[j] & 0x00f000f0u, b0, b1);
+        kv4_mma(s.o[2 * j + 1][nt], ua & 0x000f000fu, ua & 0x00f000f0u, ub & 0x000f000fu, ub & 0x00f000f0u, b0, b1);
+        // -8 * 2^-24 in rows r, -8 * 2^-20 in rows r + 8
+        kv4_mma(s.o[2 * j][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+        kv4_mma(s.o[2 * j + 1][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma, 0u, mb, 0u, p0[nt], p1[nt]);
+  }
 }
 
 // NT: n-tiles of 8 columns.  W: warps that compute; one more starts the copies, its lanes 2 w
@@ -456,6 +475,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   extern __shared__ __align__(128) uint8_t smem_raw[];
   using Smem = Kv4AttnSmem<NT, W>;
   constexpr int kCols = Smem::kCols, kRing = Smem::kRing;
+  constexpr bool kPair = false;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int HC = p.pool.heads * p.col_blocks;
@@ -485,36 +505,35 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     if (w < warp) upto += sm.scan[w];
     total += sm.scan[w];
   }
+  sm.upto[tid] = upto;
   // equal stretches, a tile a warp at least
   const int per = max((int)((unsigned)(total + gridDim.x - 1) / gridDim.x), W);
   const int c0 = (int)min((int64_t)blockIdx.x * per, (int64_t)total), c1 = min(c0 + per, total), width = c1 - c0;
-  if (mine > 0 && upto > c0 && upto - mine < c1) {
-    int base = upto - mine, b = b_lo;
-    int n = kv4_tiles(p, kv4_length(p, b)) * HC;
-    for (int w = 0; w < W; ++w) {
-      const int g = c0 + (int)((int64_t)width * w / W);
-      if (g < upto - mine || g >= upto) continue;
-      while (g >= base + n && b + 1 < b_hi) {
-        base += n;
-        n = kv4_tiles(p, kv4_length(p, ++b)) * HC;
-      }
-      sm.first[w] = b;
-      sm.base[w] = base;
-    }
-  }
   __syncthreads();
 
   // a warp's stretch; the last warp's lanes have the stretches of the warps they serve
   const int who = min(warp < W ? warp : lane >> 1, W - 1);
-  const int g0 = c0 + (int)((int64_t)width * who / W), stretch = c0 + (int)((int64_t)width * (who + 1) / W) - g0;
+  const int g0 = c0 + width / W * who + width % W * who / W;
+  const int stretch = c0 + width / W * (who + 1) + width % W * (who + 1) / W - g0;
   Kv4Cursor use;
   int seg_start = g0;                       // first tile of the segment at hand
   use.left = 0;
   if (stretch > 0 && (warp < W || lane < 2 * W)) {
-    use.b = sm.first[who];
+    int lo = 0, hi = kThreads - 1;          // the first thread whose sequences reach beyond g0
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.upto[mid] > g0) hi = mid;
+      else lo = mid + 1;
+    }
+    unsigned off = g0 - (lo ? sm.upto[lo - 1] : 0);
+    use.b = min(lo * per_thread, p.batch - 1);
     use.len = (int)kv4_length(p, use.b);
     use.tiles = kv4_tiles(p, use.len);
-    const unsigned off = g0 - sm.base[who];
+    while (off >= (unsigned)(use.tiles * HC) && use.b + 1 < p.batch) {
+      off -= use.tiles * HC;
+      use.len = (int)kv4_length(p, ++use.b);
+      use.tiles = kv4_tiles(p, use.len);
+    }
     use.hc = use.tiles ? (int)(off / (unsigned)use.tiles) : 0;
     use.t = (int)(off - (unsigned)(use.hc * use.tiles));
     use.left = use.tiles ? stretch : 0;
@@ -592,15 +611,20 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
           ok = false;
           if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
         }
+        const int pos = sm.pos[warp][slot][0], pos1 = sm.pos[warp][slot][1], bound = use.len - p.queries + 1;
+        const uint32_t tl = smem_u32(sm.ring[warp][slot][0]);
+        if (kPair && pos >= 0 && pos1 == pos + kKv4Tile && pos + 2 * kKv4Tile <= bound) {
+          kv4_tiles_step<NT, 2, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, lane);
+        } else {
 #pragma unroll 1
-        for (int j = 0; j < 2; ++j) {
-          const int pos = sm.pos[warp][slot][j];
-          if (pos < 0) continue;
-          const uint32_t tl = smem_u32(sm.ring[warp][slot][j]);
-          if (pos + kKv4Tile > use.len - p.queries + 1)
-            kv4_tile<NT, MASK, true>(s, tl, pos, use.len, mrow, p.mask_width, lane);
-          else
-            kv4_tile<NT, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, lane);
+          for (int j = 0; j < 2; ++j) {
+            const int at = j ? pos1 : pos;
+            if (at < 0) continue;
+            if (at + kKv4Tile > bound || kPair)
+              kv4_tiles_step<NT, 1, MASK, true>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, lane);
+            else
+              kv4_tiles_step<NT, 1, MASK, false>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, lane);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.empty[warp][slot]);   // the stage is read: its next copies may land
@@ -617,6 +641,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int col = nt * 8 + 2 * c + u;
+          const bool real = (use.hc % p.col_blocks) * kCols + col < p.group * p.queries;
           float l = s.l[nt][u];
           l += __shfl_xor_sync(0xffffffffu, l, 4);
           l += __shfl_xor_sync(0xffffffffu, l, 8);
@@ -638,10 +663,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
                 fmaf(s.o[2 * j][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j][nt][u + 2], 0x1p20f, y) * inv,
                 fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y) * inv);
             const int d = j * 32 + 4 * r;
-            if (!whole)
-              *reinterpret_cast<float4*>(part + col * 128 + d) = v;
-            else if (row >= 0)
+            if (!whole) {
+              if (real) *reinterpret_cast<float4*>(part + col * 128 + d) = v;
+            } else if (row >= 0) {
               kv4_store4(p, row + d, v);
+            }
           }
         }
       if (!whole) {
@@ -671,18 +697,25 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   if (c0 >= c1) return;
   __syncthreads();
 
-  // ---- merge the pieces of each segment, in line order: a warp a column, a lane a piece for
-  // the weights, then a lane 4 channels
+  // ---- merge the pieces of each segment, in line order.  A warp takes a (segment, column): a
+  // lane a piece for the weights, then a lane 4 channels.  What is not whole here goes to the
+  // workspace: at most the CTA's first and last segment.
   static_assert(2 * W <= 32, "a lane a piece");
   const int my_start = lane < 2 * W ? sm.piece[lane].start : -1;
-  unsigned todo = __ballot_sync(0xffffffffu, my_start >= 0);
-  while (todo) {
-    const Kv4Piece pc = sm.piece[__ffs(todo) - 1];
+  const unsigned pieces = __ballot_sync(0xffffffffu, my_start >= 0);
+  int unit = 0, cross[2] = {-1, -1};        // cross: a piece of the segments that other CTAs share
+  for (unsigned todo = pieces; todo;) {
+    const int one = __ffs(todo) - 1;
+    const Kv4Piece pc = sm.piece[one];
     const unsigned members = __ballot_sync(0xffffffffu, my_start == pc.start);
     todo &= ~members;
     const bool whole = pc.start >= c0 && pc.start + pc.tiles <= c1;
-    float* part = p.parts + (blockIdx.x * 2 + (pc.start <= c0 ? 0 : 1)) * kKv4PartFloats;
-    for (int col = warp; col < kCols; col += W + 1) {
+    const int side = pc.start <= c0 ? 0 : 1;
+    if (!whole) cross[side] = one;
+    float* part = p.parts + ((int64_t)blockIdx.x * 2 + side) * kKv4PartFloats;
+    const int cols = min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols);
+    for (int col = 0; col < cols; ++col) {
+      if (unit++ % (W + 1) != warp) continue;
       const bool in = members >> lane & 1;
       const float base = in ? sm.part(lane)[kCols * 128 + col] : -INFINITY;
       float mx = base;
@@ -703,11 +736,9 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       if (whole) {
         int64_t lse_at;
         const int64_t row = kv4_out_row(p, pc.b, pc.hc, col, kCols, &lse_at);
-        if (row >= 0) {
-          const float inv = kv4_inverse(l);
-          kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-          if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
-        }
+        const float inv = kv4_inverse(l);
+        kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
       } else {
         __stcg(reinterpret_cast<float4*>(part + col * 128 + lane * 4), acc);
         if (lane == 0) {
@@ -716,54 +747,63 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
         }
       }
     }
-    if (whole) continue;
+  }
+  if (cross[0] < 0 && cross[1] < 0) return; // the same for every warp
+  __threadfence();
+  __syncthreads();
+  if (tid < 2 && cross[tid] >= 0) {
+    const Kv4Piece pc = sm.piece[cross[tid]];
     const int first = pc.start / per, n = (pc.start + pc.tiles - 1) / per - first + 1;
+    const bool last = atomicAdd(p.counters + first, 1) == n - 1;
+    sm.last[tid] = last;
+    if (last) p.counters[first] = 0;
+  }
+  __syncthreads();
+  unit = 0;
+#pragma unroll 1
+  for (int side = 0; side < 2; ++side) {
+    if (cross[side] < 0 || !sm.last[side]) continue;
+    // every CTA's piece is there.  The segment's piece of a CTA is its first one, but for the CTA
+    // in whose middle it starts
     __threadfence();
-    __syncthreads();
-    if (tid == 0) sm.last = atomicAdd(p.counters + first, 1) == n - 1;
-    __syncthreads();
-    if (sm.last) {                          // every CTA's piece is there
-      __threadfence();
-      if (tid == 0) p.counters[first] = 0;
-      // the segment's piece of CTA k is its first one, but for the CTA in whose middle it starts
-      const int skip = pc.start > first * per ? 1 : 0;
-      for (int col = warp; col < kCols; col += W + 1) {
-        float mx = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k0 = 0; k0 < n; k0 += 32) {
-          const int k = k0 + lane;
-          const float* pk = p.parts + ((int64_t)(first + k) * 2 + (k == 0 ? skip : 0)) * kKv4PartFloats;
-          const float base = k < n ? __ldcg(pk + kCols * 128 + col) : -INFINITY;
-          const float lk = k < n ? __ldcg(pk + kCols * 129 + col) : 0.f;
-          float joint = fmaxf(mx, base);
+    const Kv4Piece pc = sm.piece[cross[side]];
+    const int first = pc.start / per, n = (pc.start + pc.tiles - 1) / per - first + 1;
+    const int skip = pc.start > first * per ? 1 : 0;
+    const int cols = min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols);
+    for (int col = 0; col < cols; ++col) {
+      if (unit++ % (W + 1) != warp) continue;
+      float mx = -INFINITY, l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < n; k0 += 32) {
+        const int k = k0 + lane;
+        const float* pk = p.parts + ((int64_t)(first + k) * 2 + (k == 0 ? skip : 0)) * kKv4PartFloats;
+        const float base = k < n ? __ldcg(pk + kCols * 128 + col) : -INFINITY;
+        const float lk = k < n ? __ldcg(pk + kCols * 129 + col) : 0.f;
+        float joint = fmaxf(mx, base);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) joint = fmaxf(joint, __shfl_xor_sync(0xffffffffu, joint, o));
-          const float w = kv4_weight(base, joint), old = kv4_weight(mx, joint);
-          float sum = k < n ? w * lk : 0.f;
+        for (int o = 16; o > 0; o >>= 1) joint = fmaxf(joint, __shfl_xor_sync(0xffffffffu, joint, o));
+        const float w = kv4_weight(base, joint), old = kv4_weight(mx, joint);
+        float sum = k < n ? w * lk : 0.f;
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          l = l * old + sum;
-          acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
-          mx = joint;
-          const int last = min(32, n - k0);
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = l * old + sum;
+        acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+        mx = joint;
+        const int count = min(32, n - k0);
 #pragma unroll 8
-          for (int i = 0; i < last; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(
-                p.parts + ((int64_t)(first + k0 + i) * 2 + (k0 + i == 0 ? skip : 0)) * kKv4PartFloats + col * 128 + lane * 4));
-            acc.x = fmaf(wi, v.x, acc.x), acc.y = fmaf(wi, v.y, acc.y), acc.z = fmaf(wi, v.z, acc.z), acc.w = fmaf(wi, v.w, acc.w);
-          }
-        }
-        int64_t lse_at;
-        const int64_t row = kv4_out_row(p, pc.b, pc.hc, col, kCols, &lse_at);
-        if (row >= 0) {
-          const float inv = kv4_inverse(l);
-          kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-          if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
+        for (int i = 0; i < count; ++i) {
+          const float wi = __shfl_sync(0xffffffffu, w, i);
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(
+              p.parts + ((int64_t)(first + k0 + i) * 2 + (k0 + i == 0 ? skip : 0)) * kKv4PartFloats + col * 128 + lane * 4));
+          acc.x = fmaf(wi, v.x, acc.x), acc.y = fmaf(wi, v.y, acc.y), acc.z = fmaf(wi, v.z, acc.z), acc.w = fmaf(wi, v.w, acc.w);
         }
       }
+      int64_t lse_at;
+      const int64_t row = kv4_out_row(p, pc.b, pc.hc, col, kCols, &lse_at);
+      const float inv = kv4_inverse(l);
+      kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+      if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
     }
-    __syncthreads();
   }
 }
 
