@@ -309,8 +309,9 @@ int starkv_prefill_attention(const starkv_prefill_args* args, starkv_stream_t st
  *   [0, 1024)     key codes: channel d of token t is nibble d % 8 of the 32-bit word
  *                 at t * 64 + (d % 32 / 8) * 16 + (d / 32) * 4
  *   [1024, 2048)  value codes: nibble d % 4 of the 16-bit word at
- *                 1024 + (t / 2) * 128 + (d % 32 / 4) * 16 + (d / 32) * 4 + (t % 2) * 2
- *   [2048, 2304)  key parameters, fp16: s of group g at 2048 + t * 16 + g * 2, m 8 bytes on
+ *                 1024 + (t / 8) * 512 + (d % 32 / 4) * 64 + (t / 2 % 4) * 16 + (d / 32) * 4 + (t % 2) * 2
+ *   [2048, 2304)  key parameters, fp16: s of group g at
+ *                 2048 + (t % 8) * 32 + (g / 2) * 16 + (t / 8) * 4 + (g % 2) * 2, m 8 bytes on
  *   [2304, 2560)  value parameters, fp16: s of group g at
  *                 2304 + (t / 2) * 32 + g * 4 + (t % 2) * 2, m 16 bytes on
  *   (the order in which the attention kernel's matrix instructions take them: one

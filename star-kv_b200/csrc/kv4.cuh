@@ -42,6 +42,17 @@ __device__ __forceinline__ int kv4_page(const Kv4Pool& pool, const int* __restri
   return page;
 }
 
+// Byte offsets within a tile (starkv.h): the s of a token's group in the key parameters (m: 8
+// bytes on) and in the value parameters (m: 16 bytes on), and the 16-bit word of four channels
+// (quad of a group) of its value codes.
+__host__ __device__ constexpr int kv4_kparam(int t, int g) {
+  return kKv4KParams + (t & 7) * 32 + (g >> 1) * 16 + (t >> 3) * 4 + (g & 1) * 2;
+}
+__host__ __device__ constexpr int kv4_vparam(int t, int g) { return kKv4VParams + (t >> 1) * 32 + g * 4 + (t & 1) * 2; }
+__host__ __device__ constexpr int kv4_vcode(int t, int g, int quad) {
+  return kKv4VCodes + (t >> 3) * 512 + quad * 64 + (t >> 1 & 3) * 16 + g * 4 + (t & 1) * 2;
+}
+
 struct Kv4IoParams {
   Kv4Pool pool;
   const void* k;
@@ -188,7 +199,7 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
       kx[it].get(f);
       uint32_t w = kv4_quantise8(f, s, m);
       uint32_t* kw = reinterpret_cast<uint32_t*>(tile + tt * 64 + c * 16 + g * 4);
-      __half* kpar = reinterpret_cast<__half*>(tile + kKv4KParams + tt * 16) + g;
+      __half* kpar = reinterpret_cast<__half*>(tile + kv4_kparam(tt, g));
       if (mine) {
         *kw = w;
         if (c == 0) kpar[0] = s, kpar[4] = m;
@@ -211,19 +222,18 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
       const uint32_t pw = kv4_pair_word(w, half);
       const uint32_t sm = (uint32_t)__half_as_ushort(s) | ((uint32_t)__half_as_ushort(m) << 16);
       const uint32_t so = __shfl_xor_sync(0xffffffffu, sm, 16);
-      uint8_t* vrow = tile + kKv4VCodes + it * 128 + g * 4;
-      uint8_t* vpar = tile + kKv4VParams + it * 32 + g * 4;
       const int te = t0 + 2 * it;
       if (te >= lo && te + 1 < hi) {
-        *reinterpret_cast<uint32_t*>(vrow + (2 * c + half) * 16) = pw;
+        *reinterpret_cast<uint32_t*>(tile + kv4_vcode(2 * it, g, 2 * c + half)) = pw;
         if (c == 0)
-          *reinterpret_cast<uint32_t*>(vpar + half * 16) = half ? __byte_perm(so, sm, 0x7632) : __byte_perm(sm, so, 0x5410);
+          *reinterpret_cast<uint32_t*>(tile + kv4_vparam(2 * it, g) + half * 16) =
+              half ? __byte_perm(so, sm, 0x7632) : __byte_perm(sm, so, 0x5410);
       } else if (mine) {                                       // the pair's other token is not this call's
-        *reinterpret_cast<uint16_t*>(vrow + 2 * c * 16 + half * 2) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(vrow + (2 * c + 1) * 16 + half * 2) = (uint16_t)(w >> 16);
+        *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, 2 * c)) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, 2 * c + 1)) = (uint16_t)(w >> 16);
         if (c == 0) {
-          *reinterpret_cast<__half*>(vpar + half * 2) = s;
-          *reinterpret_cast<__half*>(vpar + 16 + half * 2) = m;
+          *reinterpret_cast<__half*>(tile + kv4_vparam(tt, g)) = s;
+          *reinterpret_cast<__half*>(tile + kv4_vparam(tt, g) + 16) = m;
         }
       }
     }
@@ -328,13 +338,12 @@ __global__ void __launch_bounds__(kKv4ReadWarps * 32) kv4_read_kernel(const Kv4I
     if (i < 0 || i >= p.num_tokens) continue;
     float fk[8], fv[8];
     if (page >= 0 && i < count) {
-      const __half* kpar = reinterpret_cast<const __half*>(tile + kKv4KParams + tt * 16) + g;
+      const __half* kpar = reinterpret_cast<const __half*>(tile + kv4_kparam(tt, g));
       kv4_values8(*reinterpret_cast<const uint32_t*>(tile + tt * 64 + c * 16 + g * 4), __half2float(kpar[0]),
                   __half2float(kpar[4]), fk);
-      const uint8_t* vrow = tile + kKv4VCodes + it * 128 + g * 4 + half * 2;
-      const uint32_t w = (uint32_t)*reinterpret_cast<const uint16_t*>(vrow + 2 * c * 16) |
-                         ((uint32_t)*reinterpret_cast<const uint16_t*>(vrow + (2 * c + 1) * 16) << 16);
-      const __half* vpar = reinterpret_cast<const __half*>(tile + kKv4VParams + it * 32 + g * 4 + half * 2);
+      const uint32_t w = (uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_vcode(tt, g, 2 * c)) |
+                         ((uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_vcode(tt, g, 2 * c + 1)) << 16);
+      const __half* vpar = reinterpret_cast<const __half*>(tile + kv4_vparam(tt, g));
       kv4_values8(w, __half2float(vpar[0]), __half2float(vpar[8]), fv);
     } else {
 #pragma unroll

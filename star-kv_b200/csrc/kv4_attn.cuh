@@ -198,13 +198,35 @@ struct Kv4AttnSmem {
   }
 };
 
+__device__ __forceinline__ uint2 kv4_lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+
+// A lane's byte offsets within a tile, kept in registers (opaque to the compiler, which would
+// otherwise compute them anew for every load).
+struct Kv4Lane {
+  uint32_t code, kpar, kown, vpar, vmid;
+  __device__ __forceinline__ explicit Kv4Lane(int lane) {
+    const int r = lane >> 2, c = lane & 3;
+    code = lane * 16;
+    kpar = kKv4KParams + r * 32;
+    kown = kKv4KParams + r * 32 + (c & 1) * 16;
+    vpar = kKv4VParams + c * 32;
+    vmid = kKv4VParams + c * 32 + 16 + (r & 1) * 8;
+    asm volatile("" : "+r"(code), "+r"(kpar), "+r"(kown), "+r"(vpar), "+r"(vmid));
+  }
+};
+
 // The columns of one segment in a warp's registers.
 template <int NT>
 struct Kv4Columns {
-  uint32_t qb[NT][4][4], qc[NT][2];         // B operands of the scores: 16 q or q by nibble; sums of q for m and s
+  uint32_t qb[NT][4][4], qc[NT][2];         // B operands of the scores: 16 q or q by nibble; sums of q for s and m
   float cs[NT][2];                          // a column's scores, as computed (an eighth), to the log2 domain
   int end[NT][2];                           // first position a column does not attend to
-  float o[8][NT][4], z[NT][4], l[NT][2];
+  float o[8][NT][4], l[NT][2];
+  float z[NT][4];                           // sum w m: group j in rows j / 2 (and every second one) and j / 2 + 8
   float base[NT][2], thr[NT][2];            // w = 2^(x - base); x beyond thr moves the base
   int e;
 };
@@ -276,8 +298,8 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
     const float s0 = c & 1 ? sum[2] : sum[0], s1 = c & 1 ? sum[3] : sum[1];
     const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
     const float t0 = c & 2 ? s0 - h0 : h0, t1 = c & 2 ? s1 - h1 : h1;
-    s.qc[nt][0] = kv4_half2(0.125f * t0, 0.125f * t1);
-    s.qc[nt][1] = kv4_half2(-t0, -t1);
+    s.qc[nt][0] = kv4_half2(-t0, -t1);
+    s.qc[nt][1] = kv4_half2(0.125f * t0, 0.125f * t1);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       s.cs[nt][u] = __shfl_sync(0xffffffffu, scale, (2 * c + u) * 4);
@@ -300,7 +322,7 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
 // some of their positions are beyond what a column attends to, or beyond the length.
 template <int NT, int TILES, bool MASK, bool EDGE>
 __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, int pos, int len, const float* mrow,
-                                               int64_t mask_width, int lane) {
+                                               int64_t mask_width, const Kv4Lane& at, int lane) {
   const int r = lane >> 2, c = lane & 3;
   float x[TILES][NT][4];
   uint4 ta[TILES], tb[TILES];
@@ -311,15 +333,16 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
   uint32_t big = lim;
 #pragma unroll
   for (int h = 0; h < TILES; ++h) {
-    const uint32_t at = tl + h * kKv4TileBytes;
+    const uint32_t th = tl + h * kKv4TileBytes;
     const int p0 = pos + h * kKv4Tile;
     // ---- scores
-    const uint4 ka = kv4_lds128(at + r * 64 + c * 16), kb = kv4_lds128(at + r * 64 + c * 16 + 512);
-    const uint4 pa = kv4_lds128(at + kKv4KParams + r * 16), pb = kv4_lds128(at + kKv4KParams + r * 16 + 128);
-    ta[h] = kv4_lds128(at + kKv4VParams + c * 32);
-    tb[h] = kv4_lds128(at + kKv4VParams + c * 32 + 128);
+    const uint4 ka = kv4_lds128(th + at.code), kb = kv4_lds128(th + at.code + 512);
+    // rows r and r + 8 of s, then of m: groups 0 and 1, groups 2 and 3, and those the lane's columns of A take
+    const uint4 pa = kv4_lds128(th + at.kpar), pb = kv4_lds128(th + at.kpar + 16), own = kv4_lds128(th + at.kown);
+    ta[h] = kv4_lds128(th + at.vpar);
+    tb[h] = kv4_lds128(th + at.vpar + 128);
     const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-    const float2 sa01 = kv4_float2(pa.x), sa23 = kv4_float2(pa.y), sb01 = kv4_float2(pb.x), sb23 = kv4_float2(pb.y);
+    const float2 sa01 = kv4_float2(pa.x), sb01 = kv4_float2(pa.y), sa23 = kv4_float2(pb.x), sb23 = kv4_float2(pb.y);
     const float sa[4] = {sa01.x, sa01.y, sa23.x, sa23.y}, sb[4] = {sb01.x, sb01.y, sb23.x, sb23.y};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -351,11 +374,10 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
       add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
       add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
     }
-    const uint32_t m0 = c & 1 ? pa.w : pa.z, m1 = c & 1 ? pb.w : pb.z, s0 = c & 1 ? pa.y : pa.x, s1 = c & 1 ? pb.y : pb.x;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float d[4];
-      kv4_mma0(d, m0, m1, s0, s1, s.qc[nt][0], s.qc[nt][1]);
+      kv4_mma0(d, own.x, own.y, own.z, own.w, s.qc[nt][0], s.qc[nt][1]);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         float y = fmaf(x[h][nt][u], 0x1p17f, d[u]);   // an eighth of the column's score
@@ -426,14 +448,10 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
   // ---- weights and values
 #pragma unroll
   for (int h = 0; h < TILES; ++h) {
-    const uint32_t at = tl + h * kKv4TileBytes;
-    const uint4 va = kv4_lds128(at + kKv4VCodes + c * 128 + r * 16), vb = kv4_lds128(at + kKv4VCodes + c * 128 + r * 16 + 512);
-    uint32_t ma = 0, mb = 0;
-    if (r < 4) {
-      ma = kv4_lds32(at + kKv4VParams + 16 + c * 32 + r * 4);
-      mb = kv4_lds32(at + kKv4VParams + 16 + c * 32 + r * 4 + 128);
-    }
-    if (MASK || EDGE) ma &= keep_a[h], mb &= keep_b[h];
+    const uint32_t th = tl + h * kKv4TileBytes;
+    const uint4 va = kv4_lds128(th + at.code + kKv4VCodes), vb = kv4_lds128(th + at.code + kKv4VCodes + 512);
+    uint2 ma = kv4_lds64(th + at.vmid), mb = kv4_lds64(th + at.vmid + 128);
+    if (MASK || EDGE) ma.x &= keep_a[h], ma.y &= keep_a[h], mb.x &= keep_b[h], mb.y &= keep_b[h];
     uint32_t p0[NT], p1[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -462,7 +480,7 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
       }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma, 0u, mb, 0u, p0[nt], p1[nt]);
+    for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma.x, ma.y, mb.x, mb.y, p0[nt], p1[nt]);
   }
 }
 
@@ -597,6 +615,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       }
     }
   } else if (use.left > 0) {
+    const Kv4Lane offsets(lane);
     Kv4Columns<NT> s;
     int slot = 0, parity = 0, npieces = 0;
     bool ok = true;
@@ -614,16 +633,16 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
         const int pos = sm.pos[warp][slot][0], pos1 = sm.pos[warp][slot][1], bound = use.len - p.queries + 1;
         const uint32_t tl = smem_u32(sm.ring[warp][slot][0]);
         if (kPair && pos >= 0 && pos1 == pos + kKv4Tile && pos + 2 * kKv4Tile <= bound) {
-          kv4_tiles_step<NT, 2, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, lane);
+          kv4_tiles_step<NT, 2, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, offsets, lane);
         } else {
 #pragma unroll 1
           for (int j = 0; j < 2; ++j) {
             const int at = j ? pos1 : pos;
             if (at < 0) continue;
             if (at + kKv4Tile > bound || kPair)
-              kv4_tiles_step<NT, 1, MASK, true>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, lane);
+              kv4_tiles_step<NT, 1, MASK, true>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, offsets, lane);
             else
-              kv4_tiles_step<NT, 1, MASK, false>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, lane);
+              kv4_tiles_step<NT, 1, MASK, false>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, offsets, lane);
           }
         }
         __syncwarp();
@@ -658,7 +677,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float y = __shfl_sync(0xffffffffu, s.z[nt][u], j * 4 + c);
+            const float y = __shfl_sync(0xffffffffu, s.z[nt][u + 2 * (j & 1)], (j >> 1) * 4 + c);
             const float4 v = make_float4(
                 fmaf(s.o[2 * j][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j][nt][u + 2], 0x1p20f, y) * inv,
                 fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y) * inv);
