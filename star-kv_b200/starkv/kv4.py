@@ -40,74 +40,62 @@ _SELECT = struct.Struct("P3qPq3P8i")
 _TOKEN_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _QUERY_DTYPES = (torch.float16, torch.bfloat16)
 
+# The checks below run on every call of a decode step, several calls a layer: they
+# compare device indices and torch.Size tuples instead of building objects.
+_device_now = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _ints(t: torch.Tensor, name: str, shape, device):
-    if t.dtype != torch.int32 or t.device != device:
-        raise StarKVError(f"{name} must be an int32 tensor on {device}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+
+def _ints(t: torch.Tensor, name: str, shape, index: int) -> int:
+    if t.dtype != torch.int32 or t.get_device() != index:
+        raise StarKVError(f"{name} must be an int32 tensor on cuda:{index}")
+    if t.shape != shape or not t.is_contiguous():
         raise StarKVError(f"{name} must be contiguous of shape {shape}, got {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, shape, dtypes, device):
+def _rows(t: torch.Tensor, name: str, shape, dtypes, index: int):
     """Checks a (B, tokens, heads, 128) tensor; returns its element strides."""
-    if t.device != device:
-        raise StarKVError(f"{name} must be on {device}")
+    if t.get_device() != index:
+        raise StarKVError(f"{name} must be on cuda:{index}")
     if t.dtype not in dtypes:
         raise StarKVError(f"{name} must be one of {dtypes}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise StarKVError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     st = t.stride()
     if st[3] != 1:
         raise StarKVError(f"{name} channels must be contiguous")
     if 1 in shape:                       # the stride of a dimension of one is never used
-        st = tuple(0 if n == 1 else s for n, s in zip(shape, st))
+        st = tuple([0 if n == 1 else s for n, s in zip(shape, st)])
     return st
 
 
 def _output(t: torch.Tensor, name: str):
-    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+    if not t.is_contiguous() and any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
         raise StarKVError(f"{name} must not repeat elements (stride 0)")
-
-
-class _on:
-    """The tensors' device made current (nothing where it is already)."""
-
-    def __init__(self, device):
-        self.index, self.before = device.index, None
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.index:
-            self.before = now
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
 
 
 _WORKSPACES = {}
 _workspace_bytes = 0
 
 
-def workspace(device: torch.device, stream: int) -> torch.Tensor:
+def workspace(index: int, stream: int) -> torch.Tensor:
     """Attention scratch of one stream (zeroed once; every call leaves it zeroed
     where the next needs it).  A call under graph capture gets its own, zeroed by the
     graph, so replays never share one with eager calls."""
     global _workspace_bytes
-    key = (device.index, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is not None and not torch.cuda.is_current_stream_capturing():
+    ws = _WORKSPACES.get((index, stream))
+    capturing = torch.cuda.is_current_stream_capturing()
+    if ws is not None and not capturing:
         return ws
     if not _workspace_bytes:
         n = C.c_size_t(0)
         check(load().starkv_kv4_workspace_size(C.byref(n)), "starkv_kv4_workspace_size")
         _workspace_bytes = int(n.value)
-    ws = torch.zeros(_workspace_bytes, dtype=torch.uint8, device=device)
-    if not torch.cuda.is_current_stream_capturing():
-        _WORKSPACES[key] = ws
+    ws = torch.zeros(_workspace_bytes, dtype=torch.uint8, device=f"cuda:{index}")
+    if not capturing:
+        _WORKSPACES[index, stream] = ws
     return ws
 
 
@@ -142,26 +130,36 @@ class KV4Cache:
                                   self.bound_scales.data_ptr() if page_bounds else 0, self.error_word.data_ptr(),
                                   self.num_pages, self.num_kv_heads, self.page_size, 128)
         self._lib = load()
+        self._index = self.device.index
 
     def nbytes(self) -> int:
         """Device bytes of the pool (codes, parameters and bounds)."""
         return sum(t.numel() * t.element_size() for t in (self.data, self.bounds, self.bound_scales) if t is not None)
 
     def _table(self, t: torch.Tensor):
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 2 or t.shape[1] == 0:
-            raise StarKVError(f"block_table must be an int32 (B, W) tensor on {self.device}, W > 0")
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise StarKVError("block_table rows must be contiguous")
-        return t.shape[0], t.shape[1], t.data_ptr(), t.stride(0)
+        if t.dtype != torch.int32 or t.get_device() != self._index or t.dim() != 2:
+            raise StarKVError(f"block_table must be an int32 (B, W) tensor on {self.device}")
+        (B, W), (st, unit) = t.shape, t.stride()
+        if W == 0 or (W > 1 and unit != 1):
+            raise StarKVError("block_table must have W > 0 and contiguous rows")
+        return B, W, t.data_ptr(), st
+
+    def _call(self, fn, args: bytes, what: str):
+        """One C call on the pool's device and its current stream."""
+        if _device_now() == self._index:
+            rc = fn(self._block, args, _stream_of(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                rc = fn(self._block, args, _stream_of(self._index))
+        if rc:
+            check(rc, what)
 
     def _io(self, fn, what, k, v, ks, vs, table, start, count):
-        B, W, tp, ts = self._table(table)
-        n = k.shape[1]
-        a = _IO.pack(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], tp, ts,
-                     _ints(start, "start", (B,), self.device),
-                     0 if count is None else _ints(count, "count", (B,), self.device), _DT[k.dtype], B, n, W)
-        with _on(self.device) as stream:
-            check(fn(self._block, a, stream), what)
+        B, W, tp, ts = table
+        a = _IO.pack(k.data_ptr(), v.data_ptr(), *ks[:3], *vs[:3], tp, ts,
+                     _ints(start, "start", (B,), self._index),
+                     0 if count is None else _ints(count, "count", (B,), self._index), _DT[k.dtype], B, k.shape[1], W)
+        self._call(fn, a, what)
 
     def write(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
               count: Optional[torch.Tensor] = None) -> None:
@@ -169,10 +167,11 @@ class KV4Cache:
         stride that is a multiple of 16 bytes) into positions start[b] .. start[b] +
         count[b] - 1 (count: int32 (B,), T when None).  Filling a page's last slot
         writes the page's bounds."""
-        shape = (block_table.shape[0], k.shape[1] if k.dim() == 4 else -1, self.num_kv_heads, 128)
-        ks = _rows(k, "k", shape, _TOKEN_DTYPES, self.device)
-        vs = _rows(v, "v", shape, (k.dtype,), self.device)
-        self._io(self._lib.starkv_kv4_write, "starkv_kv4_write", k, v, ks, vs, block_table, start, count)
+        table = self._table(block_table)
+        shape = (table[0], k.shape[1] if k.dim() == 4 else -1, self.num_kv_heads, 128)
+        ks = _rows(k, "k", shape, _TOKEN_DTYPES, self._index)
+        vs = _rows(v, "v", shape, (k.dtype,), self._index)
+        self._io(self._lib.starkv_kv4_write, "starkv_kv4_write", k, v, ks, vs, table, start, count)
 
     def read(self, block_table: torch.Tensor, start: torch.Tensor, num_tokens: int,
              count: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
@@ -180,18 +179,23 @@ class KV4Cache:
         """Positions start[b] .. start[b] + num_tokens - 1 as (k, v), each (B,
         num_tokens, num_kv_heads, 128) of ``dtype`` (or into ``out``); rows past count[b]
         are 0."""
-        shape = (block_table.shape[0], int(num_tokens), self.num_kv_heads, 128)
+        table = self._table(block_table)
+        shape = (table[0], int(num_tokens), self.num_kv_heads, 128)
         if out is None:
             if num_tokens < 0:
                 raise StarKVError("num_tokens must not be negative")
-            out = (torch.empty(shape, dtype=dtype, device=self.device),
-                   torch.empty(shape, dtype=dtype, device=self.device))
-        k, v = out
-        ks = _rows(k, "out[0]", shape, _TOKEN_DTYPES, self.device)
-        vs = _rows(v, "out[1]", shape, (k.dtype,), self.device)
-        _output(k, "out[0]")
-        _output(v, "out[1]")
-        self._io(self._lib.starkv_kv4_read, "starkv_kv4_read", k, v, ks, vs, block_table, start, count)
+            if dtype not in _TOKEN_DTYPES:
+                raise StarKVError(f"dtype must be one of {_TOKEN_DTYPES}, got {dtype}")
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            v = torch.empty(shape, dtype=dtype, device=self.device)
+            ks = vs = k.stride()
+        else:
+            k, v = out
+            ks = _rows(k, "out[0]", shape, _TOKEN_DTYPES, self._index)
+            vs = _rows(v, "out[1]", shape, (k.dtype,), self._index)
+            _output(k, "out[0]")
+            _output(v, "out[1]")
+        self._io(self._lib.starkv_kv4_read, "starkv_kv4_read", k, v, ks, vs, table, start, count)
         return k, v
 
     def _queries(self, q: torch.Tensor, batch: int):
@@ -199,7 +203,7 @@ class KV4Cache:
         q4 = q.unsqueeze(1) if q.dim() == 3 else q
         if q4.dim() != 4 or q4.shape[2] == 0 or q4.shape[2] % self.num_kv_heads:
             raise StarKVError(f"q must be (B, Hq, 128) or (B, Q, Hq, 128), Hq a multiple of {self.num_kv_heads}")
-        return q4, _rows(q4, "q", (batch, q4.shape[1], q4.shape[2], 128), _QUERY_DTYPES, self.device)
+        return q4, _rows(q4, "q", (batch, q4.shape[1], q4.shape[2], 128), _QUERY_DTYPES, self._index)
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, scaling: float,
                mask: Optional[torch.Tensor] = None, pages: Optional[torch.Tensor] = None,
@@ -217,15 +221,18 @@ class KV4Cache:
         B, W, tp, ts = self._table(block_table)
         q4, qs = self._queries(q, B)
         Q, Hq = q4.shape[1], q4.shape[2]
-        lp = _ints(lengths, "lengths", (B,), self.device)
+        index = self._index
+        lp = _ints(lengths, "lengths", (B,), index)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        o4 = out.unsqueeze(1) if q.dim() == 3 and out.dim() == 3 else out
-        os_ = _rows(o4, "out", tuple(q4.shape), _TOKEN_DTYPES, self.device)
-        _output(o4, "out")
+            out = o4 = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            os_ = (Q * Hq * 128, Hq * 128, 128)
+        else:
+            o4 = out.unsqueeze(1) if q.dim() == 3 and out.dim() == 3 else out
+            os_ = _rows(o4, "out", q4.shape, _TOKEN_DTYPES, index)
+            _output(o4, "out")
         mp = mstride = mwidth = 0
         if mask is not None:
-            if mask.dtype != torch.float32 or mask.device != self.device or mask.dim() != 2 or mask.shape[0] != B:
+            if mask.dtype != torch.float32 or mask.get_device() != index or mask.dim() != 2 or mask.shape[0] != B:
                 raise StarKVError(f"mask must be an fp32 (B, L) tensor on {self.device}")
             if mask.shape[1] > 1 and mask.stride(1) != 1:
                 raise StarKVError("mask rows must be contiguous")
@@ -235,15 +242,16 @@ class KV4Cache:
             if pages.dim() != 3 or pages.shape[2] == 0:
                 raise StarKVError("pages must be (B, num_kv_heads, n), n > 0")
             n = pages.shape[2]
-            pp = _ints(pages, "pages", (B, self.num_kv_heads, n), self.device)
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-        with _on(self.device) as stream:
-            if ws is None:
-                ws = workspace(self.device, stream)
-            a = _ATTENTION.pack(q4.data_ptr(), o4.data_ptr(), lse.data_ptr() if return_lse else 0,
-                                qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], tp, ts, lp, mp, mstride, mwidth, pp,
-                                ws.data_ptr(), ws.numel(), scaling, n, _DT[q.dtype], _DT[out.dtype], B, Q, Hq, W)
-            check(self._lib.starkv_kv4_attention(self._block, a, stream), "starkv_kv4_attention")
+            pp = _ints(pages, "pages", (B, self.num_kv_heads, n), index)
+        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
+        if ws is None:
+            ws = workspace(index, _stream_of(index))
+        elif ws.get_device() != index or not ws.is_contiguous():
+            raise StarKVError(f"ws must be contiguous on {self.device}")
+        a = _ATTENTION.pack(q4.data_ptr(), o4.data_ptr(), lse.data_ptr() if return_lse else 0,
+                            *qs[:3], *os_[:3], tp, ts, lp, mp, mstride, mwidth, pp, ws.data_ptr(),
+                            ws.numel() * ws.element_size(), scaling, n, _DT[q.dtype], _DT[out.dtype], B, Q, Hq, W)
+        self._call(self._lib.starkv_kv4_attention, a, "starkv_kv4_attention")
         return (out, lse) if return_lse else out
 
     def select(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, num_pages: int,
@@ -256,18 +264,17 @@ class KV4Cache:
             raise StarKVError("this KV4Cache was made without page_bounds")
         B, W, tp, ts = self._table(block_table)
         q4, qs = self._queries(q, B)
-        lp = _ints(lengths, "lengths", (B,), self.device)
+        lp = _ints(lengths, "lengths", (B,), self._index)
         shape = (B, self.num_kv_heads, int(num_pages))
         if out is None:
             if num_pages <= 0:
                 raise StarKVError("num_pages must be positive")
             out = torch.empty(shape, dtype=torch.int32, device=self.device)
-        op = _ints(out, "out", shape, self.device)
+        op = _ints(out, "out", shape, self._index)
         scores = torch.empty(B * self.num_kv_heads * W, dtype=torch.float32, device=self.device)
-        a = _SELECT.pack(q4.data_ptr(), qs[0], qs[1], qs[2], tp, ts, lp, op, scores.data_ptr(), _DT[q.dtype], B,
+        a = _SELECT.pack(q4.data_ptr(), *qs[:3], tp, ts, lp, op, scores.data_ptr(), _DT[q.dtype], B,
                          q4.shape[1], q4.shape[2], W, num_pages, first, last)
-        with _on(self.device) as stream:
-            check(self._lib.starkv_kv4_select(self._block, a, stream), "starkv_kv4_select")
+        self._call(self._lib.starkv_kv4_select, a, "starkv_kv4_select")
         return out
 
     def read_error(self) -> int:
