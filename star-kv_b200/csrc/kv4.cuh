@@ -2,6 +2,8 @@
 // write with the page bounds, and the read-back.  Layout and quantiser are
 // specified in starkv.h.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -66,87 +68,119 @@ struct Kv4IoParams {
   int64_t units;                            // read: warps' worth of work
 };
 
-// Eight consecutive channels of one token as fp32.
+__device__ __forceinline__ float kv4_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float kv4_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sixteen consecutive channels of one token, as loaded.
 template <typename T>
-struct Vec8 {
-  uint4 w;
-  __device__ __forceinline__ void load(const T* p) { w = __ldcs(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float* f) const {
-    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+struct Kv4Row {
+  static constexpr int kVecs = sizeof(T);   // 16-byte loads
+  uint4 w[kVecs];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        const T lo = *reinterpret_cast<const T*>(&a[i]);
-        const uint32_t h = a[i] >> 16;
-        const unsigned short hs = (unsigned short)h;
-        const T hi = *reinterpret_cast<const T*>(&hs);
-        f[2 * i] = to_f32(lo);
-        f[2 * i + 1] = to_f32(hi);
+    for (int i = 0; i < kVecs; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  // Values, and their minimum and maximum (NaN if one is).
+  __device__ __forceinline__ void get(float* f, float& mn, float& mx) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[4 * i] = __uint_as_float(w[i].x), f[4 * i + 1] = __uint_as_float(w[i].y);
+        f[4 * i + 2] = __uint_as_float(w[i].z), f[4 * i + 3] = __uint_as_float(w[i].w);
       }
+      mn = mx = f[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mn = kv4_min_nan(mn, f[i]), mx = kv4_max_nan(mx, f[i]);
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      T2 v[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * i + k] = *reinterpret_cast<const T2*>(&a[k]);
+      }
+      T2 lo = v[0], hi = v[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) lo = __hmin2_nan(lo, v[i]), hi = __hmax2_nan(hi, v[i]);
+      mn = to_f32(__hmin_nan(lo.x, lo.y));
+      mx = to_f32(__hmax_nan(hi.x, hi.y));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[2 * i] = to_f32(v[i].x), f[2 * i + 1] = to_f32(v[i].y);
     }
   }
 };
-template <>
-struct Vec8<float> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = __ldcs(reinterpret_cast<const float4*>(p));
-    b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-  }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ void get(float* f) const {
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
+
+// A lane's 16 channels quantised (its neighbour lane ^ 1 has the group's other 16).
+struct Kv4Codes {
+  uint32_t w[2];                            // nibbles c + 8 in channel order
+  __half s, m;
+  float r[16];                              // c as a float
 };
 
-// Quantises a lane's 8 channels; the group of 32 is the lane's aligned group of
-// four lanes.  Returns the 8 codes (0..15) as nibbles in channel order.
-__device__ __forceinline__ uint32_t kv4_quantise8(float* f, __half& hs, __half& hm) {
-  bool nan = false;
-  float mn = 65504.f, mx = -65504.f;
+// Rounding by adding 1.5 * 2^23 + 8: the low bits of the sum are c + 8.
+constexpr float kKv4Magic = 12582920.f;
+
+template <bool CLAMP>
+__device__ __forceinline__ void kv4_encode16(const float* f, float m, float inv, Kv4Codes& q) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    nan |= f[i] != f[i];
-    f[i] = fminf(fmaxf(f[i], -65504.f), 65504.f);
-    mn = fminf(mn, f[i]);
-    mx = fmaxf(mx, f[i]);
-  }
-  const unsigned group = 0xfu << (threadIdx.x & 28);
-  nan = (__ballot_sync(0xffffffffu, nan) & group) != 0;
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w = 0;
 #pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    for (int i = 7; i >= 0; --i) {
+      float x = f[8 * h + i];
+      if (CLAMP) x = fminf(fmaxf(x, -65504.f), 65504.f);
+      float y = __fmul_rn(__fsub_rn(x, m), inv);
+      if (CLAMP) y = fminf(fmaxf(y, -8.f), 7.f);
+      y = __fadd_rn(y, kKv4Magic);
+      q.r[8 * h + i] = y - kKv4Magic;
+      // sum of 16^i times the bits, whose constant parts are taken off below (modulo 2^32)
+      w = w * 16u + __float_as_uint(y);
+    }
+    q.w[h] = w - 0x11111111u * 0x4b400000u;
   }
-  hs = __float2half_rn(__fdiv_rn(__fsub_rn(mx, mn), 15.0f));
-  if (nan) hs = __float2half_rn(0.f);
-  const float s = __half2float(hs);
-  hm = __float2half_rn(__fadd_rn(mn, 8.0f * s));
-  const float m = __half2float(hm);
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], m), inv)), -8.f), 7.f);
-    w |= (uint32_t)((int)c + 8) << (4 * i);
-  }
-  if (nan) hm = __ushort_as_half((unsigned short)0x7fff);
-  return w;
 }
 
-// The lane's word of a pair of tokens' value codes: lanes 0-15 hold the even
-// token's nibbles (8 channels: quads 2c and 2c + 1 of their group), lanes 16-31 the
-// odd token's.  Lanes 0-15 get quad 2c of both tokens, lanes 16-31 quad 2c + 1.
-__device__ __forceinline__ uint32_t kv4_pair_word(uint32_t w, int half) {
-  const uint32_t o = __shfl_xor_sync(0xffffffffu, w, 16);
-  return half ? __byte_perm(o, w, 0x7632) : __byte_perm(w, o, 0x5410);
+// The scale, centre and codes of a row's 16 channels.  Codes can leave [-8, 7] before they are
+// clamped only where fp16 holds s or m coarsely (s subnormal, |m| > 512 s) or x is beyond
+// fp16; a warp without such a group skips the clamps (3 of 8 instructions a value).
+template <typename T>
+__device__ __forceinline__ void kv4_quantise16(const Kv4Row<T>& row, Kv4Codes& q) {
+  float f[16], mn, mx;
+  row.get(f, mn, mx);
+  mn = kv4_min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
+  mx = kv4_max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  const bool nan = mx != mx, wide = mx > 65504.f || mn < -65504.f;
+  mn = fminf(fmaxf(mn, -65504.f), 65504.f);
+  mx = fminf(fmaxf(mx, -65504.f), 65504.f);
+  q.s = __float2half_rn(nan ? 0.f : __fdiv_rn(__fsub_rn(mx, mn), 15.0f));
+  const float s = __half2float(q.s);
+  q.m = __float2half_rn(__fadd_rn(mn, 8.0f * s));
+  const float m = __half2float(q.m), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  const bool plain = s == 0.f || (s >= 0x1p-14f && fabsf(m) <= 512.f * s);
+  if (__all_sync(0xffffffffu, plain && !wide && !nan))
+    kv4_encode16<false>(f, m, inv, q);
+  else
+    kv4_encode16<true>(f, m, inv, q);
+  if (nan) q.m = __ushort_as_half((unsigned short)0x7fff);
 }
 
-// ---- write: one CTA per (page, KV head) of a sequence's range, one warp per tile.
-// Each half-warp takes one token (16 bytes of fp16 per lane), so a group's minimum
-// and maximum need two shuffles and every store of codes is a full 128-byte line.
+// ---- write: one CTA per (page, KV head) of a sequence's range, one warp per tile, eight lanes
+// per token: half a group a lane, so that a group's minimum and maximum need one shuffle and
+// its scale is worked out twice, not eight times.  A full tile is put together in shared
+// memory and stored 16 bytes a lane; of a part of one, each lane stores its own words.
 template <typename T>
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
   const Kv4Pool& pool = p.pool;
@@ -166,84 +200,102 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
   const int ps = pool.page_tiles * kKv4Tile;
   const int lo = start > base ? (int)(start - base) : 0, hi = end - base < ps ? (int)(end - base) : ps;
   const bool full = hi == ps && pool.bounds != nullptr;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = lane >> 4, l16 = lane & 15;
-  const int c = l16 & 3, g = l16 >> 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tok = lane >> 3, g = lane >> 1 & 3, part = lane & 1;   // token of a step, group, half of it
   const int t0 = warp * kKv4Tile;
+  __shared__ __align__(16) uint8_t stage[kKv4MaxPageTiles][kKv4TileBytes];
   __shared__ float red[2][kKv4MaxPageTiles][128];
-  float bmax[8], bmin[8];
+  float bmax[16], bmin[16];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bmax[i] = -INFINITY, bmin[i] = INFINITY;
+  for (int i = 0; i < 16; ++i) bmax[i] = -INFINITY, bmin[i] = INFINITY;
+  const bool whole = t0 >= lo && t0 + kKv4Tile <= hi;
   if ((t0 < hi && t0 + kKv4Tile > lo) || full) {
     uint8_t* tile = pool.tile(page, head, warp);
-    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + head * p.ks[2] + l16 * 8;
-    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + head * p.vs[2] + l16 * 8;
+    uint8_t* to = whole ? stage[warp] : tile;
+    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + head * p.ks[2] + (lane & 7) * 16;
+    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + head * p.vs[2] + (lane & 7) * 16;
     const int64_t first = base + t0 - start;                   // token index of the tile's slot 0
-    Vec8<T> kx[8];
-    Vec8<T> vx[8];
+    Kv4Row<T> kx[4], vx[4];
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int t = t0 + 2 * it + half;
+    for (int it = 0; it < 4; ++it) {
+      const int t = t0 + 4 * it + tok;
       kx[it].zero();
       vx[it].zero();
       if (t >= lo && t < hi) {
-        kx[it].load(kp + (first + 2 * it + half) * p.ks[1]);
-        vx[it].load(vp + (first + 2 * it + half) * p.vs[1]);
+        kx[it].load(kp + (first + 4 * it + tok) * p.ks[1]);
+        vx[it].load(vp + (first + 4 * it + tok) * p.vs[1]);
       }
     }
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int tt = 2 * it + half, t = t0 + tt;
+    for (int it = 0; it < 4; ++it) {
+      const int tt = 4 * it + tok, t = t0 + tt;
       const bool mine = t >= lo && t < hi;
-      float f[8];
-      __half s, m;
-      kx[it].get(f);
-      uint32_t w = kv4_quantise8(f, s, m);
-      uint32_t* kw = reinterpret_cast<uint32_t*>(tile + tt * 64 + c * 16 + g * 4);
-      __half* kpar = reinterpret_cast<__half*>(tile + kv4_kparam(tt, g));
+      if (!full && (t0 + 4 * it >= hi || t0 + 4 * it + 4 <= lo)) continue;   // none of these four
+      Kv4Codes q;
+      kv4_quantise16(kx[it], q);
+      uint32_t* kw = reinterpret_cast<uint32_t*>(to + tt * 64 + part * 32 + g * 4);
+      __half* kpar = reinterpret_cast<__half*>(to + kv4_kparam(tt, g));
       if (mine) {
-        *kw = w;
-        if (c == 0) kpar[0] = s, kpar[4] = m;
+        kw[0] = q.w[0];
+        kw[4] = q.w[1];
+        if (part == 0) kpar[0] = q.s;
+        else kpar[4] = q.m;
       } else if (full) {                                       // an earlier call's token of this page
-        w = *kw;
-        s = kpar[0];
-        m = kpar[4];
+        const uint32_t old[2] = {kw[0], kw[4]};
+        q.s = kpar[0];
+        q.m = kpar[4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q.r[i] = (float)((int)((old[i >> 3] >> (4 * (i & 7))) & 15u) - 8);
       }
       if (full) {
-        const float fs = __half2float(s), fm = __half2float(m);
+        const float fs = __half2float(q.s), fm = __half2float(q.m);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x = __fmaf_rn(fs, (float)((int)((w >> (4 * i)) & 15u) - 8), fm);
+        for (int i = 0; i < 16; ++i) {
+          const float x = __fmaf_rn(fs, q.r[i], fm);
           bmax[i] = fmaxf(bmax[i], x);
           bmin[i] = fminf(bmin[i], x);
         }
       }
-      vx[it].get(f);
-      w = kv4_quantise8(f, s, m);
-      const uint32_t pw = kv4_pair_word(w, half);
-      const uint32_t sm = (uint32_t)__half_as_ushort(s) | ((uint32_t)__half_as_ushort(m) << 16);
-      const uint32_t so = __shfl_xor_sync(0xffffffffu, sm, 16);
-      const int te = t0 + 2 * it;
+      kv4_quantise16(vx[it], q);
+      // the pair's other token is eight lanes on: even tokens take quads 0 and 1 of the half group
+      // for both, odd tokens quads 2 and 3
+      const int odd = tok & 1;
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? q.w[0] : q.w[1], 8);
+      const uint32_t sm = (uint32_t)__half_as_ushort(q.s) | ((uint32_t)__half_as_ushort(q.m) << 16);
+      const uint32_t so = __shfl_xor_sync(0xffffffffu, sm, 8);
+      const int te = t - odd;                                  // the pair's even token
       if (te >= lo && te + 1 < hi) {
-        *reinterpret_cast<uint32_t*>(tile + kv4_vcode(2 * it, g, 2 * c + half)) = pw;
-        if (c == 0)
-          *reinterpret_cast<uint32_t*>(tile + kv4_vparam(2 * it, g) + half * 16) =
-              half ? __byte_perm(so, sm, 0x7632) : __byte_perm(sm, so, 0x5410);
+        const uint32_t even = odd ? other : q.w[0], second = odd ? q.w[1] : other;
+        uint32_t* vw = reinterpret_cast<uint32_t*>(to + kv4_vcode(tt & ~1, g, part * 4 + odd * 2));
+        vw[0] = __byte_perm(even, second, 0x5410);
+        vw[16] = __byte_perm(even, second, 0x7632);
+        const uint32_t pe = odd ? so : sm, po = odd ? sm : so;
+        if (part == 0)
+          *reinterpret_cast<uint32_t*>(to + kv4_vparam(tt & ~1, g) + odd * 16) = __byte_perm(pe, po, odd ? 0x7632 : 0x5410);
       } else if (mine) {                                       // the pair's other token is not this call's
-        *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, 2 * c)) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, 2 * c + 1)) = (uint16_t)(w >> 16);
-        if (c == 0) {
-          *reinterpret_cast<__half*>(tile + kv4_vparam(tt, g)) = s;
-          *reinterpret_cast<__half*>(tile + kv4_vparam(tt, g) + 16) = m;
-        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, part * 4 + k)) = (uint16_t)(q.w[k >> 1] >> (16 * (k & 1)));
+        __half* vpar = reinterpret_cast<__half*>(tile + kv4_vparam(tt, g));
+        if (part == 0) vpar[0] = q.s;
+        else vpar[8] = q.m;
       }
+    }
+    if (whole) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 5; ++i)
+        reinterpret_cast<uint4*>(tile)[lane + 32 * i] = reinterpret_cast<const uint4*>(stage[warp])[lane + 32 * i];
     }
   }
   if (!full) return;                                           // uniform over the CTA
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 16; ++i) {
+    bmax[i] = fmaxf(bmax[i], __shfl_xor_sync(0xffffffffu, bmax[i], 8));
+    bmin[i] = fminf(bmin[i], __shfl_xor_sync(0xffffffffu, bmin[i], 8));
     bmax[i] = fmaxf(bmax[i], __shfl_xor_sync(0xffffffffu, bmax[i], 16));
     bmin[i] = fminf(bmin[i], __shfl_xor_sync(0xffffffffu, bmin[i], 16));
-    if (half == 0) red[0][warp][l16 * 8 + i] = bmax[i], red[1][warp][l16 * 8 + i] = bmin[i];
+    if (tok == 0) red[0][warp][lane * 16 + i] = bmax[i], red[1][warp][lane * 16 + i] = bmin[i];
   }
   __syncthreads();
   if (warp != 0) return;

@@ -186,8 +186,7 @@ class KV4Cache:
                 raise StarKVError("num_tokens must not be negative")
             if dtype not in _TOKEN_DTYPES:
                 raise StarKVError(f"dtype must be one of {_TOKEN_DTYPES}, got {dtype}")
-            k = torch.empty(shape, dtype=dtype, device=self.device)
-            v = torch.empty(shape, dtype=dtype, device=self.device)
+            k, v = torch.empty((2, *shape), dtype=dtype, device=self.device).unbind(0)
             ks = vs = k.stride()
         else:
             k, v = out
