@@ -68,6 +68,8 @@ struct Kv4IoParams {
   int64_t units;                            // read: warps' worth of work
 };
 
+// Both halves of a word of two fp16 numbers.
+__device__ __forceinline__ float2 kv4_halves(uint32_t a) { return __half22float2(*reinterpret_cast<const __half2*>(&a)); }
 __device__ __forceinline__ float kv4_min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -92,52 +94,63 @@ struct Kv4Row {
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) w[i] = make_uint4(0, 0, 0, 0);
   }
-  // Values, and their minimum and maximum (NaN if one is).
-  __device__ __forceinline__ void get(float* f, float& mn, float& mx) const {
+  // The minimum and maximum (NaN if one value is).
+  __device__ __forceinline__ void range(float& mn, float& mx) const {
     if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[4 * i] = __uint_as_float(w[i].x), f[4 * i + 1] = __uint_as_float(w[i].y);
-        f[4 * i + 2] = __uint_as_float(w[i].z), f[4 * i + 3] = __uint_as_float(w[i].w);
-      }
+      float f[16];
+      get(f);
       mn = mx = f[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mn = kv4_min_nan(mn, f[i]), mx = kv4_max_nan(mx, f[i]);
     } else {
       using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-      T2 v[8];
+      T2 lo, hi;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t a[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[4 * i + k] = *reinterpret_cast<const T2*>(&a[k]);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = word(i);
+        const T2 v = *reinterpret_cast<const T2*>(&a);
+        lo = i ? __hmin2_nan(lo, v) : v;
+        hi = i ? __hmax2_nan(hi, v) : v;
       }
-      T2 lo = v[0], hi = v[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) lo = __hmin2_nan(lo, v[i]), hi = __hmax2_nan(hi, v[i]);
       mn = to_f32(__hmin_nan(lo.x, lo.y));
       mx = to_f32(__hmax_nan(hi.x, hi.y));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[2 * i] = to_f32(v[i].x), f[2 * i + 1] = to_f32(v[i].y);
     }
   }
-};
-
-// A lane's 16 channels quantised (its neighbour lane ^ 1 has the group's other 16).
-struct Kv4Codes {
-  uint32_t w[2];                            // nibbles c + 8 in channel order
-  __half s, m;
-  float r[16];                              // c as a float
+  __device__ __forceinline__ uint32_t word(int i) const {
+    const uint4& v = w[i >> 2];
+    return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(word(i));
+    } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = word(i);
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
+        f[2 * i] = v.x, f[2 * i + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[2 * i] = __uint_as_float(word(i) << 16), f[2 * i + 1] = __uint_as_float(word(i) & 0xffff0000u);
+    }
+  }
 };
 
 // Rounding by adding 1.5 * 2^23 + 8: the low bits of the sum are c + 8.
 constexpr float kKv4Magic = 12582920.f;
 
-template <bool CLAMP>
-__device__ __forceinline__ void kv4_encode16(const float* f, float m, float inv, Kv4Codes& q) {
+// Codes of a lane's 16 channels (nibbles c + 8 in channel order) and, where BOUNDS, the extremes
+// of the values they stand for.
+template <bool CLAMP, bool BOUNDS, typename T>
+__device__ __forceinline__ void kv4_encode16(const Kv4Row<T>& row, float s, float m, float inv, uint32_t* w, float* bmax,
+                                             float* bmin) {
+  float f[16];
+  row.get(f);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t w = 0;
+    uint32_t sum = 0;
 #pragma unroll
     for (int i = 7; i >= 0; --i) {
       float x = f[8 * h + i];
@@ -145,44 +158,35 @@ __device__ __forceinline__ void kv4_encode16(const float* f, float m, float inv,
       float y = __fmul_rn(__fsub_rn(x, m), inv);
       if (CLAMP) y = fminf(fmaxf(y, -8.f), 7.f);
       y = __fadd_rn(y, kKv4Magic);
-      q.r[8 * h + i] = y - kKv4Magic;
+      if (BOUNDS) {
+        x = __fmaf_rn(s, y - kKv4Magic, m);
+        bmax[8 * h + i] = fmaxf(bmax[8 * h + i], x);
+        bmin[8 * h + i] = fminf(bmin[8 * h + i], x);
+      }
       // sum of 16^i times the bits, whose constant parts are taken off below (modulo 2^32)
-      w = w * 16u + __float_as_uint(y);
+      sum = sum * 16u + __float_as_uint(y);
     }
-    q.w[h] = w - 0x11111111u * 0x4b400000u;
+    w[h] = sum - 0x11111111u * 0x4b400000u;
   }
 }
 
-// The scale, centre and codes of a row's 16 channels.  Codes can leave [-8, 7] before they are
-// clamped only where fp16 holds s or m coarsely (s subnormal, |m| > 512 s) or x is beyond
-// fp16; a warp without such a group skips the clamps (3 of 8 instructions a value).
-template <typename T>
-__device__ __forceinline__ void kv4_quantise16(const Kv4Row<T>& row, Kv4Codes& q) {
-  float f[16], mn, mx;
-  row.get(f, mn, mx);
-  mn = kv4_min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
-  mx = kv4_max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-  const bool nan = mx != mx, wide = mx > 65504.f || mn < -65504.f;
-  mn = fminf(fmaxf(mn, -65504.f), 65504.f);
-  mx = fminf(fmaxf(mx, -65504.f), 65504.f);
-  q.s = __float2half_rn(nan ? 0.f : __fdiv_rn(__fsub_rn(mx, mn), 15.0f));
-  const float s = __half2float(q.s);
-  q.m = __float2half_rn(__fadd_rn(mn, 8.0f * s));
-  const float m = __half2float(q.m), inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  const bool plain = s == 0.f || (s >= 0x1p-14f && fabsf(m) <= 512.f * s);
-  if (__all_sync(0xffffffffu, plain && !wide && !nan))
-    kv4_encode16<false>(f, m, inv, q);
-  else
-    kv4_encode16<true>(f, m, inv, q);
-  if (nan) q.m = __ushort_as_half((unsigned short)0x7fff);
+// The token that a 16-bit unit of a tile belongs to.
+__device__ __forceinline__ int kv4_unit_token(int u) {
+  const int o = 2 * u;
+  if (o < kKv4VCodes) return o >> 6;
+  if (o < kKv4KParams) return (o - kKv4VCodes) / 512 * 8 + (o >> 4 & 3) * 2 + (o >> 1 & 1);
+  if (o < kKv4VParams) return (o - kKv4KParams) / 32 + (o >> 2 & 1) * 8;
+  return (o - kKv4VParams) / 32 * 2 + (o >> 1 & 1);
 }
 
 // ---- write: one CTA per (page, KV head) of a sequence's range, one warp per tile, eight lanes
-// per token: half a group a lane, so that a group's minimum and maximum need one shuffle and
-// its scale is worked out twice, not eight times.  A full tile is put together in shared
-// memory and stored 16 bytes a lane; of a part of one, each lane stores its own words.
+// per token: half a group a lane.  Of the two lanes of a group one works out the scale of
+// the key's group, the other that of the value's.  The tile is put together in shared
+// memory and stored 16 bytes a lane, or only its new tokens where others stay.
+// Codes can leave [-8, 7] before they are clamped only where fp16 holds s or m coarsely (s
+// subnormal, |m| > 512 s) or x is beyond fp16; a warp without such a group skips the clamps.
 template <typename T>
-__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
+__global__ void __launch_bounds__(256, 2) kv4_write_kernel(const Kv4IoParams p) {
   const Kv4Pool& pool = p.pool;
   const int head = blockIdx.x % pool.heads, b = blockIdx.y;
   const int64_t start = p.start[b];
@@ -195,132 +199,168 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4IoParams p) {
   const int64_t ord = (start >> pool.page_shift) + blockIdx.x / pool.heads;
   const int64_t base = ord << pool.page_shift;                 // position of the page's slot 0
   if (base >= end) return;
-  const int page = kv4_page(pool, p.table + b * p.table_stride, ord, p.width);
-  if (page < 0) return;
-  const int ps = pool.page_tiles * kKv4Tile;
-  const int lo = start > base ? (int)(start - base) : 0, hi = end - base < ps ? (int)(end - base) : ps;
-  const bool full = hi == ps && pool.bounds != nullptr;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tok = lane >> 3, g = lane >> 1 & 3, part = lane & 1;   // token of a step, group, half of it
-  const int t0 = warp * kKv4Tile;
+  const int ps = pool.page_tiles * kKv4Tile, t0 = warp * kKv4Tile;
+  // new tokens: slots [lo, hi) of the page, [a, e) of the tile
+  const int lo = start > base ? (int)(start - base) : 0, hi = end - base < ps ? (int)(end - base) : ps;
+  const int a = max(lo - t0, 0), e = min(hi - t0, kKv4Tile);
+  const bool full = hi == ps && pool.bounds != nullptr;
   __shared__ __align__(16) uint8_t stage[kKv4MaxPageTiles][kKv4TileBytes];
-  __shared__ float red[2][kKv4MaxPageTiles][128];
+  __shared__ __align__(16) float red[2][kKv4MaxPageTiles][128];
   float bmax[16], bmin[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) bmax[i] = -INFINITY, bmin[i] = INFINITY;
-  const bool whole = t0 >= lo && t0 + kKv4Tile <= hi;
-  if ((t0 < hi && t0 + kKv4Tile > lo) || full) {
-    uint8_t* tile = pool.tile(page, head, warp);
-    uint8_t* to = whole ? stage[warp] : tile;
-    const T* kp = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + head * p.ks[2] + (lane & 7) * 16;
-    const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + head * p.vs[2] + (lane & 7) * 16;
-    const int64_t first = base + t0 - start;                   // token index of the tile's slot 0
-    Kv4Row<T> kx[4], vx[4];
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int t = t0 + 4 * it + tok;
-      kx[it].zero();
-      vx[it].zero();
-      if (t >= lo && t < hi) {
-        kx[it].load(kp + (first + 4 * it + tok) * p.ks[1]);
-        vx[it].load(vp + (first + 4 * it + tok) * p.vs[1]);
-      }
+  // the rows of the first steps, before the page is known
+  const int64_t first = base + t0 - start + tok;               // token of the lane's row in step 0
+  const T* kp = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + first * p.ks[1] + head * p.ks[2] + (lane & 7) * 16;
+  const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + first * p.vs[1] + head * p.vs[2] + (lane & 7) * 16;
+  constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+  Kv4Row<T> kx[kAhead], vx[kAhead];
+  auto load = [&](int it) {
+    const int t = 4 * it + tok;
+    Kv4Row<T>&k = kx[it % kAhead], &v = vx[it % kAhead];
+    k.zero();
+    v.zero();
+    if (t >= a && t < e) {
+      k.load(kp + 4 * it * p.ks[1]);
+      v.load(vp + 4 * it * p.vs[1]);
     }
+  };
+#pragma unroll
+  for (int it = 0; it < kAhead; ++it) load(it);
+  const int page = kv4_page(pool, p.table + b * p.table_stride, ord, p.width);
+  if (page < 0) return;
+  uint8_t* tile = pool.tile(page, head, warp);
+  if (a < e) {
+    uint8_t* sk = stage[warp] + tok * 64 + part * 32 + g * 4;
+    uint8_t* sp = stage[warp] + kKv4KParams + tok * 32 + (g >> 1) * 16 + (g & 1) * 2;
+    uint8_t* sv = stage[warp] + kKv4VCodes + (part * 4 + (tok & 1) * 2) * 64 + (tok >> 1) * 16 + g * 4;
+    uint8_t* sq = stage[warp] + kKv4VParams + (tok >> 1) * 32 + g * 4 + (tok & 1) * 16;
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const int tt = 4 * it + tok, t = t0 + tt;
-      const bool mine = t >= lo && t < hi;
-      if (!full && (t0 + 4 * it >= hi || t0 + 4 * it + 4 <= lo)) continue;   // none of these four
-      Kv4Codes q;
-      kv4_quantise16(kx[it], q);
-      uint32_t* kw = reinterpret_cast<uint32_t*>(to + tt * 64 + part * 32 + g * 4);
-      __half* kpar = reinterpret_cast<__half*>(to + kv4_kparam(tt, g));
-      if (mine) {
-        kw[0] = q.w[0];
-        kw[4] = q.w[1];
-        if (part == 0) kpar[0] = q.s;
-        else kpar[4] = q.m;
-      } else if (full) {                                       // an earlier call's token of this page
-        const uint32_t old[2] = {kw[0], kw[4]};
-        q.s = kpar[0];
-        q.m = kpar[4];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q.r[i] = (float)((int)((old[i >> 3] >> (4 * (i & 7))) & 15u) - 8);
+      const Kv4Row<T> k = kx[it % kAhead], v = vx[it % kAhead];
+      if (it + kAhead < 4) load(it + kAhead);
+      if (4 * it >= e || 4 * it + 4 <= a) continue;            // none of these four
+      const bool mine = 4 * it + tok >= a && 4 * it + tok < e;
+      // ranges: lane part 0 gets the key group's, part 1 the value group's
+      float kmn, kmx, vmn, vmx;
+      k.range(kmn, kmx);
+      v.range(vmn, vmx);
+      float mn = __shfl_xor_sync(0xffffffffu, part ? kmn : vmn, 1), mx = __shfl_xor_sync(0xffffffffu, part ? kmx : vmx, 1);
+      mn = kv4_min_nan(mn, part ? vmn : kmn);
+      mx = kv4_max_nan(mx, part ? vmx : kmx);
+      const bool nan = mx != mx, wide = mx > 65504.f || mn < -65504.f;
+      mn = fminf(fmaxf(mn, -65504.f), 65504.f);
+      mx = fminf(fmaxf(mx, -65504.f), 65504.f);
+      const __half hs = __float2half_rn(nan ? 0.f : __fdiv_rn(__fsub_rn(mx, mn), 15.0f));
+      const float s = __half2float(hs);
+      __half hm = __float2half_rn(__fadd_rn(mn, 8.0f * s));
+      const float am = fabsf(__half2float(hm)), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+      const bool plain = !nan && !wide && (s == 0.f || (s >= 0x1p-14f && am <= 512.f * s));
+      if (nan) hm = __ushort_as_half((unsigned short)0x7fff);
+      const uint32_t sm = (uint32_t)__half_as_ushort(hs) | ((uint32_t)__half_as_ushort(hm) << 16);
+      const float2 ksm = kv4_halves(__shfl_sync(0xffffffffu, sm, lane & 30)), vsm = kv4_halves(__shfl_sync(0xffffffffu, sm, lane | 1));
+      const float kinv = __shfl_sync(0xffffffffu, inv, lane & 30), vinv = __shfl_sync(0xffffffffu, inv, lane | 1);
+      uint32_t kw[2], vw[2];
+      if (__all_sync(0xffffffffu, plain)) {
+        if (full && mine) kv4_encode16<false, true>(k, ksm.x, ksm.y, kinv, kw, bmax, bmin);
+        else kv4_encode16<false, false>(k, ksm.x, ksm.y, kinv, kw, bmax, bmin);
+        kv4_encode16<false, false>(v, vsm.x, vsm.y, vinv, vw, bmax, bmin);
+      } else {
+        if (full && mine) kv4_encode16<true, true>(k, ksm.x, ksm.y, kinv, kw, bmax, bmin);
+        else kv4_encode16<true, false>(k, ksm.x, ksm.y, kinv, kw, bmax, bmin);
+        kv4_encode16<true, false>(v, vsm.x, vsm.y, vinv, vw, bmax, bmin);
       }
-      if (full) {
-        const float fs = __half2float(q.s), fm = __half2float(q.m);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float x = __fmaf_rn(fs, q.r[i], fm);
-          bmax[i] = fmaxf(bmax[i], x);
-          bmin[i] = fminf(bmin[i], x);
-        }
-      }
-      kv4_quantise16(vx[it], q);
-      // the pair's other token is eight lanes on: even tokens take quads 0 and 1 of the half group
-      // for both, odd tokens quads 2 and 3
+      *reinterpret_cast<uint32_t*>(sk + it * 256) = kw[0];
+      *reinterpret_cast<uint32_t*>(sk + it * 256 + 16) = kw[1];
+      // a pair's other token is eight lanes on: even tokens put together quads 0 and 1 of the half
+      // group for both and the pair's s, odd tokens quads 2 and 3 and its m
       const int odd = tok & 1;
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? q.w[0] : q.w[1], 8);
-      const uint32_t sm = (uint32_t)__half_as_ushort(q.s) | ((uint32_t)__half_as_ushort(q.m) << 16);
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? vw[0] : vw[1], 8);
+      const uint32_t even = odd ? other : vw[0], second = odd ? vw[1] : other;
+      const int at = (it >> 1) * 512 + (it & 1) * 32;
+      *reinterpret_cast<uint32_t*>(sv + at) = __byte_perm(even, second, 0x5410);
+      *reinterpret_cast<uint32_t*>(sv + at + 64) = __byte_perm(even, second, 0x7632);
       const uint32_t so = __shfl_xor_sync(0xffffffffu, sm, 8);
-      const int te = t - odd;                                  // the pair's even token
-      if (te >= lo && te + 1 < hi) {
-        const uint32_t even = odd ? other : q.w[0], second = odd ? q.w[1] : other;
-        uint32_t* vw = reinterpret_cast<uint32_t*>(to + kv4_vcode(tt & ~1, g, part * 4 + odd * 2));
-        vw[0] = __byte_perm(even, second, 0x5410);
-        vw[16] = __byte_perm(even, second, 0x7632);
-        const uint32_t pe = odd ? so : sm, po = odd ? sm : so;
-        if (part == 0)
-          *reinterpret_cast<uint32_t*>(to + kv4_vparam(tt & ~1, g) + odd * 16) = __byte_perm(pe, po, odd ? 0x7632 : 0x5410);
-      } else if (mine) {                                       // the pair's other token is not this call's
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<uint16_t*>(tile + kv4_vcode(tt, g, part * 4 + k)) = (uint16_t)(q.w[k >> 1] >> (16 * (k & 1)));
-        __half* vpar = reinterpret_cast<__half*>(tile + kv4_vparam(tt, g));
-        if (part == 0) vpar[0] = q.s;
-        else vpar[8] = q.m;
+      if (part == 0) {
+        *reinterpret_cast<__half*>(sp + (it & 1) * 128 + (it >> 1) * 4) = hs;
+        *reinterpret_cast<__half*>(sp + (it & 1) * 128 + (it >> 1) * 4 + 8) = hm;
+      } else {
+        *reinterpret_cast<uint32_t*>(sq + it * 64) = __byte_perm(odd ? so : sm, odd ? sm : so, odd ? 0x7632 : 0x5410);
       }
     }
-    if (whole) {
-      __syncwarp();
+    __syncwarp();
+    if (a == 0 && e == kKv4Tile) {
 #pragma unroll
       for (int i = 0; i < 5; ++i)
         reinterpret_cast<uint4*>(tile)[lane + 32 * i] = reinterpret_cast<const uint4*>(stage[warp])[lane + 32 * i];
+    } else {
+#pragma unroll 4
+      for (int u = lane; u < kKv4TileBytes / 2; u += 32) {
+        const int t = kv4_unit_token(u);
+        if (t >= a && t < e) reinterpret_cast<uint16_t*>(tile)[u] = reinterpret_cast<const uint16_t*>(stage[warp])[u];
+      }
     }
   }
   if (!full) return;                                           // uniform over the CTA
+  for (int t = tok; t < min(a, kKv4Tile); t += 4) {            // the page's tokens of earlier calls
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(tile + t * 64 + part * 32 + g * 4);
+    const __half* kpar = reinterpret_cast<const __half*>(tile + kv4_kparam(t, g));
+    const uint32_t old[2] = {kw[0], kw[4]};
+    const float s = __half2float(kpar[0]), m = __half2float(kpar[4]);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    bmax[i] = fmaxf(bmax[i], __shfl_xor_sync(0xffffffffu, bmax[i], 8));
-    bmin[i] = fminf(bmin[i], __shfl_xor_sync(0xffffffffu, bmin[i], 8));
-    bmax[i] = fmaxf(bmax[i], __shfl_xor_sync(0xffffffffu, bmax[i], 16));
-    bmin[i] = fminf(bmin[i], __shfl_xor_sync(0xffffffffu, bmin[i], 16));
-    if (tok == 0) red[0][warp][lane * 16 + i] = bmax[i], red[1][warp][lane * 16 + i] = bmin[i];
+    for (int i = 0; i < 16; ++i) {
+      const float x = __fmaf_rn(s, (float)((int)((old[i >> 3] >> (4 * (i & 7))) & 15u) - 8), m);
+      bmax[i] = fmaxf(bmax[i], x);
+      bmin[i] = fminf(bmin[i], x);
+    }
   }
+  // over the four tokens of a step: first half of the channels stay with lanes of bit 3 clear, and so on
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool up = lane & 8;
+    const float gx = __shfl_xor_sync(0xffffffffu, up ? bmax[i] : bmax[i + 8], 8);
+    const float gn = __shfl_xor_sync(0xffffffffu, up ? bmin[i] : bmin[i + 8], 8);
+    bmax[i] = fmaxf(gx, up ? bmax[i + 8] : bmax[i]);
+    bmin[i] = fminf(gn, up ? bmin[i + 8] : bmin[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool up = lane & 16;
+    const float gx = __shfl_xor_sync(0xffffffffu, up ? bmax[i] : bmax[i + 4], 16);
+    const float gn = __shfl_xor_sync(0xffffffffu, up ? bmin[i] : bmin[i + 4], 16);
+    bmax[i] = fmaxf(gx, up ? bmax[i + 4] : bmax[i]);
+    bmin[i] = fminf(gn, up ? bmin[i + 4] : bmin[i]);
+  }
+  const int ch = (lane & 7) * 16 + (lane >> 3 & 1) * 8 + (lane >> 4) * 4;
+  *reinterpret_cast<float4*>(&red[0][warp][ch]) = make_float4(bmax[0], bmax[1], bmax[2], bmax[3]);
+  *reinterpret_cast<float4*>(&red[1][warp][ch]) = make_float4(bmin[0], bmin[1], bmin[2], bmin[3]);
   __syncthreads();
   if (warp != 0) return;
-  float up[4], dn[4], a = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 32 * i;
-    up[i] = red[0][0][d];
-    dn[i] = red[1][0][d];
-    for (int w = 1; w < pool.page_tiles; ++w) up[i] = fmaxf(up[i], red[0][w][d]), dn[i] = fminf(dn[i], red[1][w][d]);
-    a = fmaxf(a, fmaxf(fabsf(up[i]), fabsf(dn[i])));
+  // a lane 4 channels
+  float4 up = *reinterpret_cast<const float4*>(&red[0][0][lane * 4]), dn = *reinterpret_cast<const float4*>(&red[1][0][lane * 4]);
+  for (int w = 1; w < pool.page_tiles; ++w) {
+    const float4 x = *reinterpret_cast<const float4*>(&red[0][w][lane * 4]), y = *reinterpret_cast<const float4*>(&red[1][w][lane * 4]);
+    up = make_float4(fmaxf(up.x, x.x), fmaxf(up.y, x.y), fmaxf(up.z, x.z), fmaxf(up.w, x.w));
+    dn = make_float4(fminf(dn.x, y.x), fminf(dn.y, y.y), fminf(dn.z, y.z), fminf(dn.w, y.w));
   }
+  float top = fmaxf(fmaxf(fmaxf(fabsf(up.x), fabsf(up.y)), fmaxf(fabsf(up.z), fabsf(up.w))),
+                    fmaxf(fmaxf(fabsf(dn.x), fabsf(dn.y)), fmaxf(fabsf(dn.z), fabsf(dn.w))));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-  const float t = __fdiv_rn(a, 127.f);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float t = __fdiv_rn(top, 127.f);
   const int64_t at = (int64_t)page * pool.heads + head;
   if (lane == 0) pool.bound_scales[at] = t;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 32 * i;
-    const float u = t > 0.f ? fminf(ceilf(__fdiv_rn(up[i], t)), 127.f) : 0.f;
-    const float l = t > 0.f ? fmaxf(floorf(__fdiv_rn(dn[i], t)), -127.f) : 0.f;
-    pool.bounds[at * 256 + d] = (int8_t)(int)u;
-    pool.bounds[at * 256 + 128 + d] = (int8_t)(int)l;
-  }
+  auto code = [&](float x, bool upper) {
+    if (t <= 0.f) return 0u;
+    const float y = __fdiv_rn(x, t);
+    return (uint32_t)(int)(upper ? fminf(ceilf(y), 127.f) : fmaxf(floorf(y), -127.f)) & 255u;
+  };
+  uint32_t* bd = reinterpret_cast<uint32_t*>(pool.bounds + at * 256);
+  bd[lane] = code(up.x, true) | code(up.y, true) << 8 | code(up.z, true) << 16 | code(up.w, true) << 24;
+  bd[32 + lane] = code(dn.x, false) | code(dn.y, false) << 8 | code(dn.z, false) << 16 | code(dn.w, false) << 24;
 }
 
 // A lane's 8 channels from 8 nibbles in channel order.

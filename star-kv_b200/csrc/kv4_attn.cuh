@@ -93,9 +93,6 @@ __device__ __forceinline__ uint32_t kv4_hmul2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float2 kv4_float2(uint32_t a) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&a));
-}
 
 // Tokens of a sequence, within the block table.
 __device__ __forceinline__ int64_t kv4_length(const Kv4AttnParams& p, int b) {
@@ -251,7 +248,7 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
         const uint32_t a[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 h = kv4_float2(a[i]);
+          const float2 h = kv4_halves(a[i]);
           const bool f16 = p.q_dtype == STARKV_F16;
           f[j * 8 + 2 * i] = f16 ? h.x : __uint_as_float(a[i] << 16);
           f[j * 8 + 2 * i + 1] = f16 ? h.y : __uint_as_float(a[i] & 0xffff0000u);
@@ -342,7 +339,7 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
     ta[h] = kv4_lds128(th + at.vpar);
     tb[h] = kv4_lds128(th + at.vpar + 128);
     const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-    const float2 sa01 = kv4_float2(pa.x), sb01 = kv4_float2(pa.y), sa23 = kv4_float2(pb.x), sb23 = kv4_float2(pb.y);
+    const float2 sa01 = kv4_halves(pa.x), sb01 = kv4_halves(pa.y), sa23 = kv4_halves(pb.x), sb23 = kv4_halves(pb.y);
     const float sa[4] = {sa01.x, sa01.y, sa23.x, sa23.y}, sb[4] = {sb01.x, sb01.y, sb23.x, sb23.y};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -895,7 +892,7 @@ __global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv
       const uint2 raw = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.q) + at));
       float x[4];
       if (p.q_dtype == STARKV_F16) {
-        const float2 f0 = kv4_float2(raw.x), f1 = kv4_float2(raw.y);
+        const float2 f0 = kv4_halves(raw.x), f1 = kv4_halves(raw.y);
         x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
       } else {
         x[0] = __uint_as_float(raw.x << 16), x[1] = __uint_as_float(raw.x & 0xffff0000u);
