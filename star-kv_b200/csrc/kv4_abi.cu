@@ -76,8 +76,8 @@ int io_params(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, Kv4IoP
 template <int NT, int W, bool MASK>
 int launch_attn(const Kv4AttnParams& p, int grid, cudaStream_t st) {
   auto kern = kv4_attn_kernel<NT, W, MASK>;
-  const size_t smem = sizeof(Kv4AttnSmem<NT, W>);
-  static_assert(sizeof(Kv4AttnSmem<NT, W>) <= 227 * 1024, "shared memory of one SM");
+  const size_t smem = sizeof(Kv4AttnSmem<NT, W, MASK>);
+  static_assert(sizeof(Kv4AttnSmem<NT, W, MASK>) <= 227 * 1024, "shared memory of one SM");
   static std::atomic<uint64_t> raised{0};                      // one bit a device
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return host_launch_status();
@@ -146,7 +146,7 @@ int starkv_kv4_read(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, 
 
 int starkv_kv4_workspace_size(size_t* bytes) {
   if (!bytes) return host_error(STARKV_ERR_INVALID, "null argument");
-  *bytes = kKv4CounterBytes + (size_t)kKv4MaxGrid * 2 * kKv4PartFloats * sizeof(float);
+  *bytes = kKv4WorkspaceBytes;
   return STARKV_OK;
 }
 
@@ -211,10 +211,11 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   const int grid = sms < kKv4MaxGrid ? sms : kKv4MaxGrid;
   p.counters = (int*)a->workspace;
   p.parts = (float*)((uint8_t*)a->workspace + kKv4CounterBytes);
+  p.heads = p.parts + (size_t)kKv4MaxGrid * 2 * kKv4PartFloats;
   cudaStream_t st = (cudaStream_t)stream;
   if (nt == 1)
     return p.mask ? launch_attn<1, 15, true>(p, grid, st) : launch_attn<1, 15, false>(p, grid, st);
-  return p.mask ? launch_attn<2, 7, true>(p, grid, st) : launch_attn<2, 7, false>(p, grid, st);
+  return p.mask ? launch_attn<2, 11, true>(p, grid, st) : launch_attn<2, 11, false>(p, grid, st);
 }
 
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* a, starkv_stream_t stream) {

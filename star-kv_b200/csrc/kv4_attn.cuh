@@ -37,10 +37,14 @@
 
 namespace starkv {
 
-constexpr int kKv4MaxGrid = 256;            // CTAs the workspace has room for
-constexpr int kKv4MaxCols = 16;
-constexpr size_t kKv4PartFloats = kKv4MaxCols * 130;   // one piece: o (cols, 128), base (cols), l (cols)
-constexpr size_t kKv4CounterBytes = kKv4MaxGrid * sizeof(int);
+constexpr int kKv4MaxGrid = 160;            // CTAs the workspace has room for
+constexpr int kKv4MaxCols = 16, kKv4MaxWarps = 15;
+constexpr int kKv4PartFloats = kKv4MaxCols * 130;   // one piece: o (cols, 128), base (cols), l (cols)
+constexpr size_t kKv4CounterBytes = 1024;
+static_assert(kKv4MaxGrid * sizeof(int) <= kKv4CounterBytes, "a counter a CTA");
+// counters, two pieces a CTA for other CTAs, one a warp
+constexpr size_t kKv4WorkspaceBytes =
+    kKv4CounterBytes + (size_t)kKv4MaxGrid * (2 + kKv4MaxWarps) * kKv4PartFloats * sizeof(float);
 
 struct Kv4AttnParams {
   Kv4Pool pool;
@@ -56,6 +60,7 @@ struct Kv4AttnParams {
   const int* pages;
   int* counters;                            // (kKv4MaxGrid) zero between calls
   float* parts;                             // (grid, 2, kKv4PartFloats)
+  float* heads;                             // (grid, kKv4MaxWarps, kKv4PartFloats)
   float scaling;
   int num_selected, q_dtype, out_dtype, batch, queries, q_heads, group, width, col_blocks;
 };
@@ -138,6 +143,13 @@ __device__ __forceinline__ float kv4_weight(float base, float joint) {
   return base == -INFINITY ? 0.f : kv4_exp2(base - joint);
 }
 
+// mask[i] to shared memory, 0 where i is past its width (grouped with the thread's other copies).
+__device__ __forceinline__ void kv4_cp_async4(void* dst, const float* mask, int i, int64_t width) {
+  const int bytes = i < width ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(mask + (bytes ? i : 0)), "r"(bytes)
+               : "memory");
+}
+
 __device__ __forceinline__ uint4 kv4_lds128(uint32_t at) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
@@ -176,23 +188,20 @@ struct Kv4Piece {
   int start, b, hc, tiles;                  // first tile of its segment on the line (-1: unused)
 };
 
-template <int NT, int W>
+template <int NT, int W, bool MASK>
 struct Kv4AttnSmem {
   static constexpr int kCols = NT * 8;
-  static constexpr int kRing = 32 / W;      // stages of a warp, two tiles each
-  alignas(128) uint8_t ring[W][kRing][2][kKv4TileBytes];
-  alignas(16) float head[W][kCols * 130];
+  static constexpr int kRing = W > 11 ? 5 : 6;   // tile slots of a warp
+  static constexpr bool kQueries = NT > 1;  // B operands of the scores held here, not in registers
+  alignas(128) uint8_t ring[W][kRing][kKv4TileBytes];
+  alignas(16) uint4 queries[kQueries ? W : 1][kQueries ? NT * 4 * 32 : 1];
+  alignas(16) float mask[MASK ? W : 1][MASK ? kRing : 1][kKv4Tile];
   alignas(8) uint64_t full[W][kRing], empty[W][kRing];
-  int pos[W][kRing][2];                     // position of a tile's first token, -1: nothing to attend to
+  int pos[W][kRing];                        // position of a tile's first token, -1: nothing to attend to
   Kv4Piece piece[2 * W];
   int scan[W + 1];
   int upto[(W + 1) * 32];                   // tiles of the sequences up to and with a thread's
   int last[2];
-  // piece i: o (cols, 128), base (cols), l (cols).  The first piece of a warp has its own space,
-  // the second lies over the warp's ring.
-  __device__ __forceinline__ float* part(int i) {
-    return i & 1 ? reinterpret_cast<float*>(ring[i >> 1][0][0]) : head[i >> 1];
-  }
 };
 
 __device__ __forceinline__ uint2 kv4_lds64(uint32_t at) {
@@ -204,7 +213,7 @@ __device__ __forceinline__ uint2 kv4_lds64(uint32_t at) {
 // A lane's byte offsets within a tile, kept in registers (opaque to the compiler, which would
 // otherwise compute them anew for every load).
 struct Kv4Lane {
-  uint32_t code, kpar, kown, vpar, vmid;
+  uint32_t code, kpar, kown, vpar, vmid, row, pair;
   __device__ __forceinline__ explicit Kv4Lane(int lane) {
     const int r = lane >> 2, c = lane & 3;
     code = lane * 16;
@@ -212,6 +221,8 @@ struct Kv4Lane {
     kown = kKv4KParams + r * 32 + (c & 1) * 16;
     vpar = kKv4VParams + c * 32;
     vmid = kKv4VParams + c * 32 + 16 + (r & 1) * 8;
+    row = r * 4;                            // of the mask: the lane's rows, and its pairs of tokens
+    pair = c * 8;
     asm volatile("" : "+r"(code), "+r"(kpar), "+r"(kown), "+r"(vpar), "+r"(vmid));
   }
 };
@@ -219,7 +230,8 @@ struct Kv4Lane {
 // The columns of one segment in a warp's registers.
 template <int NT>
 struct Kv4Columns {
-  uint32_t qb[NT][4][4], qc[NT][2];         // B operands of the scores: 16 q or q by nibble; sums of q for s and m
+  uint32_t qb[1][4][4];                     // B operands of the scores, 16 q or q by nibble (NT > 1: in shared memory)
+  uint32_t qc[NT][2];                       // sums of q for s and m
   float cs[NT][2];                          // a column's scores, as computed (an eighth), to the log2 domain
   int end[NT][2];                           // first position a column does not attend to
   float o[8][NT][4], l[NT][2];
@@ -230,7 +242,7 @@ struct Kv4Columns {
 
 // Loads a segment's queries and clears its sums.
 template <int NT>
-__device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>& s, int b, int hc, int len, int lane) {
+__device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>& s, uint4* queries, int b, int hc, int len, int lane) {
   const int r = lane >> 2, c = lane & 3, head = hc / p.col_blocks, cb = hc % p.col_blocks;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -281,10 +293,12 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
         f[j * 8 + i] *= up;
         sum[j] += f[j * 8 + i];
       }
-      s.qb[nt][j][0] = kv4_half2(f[j * 8] * 16.f, f[j * 8 + 4] * 16.f);
-      s.qb[nt][j][1] = kv4_half2(f[j * 8 + 1], f[j * 8 + 5]);
-      s.qb[nt][j][2] = kv4_half2(f[j * 8 + 2] * 16.f, f[j * 8 + 6] * 16.f);
-      s.qb[nt][j][3] = kv4_half2(f[j * 8 + 3], f[j * 8 + 7]);
+      const uint4 v = make_uint4(kv4_half2(f[j * 8] * 16.f, f[j * 8 + 4] * 16.f), kv4_half2(f[j * 8 + 1], f[j * 8 + 5]),
+                                 kv4_half2(f[j * 8 + 2] * 16.f, f[j * 8 + 6] * 16.f), kv4_half2(f[j * 8 + 3], f[j * 8 + 7]));
+      if (NT == 1)
+        s.qb[0][j][0] = v.x, s.qb[0][j][1] = v.y, s.qb[0][j][2] = v.z, s.qb[0][j][3] = v.w;
+      else
+        queries[(nt * 4 + j) * 32 + lane] = v;   // read back by this lane alone
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
@@ -315,29 +329,18 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
   s.e = 0;
 }
 
-// TILES consecutive tiles at shared address tl.  MASK: an additive mask (mrow, its row).  EDGE:
-// some of their positions are beyond what a column attends to, or beyond the length.
-template <int NT, int TILES, bool MASK, bool EDGE>
-__device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, int pos, int len, const float* mrow,
-                                               int64_t mask_width, const Kv4Lane& at, int lane) {
-  const int r = lane >> 2, c = lane & 3;
-  float x[TILES][NT][4];
-  uint4 ta[TILES], tb[TILES];
-  uint32_t keep_a[TILES], keep_b[TILES];    // halves of the value parameters that count
-  bool over = false;
-  // an s above 2^e (the bits of positive fp16 numbers order like integers)
-  const uint32_t lim = (uint32_t)(15 + s.e) * 0x04000400u;
-  uint32_t big = lim;
-#pragma unroll
-  for (int h = 0; h < TILES; ++h) {
-    const uint32_t th = tl + h * kKv4TileBytes;
-    const int p0 = pos + h * kKv4Tile;
-    // ---- scores
-    const uint4 ka = kv4_lds128(th + at.code), kb = kv4_lds128(th + at.code + 512);
-    // rows r and r + 8 of s, then of m: groups 0 and 1, groups 2 and 3, and those the lane's columns of A take
-    const uint4 pa = kv4_lds128(th + at.kpar), pb = kv4_lds128(th + at.kpar + 16), own = kv4_lds128(th + at.kown);
-    ta[h] = kv4_lds128(th + at.vpar);
-    tb[h] = kv4_lds128(th + at.vpar + 128);
+// One tile at shared address tl.  MASK: its additive mask at shared address mk.  EDGE: some of its
+// positions are beyond what a column attends to, or beyond the length.
+template <int NT, bool MASK, bool EDGE>
+__device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries, uint32_t tl, int pos, int len, uint32_t mk,
+                                         const Kv4Lane& at, int lane) {
+  float x[NT][4];
+  // ---- scores
+  const uint4 ka = kv4_lds128(tl + at.code), kb = kv4_lds128(tl + at.code + 512);
+  // rows r and r + 8 of s, then of m: groups 0 and 1, groups 2 and 3, and those the lane's columns of A take
+  const uint4 pa = kv4_lds128(tl + at.kpar), pb = kv4_lds128(tl + at.kpar + 16), own = kv4_lds128(tl + at.kown);
+  uint4 ta = kv4_lds128(tl + at.vpar), tb = kv4_lds128(tl + at.vpar + 128);
+  {
     const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
     const float2 sa01 = kv4_halves(pa.x), sb01 = kv4_halves(pa.y), sa23 = kv4_halves(pb.x), sb23 = kv4_halves(pb.y);
     const float sa[4] = {sa01.x, sa01.y, sa23.x, sa23.y}, sb[4] = {sb01.x, sb01.y, sb23.x, sb23.y};
@@ -346,72 +349,64 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
       const uint32_t ua = wa[j] >> 8, ub = wb[j] >> 8;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const uint4 q = NT == 1 ? make_uint4(s.qb[0][j][0], s.qb[0][j][1], s.qb[0][j][2], s.qb[0][j][3])
+                                : queries[(nt * 4 + j) * 32 + lane];
         float d[4];
-        kv4_mma0(d, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, s.qb[nt][j][0],
-                 s.qb[nt][j][1]);
-        kv4_mma(d, ua & 0x000f000fu, ub & 0x000f000fu, ua & 0x00f000f0u, ub & 0x00f000f0u, s.qb[nt][j][2], s.qb[nt][j][3]);
-        x[h][nt][0] = j ? fmaf(sa[j], d[0], x[h][nt][0]) : sa[j] * d[0];
-        x[h][nt][1] = j ? fmaf(sa[j], d[1], x[h][nt][1]) : sa[j] * d[1];
-        x[h][nt][2] = j ? fmaf(sb[j], d[2], x[h][nt][2]) : sb[j] * d[2];
-        x[h][nt][3] = j ? fmaf(sb[j], d[3], x[h][nt][3]) : sb[j] * d[3];
+        kv4_mma0(d, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, q.x, q.y);
+        kv4_mma(d, ua & 0x000f000fu, ub & 0x000f000fu, ua & 0x00f000f0u, ub & 0x00f000f0u, q.z, q.w);
+        x[nt][0] = j ? fmaf(sa[j], d[0], x[nt][0]) : sa[j] * d[0];
+        x[nt][1] = j ? fmaf(sa[j], d[1], x[nt][1]) : sa[j] * d[1];
+        x[nt][2] = j ? fmaf(sb[j], d[2], x[nt][2]) : sb[j] * d[2];
+        x[nt][3] = j ? fmaf(sb[j], d[3], x[nt][3]) : sb[j] * d[3];
       }
     }
-    unsigned live = 0xffffu;                // MASK: tokens that are not masked out
-    float add0 = 0.f, add1 = 0.f;
-    if (MASK) {
-      const int t0 = p0 + r, t1 = t0 + 8;
-      if (t0 < len && t0 < mask_width) add0 = __ldg(mrow + t0);
-      if (t1 < len && t1 < mask_width) add1 = __ldg(mrow + t1);
-      // one bit a token: lanes c = 0 and c = 1 of row r hold tokens r and r + 8
-      const unsigned votes = __ballot_sync(0xffffffffu, (c == 0 ? add0 : add1) != -INFINITY);
-      live = 0;
-#pragma unroll
-      for (int t = 0; t < 16; ++t) live |= ((votes >> (4 * (t & 7) + (t >> 3))) & 1u) << t;
-      // beyond -2.3e38 the sum would leave fp32 in the log2 domain
-      add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
-      add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float d[4];
-      kv4_mma0(d, own.x, own.y, own.z, own.w, s.qc[nt][0], s.qc[nt][1]);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float y = fmaf(x[h][nt][u], 0x1p17f, d[u]);   // an eighth of the column's score
-        if (MASK) {
-          const float add = u & 2 ? add1 : add0;
-          y = add == -INFINITY ? -INFINITY : fmaf(y, s.cs[nt][u & 1], add);
-        }
-        if (EDGE && p0 + r + (u & 2 ? 8 : 0) >= s.end[nt][u & 1]) y = -INFINITY;
-        x[h][nt][u] = y;
-      }
-    }
-    if (MASK || EDGE) {                     // tokens that do not count may hold anything
-      const int t = p0 + 2 * c;
-      uint32_t la = (t < len ? 0xffffu : 0u) | (t + 1 < len ? 0xffff0000u : 0u);
-      uint32_t lb = (t + 8 < len ? 0xffffu : 0u) | (t + 9 < len ? 0xffff0000u : 0u);
-      if (MASK) {
-        const unsigned ba = live >> (2 * c), bb = live >> (2 * c + 8);
-        la &= (ba & 1 ? 0xffffu : 0u) | (ba & 2 ? 0xffff0000u : 0u);
-        lb &= (bb & 1 ? 0xffffu : 0u) | (bb & 2 ? 0xffff0000u : 0u);
-      }
-      ta[h].x &= la, ta[h].y &= la, ta[h].z &= la, ta[h].w &= la;
-      tb[h].x &= lb, tb[h].y &= lb, tb[h].z &= lb, tb[h].w &= lb;
-      keep_a[h] = la;
-      keep_b[h] = lb;
-    }
-    big = __vimax3_u16x2(big, __vimax3_u16x2(ta[h].x, ta[h].y, ta[h].z),
-                         __vimax3_u16x2(ta[h].w, tb[h].x, __vimax3_u16x2(tb[h].y, tb[h].z, tb[h].w)));
   }
-  over = big != lim;
+  float add0 = 0.f, add1 = 0.f;
+  if (MASK) {
+    add0 = __uint_as_float(kv4_lds32(mk + at.row));
+    add1 = __uint_as_float(kv4_lds32(mk + at.row + 32));
+    // beyond -2.3e38 the sum would leave fp32 in the log2 domain
+    add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
+    add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
+  }
+  bool over = false;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
+    float d[4];
+    kv4_mma0(d, own.x, own.y, own.z, own.w, s.qc[nt][0], s.qc[nt][1]);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float t = fmaxf(x[0][nt][u], x[0][nt][u + 2]);
-      if (TILES == 2) t = fmaxf(t, fmaxf(x[TILES - 1][nt][u], x[TILES - 1][nt][u + 2]));
-      over |= t > s.thr[nt][u];
+    for (int u = 0; u < 4; ++u) {
+      float y = fmaf(x[nt][u], 0x1p17f, d[u]);    // an eighth of the column's score
+      if (MASK) {
+        const float add = u & 2 ? add1 : add0;
+        y = add == -INFINITY ? -INFINITY : fmaf(y, s.cs[nt][u & 1], add);
+      }
+      if (EDGE && pos + (lane >> 2) + (u & 2 ? 8 : 0) >= s.end[nt][u & 1]) y = -INFINITY;
+      x[nt][u] = y;
     }
+    over |= fmaxf(x[nt][0], x[nt][2]) > s.thr[nt][0];
+    over |= fmaxf(x[nt][1], x[nt][3]) > s.thr[nt][1];
+  }
+  uint32_t la = 0xffffffffu, lb = 0xffffffffu;
+  if (MASK || EDGE) {                       // tokens that do not count may hold anything
+    if (EDGE) {
+      const int t = pos + 2 * (lane & 3);
+      la = (t < len ? 0xffffu : 0u) | (t + 1 < len ? 0xffff0000u : 0u);
+      lb = (t + 8 < len ? 0xffffu : 0u) | (t + 9 < len ? 0xffff0000u : 0u);
+    }
+    if (MASK) {                             // 0xff800000: -inf
+      const uint2 m0 = kv4_lds64(mk + at.pair), m1 = kv4_lds64(mk + at.pair + 32);
+      la &= (m0.x != 0xff800000u ? 0xffffu : 0u) | (m0.y != 0xff800000u ? 0xffff0000u : 0u);
+      lb &= (m1.x != 0xff800000u ? 0xffffu : 0u) | (m1.y != 0xff800000u ? 0xffff0000u : 0u);
+    }
+    ta.x &= la, ta.y &= la, ta.z &= la, ta.w &= la;
+    tb.x &= lb, tb.y &= lb, tb.z &= lb, tb.w &= lb;
+  }
+  // an s above 2^e (the bits of positive fp16 numbers order like integers)
+  const uint32_t lim = (uint32_t)(15 + s.e) * 0x04000400u;
+  const uint32_t big = __vimax3_u16x2(__vimax3_u16x2(ta.x, ta.y, ta.z), __vimax3_u16x2(ta.w, tb.x, tb.y),
+                                      __vimax3_u16x2(tb.z, tb.w, lim));
+  over |= big != lim;
   // ---- a score or an s that the base does not cover
   if (__any_sync(0xffffffffu, over)) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
@@ -420,8 +415,7 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float t = fmaxf(x[0][nt][u], x[0][nt][u + 2]);
-        if (TILES == 2) t = fmaxf(t, fmaxf(x[TILES - 1][nt][u], x[TILES - 1][nt][u + 2]));
+        float t = fmaxf(x[nt][u], x[nt][u + 2]);
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
@@ -443,57 +437,59 @@ __device__ __forceinline__ void kv4_tiles_step(Kv4Columns<NT>& s, uint32_t tl, i
     s.e = e_new;
   }
   // ---- weights and values
+  const uint4 va = kv4_lds128(tl + at.code + kKv4VCodes), vb = kv4_lds128(tl + at.code + kKv4VCodes + 512);
+  uint2 ma = kv4_lds64(tl + at.vmid), mb = kv4_lds64(tl + at.vmid + 128);
+  if (MASK || EDGE) ma.x &= la, ma.y &= la, mb.x &= lb, mb.y &= lb;
+  uint32_t p0[NT], p1[NT];
 #pragma unroll
-  for (int h = 0; h < TILES; ++h) {
-    const uint32_t th = tl + h * kKv4TileBytes;
-    const uint4 va = kv4_lds128(th + at.code + kKv4VCodes), vb = kv4_lds128(th + at.code + kKv4VCodes + 512);
-    uint2 ma = kv4_lds64(th + at.vmid), mb = kv4_lds64(th + at.vmid + 128);
-    if (MASK || EDGE) ma.x &= keep_a[h], ma.y &= keep_a[h], mb.x &= keep_b[h], mb.y &= keep_b[h];
-    uint32_t p0[NT], p1[NT];
+  for (int nt = 0; nt < NT; ++nt) {
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      w[u] = kv4_exp2(MASK ? x[nt][u] - s.base[nt][u & 1] : fmaf(x[nt][u], s.cs[nt][u & 1], -s.base[nt][u & 1]));
+    s.l[nt][0] += w[0] + w[2];
+    s.l[nt][1] += w[1] + w[3];
+    p0[nt] = kv4_transpose(kv4_half2(w[0], w[1]));
+    p1[nt] = kv4_transpose(kv4_half2(w[2], w[3]));
+  }
+  const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+  const uint32_t sa[4] = {ta.x, ta.y, ta.z, ta.w}, sb[4] = {tb.x, tb.y, tb.z, tb.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t ua = wa[j] >> 8, ub = wb[j] >> 8;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float w[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        w[u] = kv4_exp2(MASK ? x[h][nt][u] - s.base[nt][u & 1] : fmaf(x[h][nt][u], s.cs[nt][u & 1], -s.base[nt][u & 1]));
-      s.l[nt][0] += w[0] + w[2];
-      s.l[nt][1] += w[1] + w[3];
-      p0[nt] = kv4_transpose(kv4_half2(w[0], w[1]));
-      p1[nt] = kv4_transpose(kv4_half2(w[2], w[3]));
+      const uint32_t b0 = kv4_hmul2(p0[nt], sa[j]), b1 = kv4_hmul2(p1[nt], sb[j]);
+      kv4_mma(s.o[2 * j][nt], wa[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x000f000fu, wb[j] & 0x00f000f0u, b0, b1);
+      kv4_mma(s.o[2 * j + 1][nt], ua & 0x000f000fu, ua & 0x00f000f0u, ub & 0x000f000fu, ub & 0x00f000f0u, b0, b1);
+      // -8 * 2^-24 in rows r, -8 * 2^-20 in rows r + 8
+      kv4_mma(s.o[2 * j][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+      kv4_mma(s.o[2 * j + 1][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
     }
-    const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
-    const uint32_t sa[4] = {ta[h].x, ta[h].y, ta[h].z, ta[h].w}, sb[4] = {tb[h].x, tb[h].y, tb[h].z, tb[h].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t ua = wa[j] >> 8, ub = wb[j] >> 8;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const uint32_t b0 = kv4_hmul2(p0[nt], sa[j]), b1 = kv4_hmul2(p1[nt], sb[j]);
-        kv4_mma(s.o[2 * j][nt], wa[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x000f000fu, wb[j] & 0x00f000f0u, b0, b1);
-        kv4_mma(s.o[2 * j + 1][nt], ua & 0x000f000fu, ua & 0x00f000f0u, ub & 0x000f000fu, ub & 0x00f000f0u, b0, b1);
-        // -8 * 2^-24 in rows r, -8 * 2^-20 in rows r + 8
-        kv4_mma(s.o[2 * j][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-        kv4_mma(s.o[2 * j + 1][nt], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma.x, ma.y, mb.x, mb.y, p0[nt], p1[nt]);
   }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) kv4_mma(s.z[nt], ma.x, ma.y, mb.x, mb.y, p0[nt], p1[nt]);
 }
 
 // NT: n-tiles of 8 columns.  W: warps that compute; one more starts the copies, its lanes 2 w
-// and 2 w + 1 the two tiles of each stage of warp w.  Up to 8 columns 16 warps (4 a scheduler: enough to hide the
-// latencies of a tile's dependent steps; 8 warps that took 4 tiles a step ran at 37 % of the
-// issue slots, 2.5 TB/s); 16 columns need twice the accumulators and take 8 warps.
+// and 2 w + 1 taking turns at the tiles of warp w.  Up to 8 columns 15 warps of 128 registers
+// (about 4 a scheduler: enough to hide the latencies of a tile's dependent steps; 8
+// warps that took 4 tiles a step ran at 37 % of the issue slots, 2.5 TB/s); 16 columns need
+// twice the accumulators and take 11 warps of 168, with the queries' operands in shared memory.
 template <int NT, int W, bool MASK>
 __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  using Smem = Kv4AttnSmem<NT, W>;
+  using Smem = Kv4AttnSmem<NT, W, MASK>;
   constexpr int kCols = Smem::kCols, kRing = Smem::kRing;
-  constexpr bool kPair = false;
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int HC = p.pool.heads * p.col_blocks;
+  // piece i of the CTA: o (cols, 128), base (cols), l (cols).  A warp's last piece lies over its ring,
+  // one before it (the end of a segment that an earlier warp began) in the workspace.
+  auto piece_at = [&](int i) {
+    return i & 1 ? p.heads + ((int64_t)blockIdx.x * kKv4MaxWarps + (i >> 1)) * kKv4PartFloats
+                 : reinterpret_cast<float*>(sm.ring[i >> 1][0]);
+  };
 
   // ---- the line of tiles: total, this CTA's stretch, the warps' first sequences
   constexpr int kThreads = (W + 1) * 32;
@@ -509,7 +505,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   }
   if (lane == 31) sm.scan[warp] = upto;
   if (warp < W) {
-    if (lane < kRing) mbar_init(&sm.full[warp][lane], 1), mbar_init(&sm.empty[warp][lane], 1);
+    if (lane < kRing) mbar_init(&sm.full[warp][lane], MASK ? 2 : 1), mbar_init(&sm.empty[warp][lane], 1);
     if (lane < 2) sm.piece[2 * warp + lane].start = -1;
   }
   fence_mbar_init();
@@ -555,36 +551,34 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     seg_start -= use.t;
   }
   if (warp == W) {
-    // ---- copies.  The page of a lane's next tile is looked up a stage ahead, so that the block
+    // ---- copies.  The page of a lane's next tile is looked up a turn ahead, so that the block
     // table's latency is not waited for.
     static_assert(2 * W <= 32, "two lanes a warp");
-    const int q = lane & 1;
-    int slot = 0, parity = 1, at = 0, page = 0, tile = 0, head = 0;
-    bool more = false, there = false;       // a stage to issue; this lane's tile of it has tokens
+    int slot = lane & 1, parity = 1, at = 0, page = 0, tile = 0, head = 0, seq = 0;
+    bool more = false, there = false;       // a tile to issue; it has tokens
     auto look = [&]() {
       more = use.left > 0;
       there = false;
       if (!more) return;
-      const int n = min(2, use.here()), t = use.t + q;
       head = use.hc / p.col_blocks;
-      tile = t & (p.pool.page_tiles - 1);
-      if (q < n) {
-        int ord = t >> (p.pool.page_shift - 4);
-        if (p.pages) ord = __ldg(p.pages + ((int64_t)use.b * p.pool.heads + head) * p.num_selected + ord);
-        const int64_t pos = ((int64_t)ord << p.pool.page_shift) + tile * kKv4Tile;
-        if (ord >= 0 && pos < use.len) {    // a selected page may lie past the length, or end before it
-          at = (int)pos;
-          page = __ldg(p.table + use.b * p.table_stride + ord);
-          there = true;
-        }
+      seq = use.b;
+      tile = use.t & (p.pool.page_tiles - 1);
+      int ord = use.t >> (p.pool.page_shift - 4);
+      if (p.pages) ord = __ldg(p.pages + ((int64_t)use.b * p.pool.heads + head) * p.num_selected + ord);
+      const int64_t pos = ((int64_t)ord << p.pool.page_shift) + tile * kKv4Tile;
+      if (ord >= 0 && pos < use.len) {      // a selected page may lie past the length, or end before it
+        at = (int)pos;
+        page = __ldg(p.table + use.b * p.table_stride + ord);
+        there = true;
       }
-      use.advance(p, n);
+      use.advance(p, 1);
+      if (use.left > 0) use.advance(p, 1);  // the other lane's
     };
+    if ((lane & 1) && use.left > 0) use.advance(p, 1);
     look();
     unsigned long long idle_since = 0;
     while (__any_sync(0xffffffffu, more)) {
-      bool go = more && q == 0 && mbar_test_wait(&sm.empty[who][slot], parity);
-      go = __shfl_sync(0xffffffffu, go, lane & 30);
+      const bool go = more && mbar_test_wait(&sm.empty[who][slot], parity);
       if (!__any_sync(0xffffffffu, go)) {
         const unsigned long long now = global_timer_ns();
         if (idle_since == 0) idle_since = now;
@@ -596,62 +590,74 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
         continue;
       }
       idle_since = 0;
-      if (go && there && (unsigned)page >= (unsigned)p.pool.num_pages) {
-        record_error(p.pool.err, kDevBadPage);
-        there = false;
-      }
-      const unsigned copies = __ballot_sync(0xffffffffu, go && there) >> (lane & 30) & 3u;
-      if (go) sm.pos[who][slot][q] = there ? at : -1;
-      __syncwarp();
-      if (go && q == 0) mbar_arrive_expect_tx(&sm.full[who][slot], __popc(copies) * kKv4TileBytes);
-      __syncwarp();
       if (go) {
-        if (there) bulk_g2s(sm.ring[who][slot][q], p.pool.tile(page, head, tile), kKv4TileBytes, &sm.full[who][slot]);
-        if (++slot == kRing) slot = 0, parity ^= 1;
+        if (there && (unsigned)page >= (unsigned)p.pool.num_pages) {
+          record_error(p.pool.err, kDevBadPage);
+          there = false;
+        }
+        sm.pos[who][slot] = there ? at : -1;
+        uint64_t* bar = &sm.full[who][slot];
+        if (there) {
+          mbar_arrive_expect_tx(bar, kKv4TileBytes);
+          bulk_g2s(sm.ring[who][slot], p.pool.tile(page, head, tile), kKv4TileBytes, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+        if (MASK) {
+          if (there) {
+            const float* row = p.mask + seq * p.mask_stride;
+            if (at + kKv4Tile <= p.mask_width && (reinterpret_cast<uintptr_t>(row + at) & 15) == 0) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) cp_async16(&sm.mask[who][slot][4 * i], row + at + 4 * i);
+            } else {
+#pragma unroll 1
+              for (int i = 0; i < kKv4Tile; ++i) kv4_cp_async4(&sm.mask[who][slot][i], row, at + i, p.mask_width);
+            }
+            cp_async_arrive(bar);
+          } else {
+            mbar_arrive(bar);
+          }
+        }
+        slot += 2;
+        if (slot >= kRing) slot -= kRing, parity ^= 1;
         look();
       }
     }
   } else if (use.left > 0) {
     const Kv4Lane offsets(lane);
     Kv4Columns<NT> s;
-    int slot = 0, parity = 0, npieces = 0;
+    uint4* queries = sm.queries[Smem::kQueries ? warp : 0];
+    int slot = 0, parity = 0;
     bool ok = true;
     while (use.left > 0) {
       const int n = use.here();
-      kv4_begin<NT>(p, s, use.b, use.hc, use.len, lane);
-      const float* mrow = MASK ? p.mask + use.b * p.mask_stride : nullptr;
+      kv4_begin<NT>(p, s, queries, use.b, use.hc, use.len, lane);
 #pragma unroll 1
-      for (int i = 0; i < n; i += 2) {
+      for (int i = 0; i < n; ++i) {
         // a wait that runs out is recorded; what follows waits briefly and computes on what is there
         if (!mbar_wait(&sm.full[warp][slot], parity, ok ? kWaitLimitNs : 1000000ull)) {
           ok = false;
           if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
         }
-        const int pos = sm.pos[warp][slot][0], pos1 = sm.pos[warp][slot][1], bound = use.len - p.queries + 1;
-        const uint32_t tl = smem_u32(sm.ring[warp][slot][0]);
-        if (kPair && pos >= 0 && pos1 == pos + kKv4Tile && pos + 2 * kKv4Tile <= bound) {
-          kv4_tiles_step<NT, 2, MASK, false>(s, tl, pos, use.len, mrow, p.mask_width, offsets, lane);
-        } else {
-#pragma unroll 1
-          for (int j = 0; j < 2; ++j) {
-            const int at = j ? pos1 : pos;
-            if (at < 0) continue;
-            if (at + kKv4Tile > bound || kPair)
-              kv4_tiles_step<NT, 1, MASK, true>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, offsets, lane);
-            else
-              kv4_tiles_step<NT, 1, MASK, false>(s, tl + j * kKv4TileBytes, at, use.len, mrow, p.mask_width, offsets, lane);
-          }
+        const int pos = sm.pos[warp][slot];
+        if (pos >= 0) {
+          const uint32_t tl = smem_u32(sm.ring[warp][slot]), mk = MASK ? smem_u32(sm.mask[warp][slot]) : 0;
+          if (pos + kKv4Tile > use.len - p.queries + 1)
+            kv4_tile<NT, MASK, true>(s, queries, tl, pos, use.len, mk, offsets, lane);
+          else
+            kv4_tile<NT, MASK, false>(s, queries, tl, pos, use.len, mk, offsets, lane);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.empty[warp][slot]);   // the stage is read: its next copies may land
+        if (lane == 0) mbar_arrive(&sm.empty[warp][slot]);   // the slot is read: its next copy may land
         if (++slot == kRing) slot = 0, parity ^= 1;
       }
 
       // ---- end of the segment, or of the stretch
       const int r = lane >> 2, c = lane & 3;
       const bool whole = n == use.tiles;
-      const int pi = 2 * warp + npieces;
-      float* part = sm.part(pi);
+      // pieces 2 w: the last of warp w, 2 w + 1: one before it.  In line order the latter comes first.
+      const int pi = 2 * warp + (use.left > n);
+      float* part = piece_at(pi);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -694,7 +700,6 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
           q.hc = use.hc;
           q.tiles = use.tiles;
         }
-        ++npieces;
       }
       seg_start += use.tiles;
       use.advance(p, n);
@@ -733,12 +738,12 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     for (int col = 0; col < cols; ++col) {
       if (unit++ % (W + 1) != warp) continue;
       const bool in = members >> lane & 1;
-      const float base = in ? sm.part(lane)[kCols * 128 + col] : -INFINITY;
+      const float base = in ? piece_at(lane)[kCols * 128 + col] : -INFINITY;
       float mx = base;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       const float w = kv4_weight(base, mx);
-      float l = in ? w * sm.part(lane)[kCols * 129 + col] : 0.f;
+      float l = in ? w * piece_at(lane)[kCols * 129 + col] : 0.f;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -746,7 +751,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       for (unsigned m = members; m; m &= m - 1) {
         const int k = __ffs(m) - 1;
         const float wk = __shfl_sync(0xffffffffu, w, k);
-        const float4 v = *reinterpret_cast<const float4*>(sm.part(k) + col * 128 + lane * 4);
+        const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + col * 128 + lane * 4);
         acc.x = fmaf(wk, v.x, acc.x), acc.y = fmaf(wk, v.y, acc.y), acc.z = fmaf(wk, v.z, acc.z), acc.w = fmaf(wk, v.w, acc.w);
       }
       if (whole) {
