@@ -203,7 +203,7 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
     return host_error(STARKV_ERR_UNSUPPORTED, "too many query columns");
   if (((int64_t)a->table_width << p.pool.page_shift) > 0x7fffff00)
     return host_error(STARKV_ERR_UNSUPPORTED, "block table of 2^31 positions or more");
-  const int64_t tiles = (a->pages ? (int64_t)a->num_selected : (int64_t)a->table_width) * p.pool.page_tiles;
+  const int64_t tiles = (a->pages ? (int64_t)a->num_selected : (int64_t)a->table_width) * p.pool.page_tiles + kKv4PadTiles;
   if ((double)tiles * p.pool.heads * p.col_blocks * a->batch > 2.0e9)
     return host_error(STARKV_ERR_UNSUPPORTED, "batch * KV heads * tiles of a block table row must stay below 2e9");
   int sms = 0;

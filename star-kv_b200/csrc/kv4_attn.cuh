@@ -37,6 +37,7 @@
 
 namespace starkv {
 
+constexpr int kKv4PadTiles = 2;
 constexpr int kKv4MaxGrid = 160;            // CTAs the workspace has room for
 constexpr int kKv4MaxCols = 16, kKv4MaxWarps = 15;
 constexpr int kKv4PartFloats = kKv4MaxCols * 130;   // one piece: o (cols, 128), base (cols), l (cols)
@@ -109,21 +110,21 @@ __device__ __forceinline__ int64_t kv4_length(const Kv4AttnParams& p, int b) {
   }
   return n < 0 ? 0 : n;
 }
-// Tiles of one of its segments.
+// Tiles of one of its segments, with two that hold nothing: about what a warp's change of segment
+// costs, so that stretches with many short segments are not longer than others.
 __device__ __forceinline__ int kv4_tiles(const Kv4AttnParams& p, int64_t len) {
-  if (p.pages) return len > 0 ? p.num_selected * p.pool.page_tiles : 0;
-  return (int)((len + kKv4Tile - 1) >> 4);
+  if (len <= 0) return 0;
+  return (p.pages ? p.num_selected * p.pool.page_tiles : (int)((len + kKv4Tile - 1) >> 4)) + kKv4PadTiles;
 }
 
-// Where a column's output goes: element offset of its row, or -1 past the last column.
-__device__ __forceinline__ int64_t kv4_out_row(const Kv4AttnParams& p, int b, int hc, int col, int cols, int64_t* lse_at) {
-  const int head = hc / p.col_blocks, gcol = (hc % p.col_blocks) * cols + col;
-  if (gcol >= p.group * p.queries) return -1;
-  const int qi = gcol / p.group, qh = head * p.group + gcol % p.group;
-  *lse_at = ((int64_t)b * p.queries + qi) * p.q_heads + qh;
-  return b * p.os[0] + qi * p.os[1] + qh * p.os[2];
-}
-__device__ __forceinline__ void kv4_store4(const Kv4AttnParams& p, int64_t at, float4 o) {
+// Writes one column of a segment, a lane 4 channels: o / l and log(l) above the base.
+__device__ __forceinline__ void kv4_store_column(const Kv4AttnParams& p, int b, int hc, int col, int cols, float4 o, float base,
+                                              float l) {
+  const int lane = threadIdx.x & 31, head = hc / p.col_blocks, gcol = (hc - head * p.col_blocks) * cols + col;
+  const int qi = gcol / p.group, qh = head * p.group + gcol - qi * p.group;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;    // a NaN stays one
+  o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+  const int64_t at = b * p.os[0] + qi * p.os[1] + qh * p.os[2] + lane * 4;
   if (p.out_dtype == STARKV_F32) {
     *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = o;
   } else if (p.out_dtype == STARKV_F16) {
@@ -132,10 +133,9 @@ __device__ __forceinline__ void kv4_store4(const Kv4AttnParams& p, int64_t at, f
     __nv_bfloat162 h[2] = {__floats2bfloat162_rn(o.x, o.y), __floats2bfloat162_rn(o.z, o.w)};
     *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = *reinterpret_cast<uint2*>(h);
   }
-}
-__device__ __forceinline__ float kv4_inverse(float l) { return l > 0.f ? 1.f / l : l == 0.f ? 0.f : l; }  // a NaN stays one
-__device__ __forceinline__ float kv4_lse(float base, float l) {
-  return l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718055994531f;
+  if (p.lse && lane == 0)
+    p.lse[((int64_t)b * p.queries + qi) * p.q_heads + qh] =
+        l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718055994531f;
 }
 
 // Weight of a piece against the joint base.
@@ -184,6 +184,8 @@ struct Kv4Cursor {
   }
 };
 
+constexpr int kKv4QueryVecs = 5 * 32;       // vectors of the prepared queries of 8 columns
+
 struct Kv4Piece {
   int start, b, hc, tiles;                  // first tile of its segment on the line (-1: unused)
 };
@@ -191,14 +193,16 @@ struct Kv4Piece {
 template <int NT, int W, bool MASK>
 struct Kv4AttnSmem {
   static constexpr int kCols = NT * 8;
-  static constexpr int kRing = W > 11 ? 5 : 6;   // tile slots of a warp
-  static constexpr bool kQueries = NT > 1;  // B operands of the scores held here, not in registers
+  static constexpr int kRing = W > 11 ? 4 : 5;   // tile slots of a warp
   alignas(128) uint8_t ring[W][kRing][kKv4TileBytes];
-  alignas(16) uint4 queries[kQueries ? W : 1][kQueries ? NT * 4 * 32 : 1];
+  static constexpr int kShared = 4;         // segments whose queries are prepared once for the CTA
+  alignas(16) uint4 shared[kShared][NT * kKv4QueryVecs];
+  alignas(16) uint4 queries[W][NT * kKv4QueryVecs];   // a warp's own, for segments beyond those
   alignas(16) float mask[MASK ? W : 1][MASK ? kRing : 1][kKv4Tile];
   alignas(8) uint64_t full[W][kRing], empty[W][kRing];
   int pos[W][kRing];                        // position of a tile's first token, -1: nothing to attend to
   Kv4Piece piece[2 * W];
+  int shared_start[kShared];                // first tiles of the shared segments
   int scan[W + 1];
   int upto[(W + 1) * 32];                   // tiles of the sequences up to and with a thread's
   int last[2];
@@ -240,81 +244,83 @@ struct Kv4Columns {
   int e;
 };
 
-// Loads a segment's queries and clears its sums.
+// The queries of 8 columns of a segment as the scores' operands: five vectors a lane in `buf` (32
+// vectors apart), the four groups' B operands and { sums of q for s, for m, scale, - }.
+__device__ __forceinline__ void kv4_prepare(const Kv4AttnParams& p, uint4* buf, int b, int hc, int nt, int cols, int lane) {
+  const int r = lane >> 2, c = lane & 3, head = hc / p.col_blocks;
+  const int gcol = (hc - head * p.col_blocks) * cols + nt * 8 + r, qi = gcol / p.group;
+  const bool f16 = p.q_dtype == STARKV_F16;
+  const int64_t at = b * p.qs[0] + qi * p.qs[1] + (head * p.group + gcol - qi * p.group) * p.qs[2] + c * 8;
+  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at);
+  uint32_t raw[16];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 w = gcol < p.group * p.queries ? __ldg(src + j * 4) : make_uint4(0, 0, 0, 0);
+    raw[4 * j] = w.x, raw[4 * j + 1] = w.y, raw[4 * j + 2] = w.z, raw[4 * j + 3] = w.w;
+  }
+  uint32_t big = 0;                         // the largest magnitude's bits (they order like integers)
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) big = __vimax3_u16x2(big, raw[i] & 0x7fff7fffu, raw[i + 1] & 0x7fff7fffu);
+  big = max(big & 0xffffu, big >> 16);
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+  big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+  const float a = f16 ? kv4_halves(big).x : __uint_as_float(big << 16);
+  // q scaled by a power of two to [512, 1024) in magnitude, the scaling's sign with it; a column
+  // whose scores vanish (q or scaling below 2^-100) becomes zero
+  float up = 0.f, scale = 1.f;
+  if (!(a < 0x1p-100f) && fabsf(p.scaling) >= 0x1p-100f) {
+    const int ex = (__float_as_int(a) >> 23) - 127;
+    up = __int_as_float((127 + 9 - ex) << 23);
+    scale = fabsf(p.scaling) * 1.4426950408889634f * __int_as_float((127 - 9 + 3 + ex) << 23);
+    if (p.scaling < 0.f) up = -up;
+  }
+  float sum[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = raw[4 * j + i];
+      const float2 h = kv4_halves(w);
+      f[2 * i] = (f16 ? h.x : __uint_as_float(w << 16)) * up;
+      f[2 * i + 1] = (f16 ? h.y : __uint_as_float(w & 0xffff0000u)) * up;
+    }
+    buf[j * 32 + lane] = make_uint4(kv4_half2(f[0] * 16.f, f[4] * 16.f), kv4_half2(f[1], f[5]),
+                                    kv4_half2(f[2] * 16.f, f[6] * 16.f), kv4_half2(f[3], f[7]));
+    sum[j] = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
+  // lanes c = 0, 1: the upper parts of sums 0, 1 and 2, 3; c = 2, 3: what is left of them.
+  // An eighth of the sums (exact) for m, so that -8 times it, for s, fits fp16 too.
+  const float s0 = c & 1 ? sum[2] : sum[0], s1 = c & 1 ? sum[3] : sum[1];
+  const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
+  const float t0 = c & 2 ? s0 - h0 : h0, t1 = c & 2 ? s1 - h1 : h1;
+  buf[128 + lane] = make_uint4(kv4_half2(-t0, -t1), kv4_half2(0.125f * t0, 0.125f * t1), __float_as_uint(scale), 0);
+}
+
+// Takes a segment's prepared queries and clears its sums.
 template <int NT>
-__device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>& s, uint4* queries, int b, int hc, int len, int lane) {
-  const int r = lane >> 2, c = lane & 3, head = hc / p.col_blocks, cb = hc % p.col_blocks;
+__device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>& s, const uint4* buf, int hc, int len, int lane) {
+  const int first = hc % p.col_blocks * (NT * 8), c = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int gcol = cb * NT * 8 + nt * 8 + r;
-    float f[32];
-    if (gcol < p.group * p.queries) {
-      const int qi = gcol / p.group;
-      const int64_t at = b * p.qs[0] + qi * p.qs[1] + (head * p.group + gcol - qi * p.group) * p.qs[2] + c * 8;
-      uint4 raw[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        raw[j] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at + j * 32));
+    if (NT == 1) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t a[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 h = kv4_halves(a[i]);
-          const bool f16 = p.q_dtype == STARKV_F16;
-          f[j * 8 + 2 * i] = f16 ? h.x : __uint_as_float(a[i] << 16);
-          f[j * 8 + 2 * i + 1] = f16 ? h.y : __uint_as_float(a[i] & 0xffff0000u);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = 0.f;
-    }
-    float a = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) a = fmaxf(a, fabsf(f[i]));
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    // q scaled by a power of two to [512, 1024) in magnitude, the scaling's sign with it; a
-    // column whose scores vanish (q or scaling below 2^-100) becomes zero
-    float up = 0.f, scale = 1.f;
-    if (a >= 0x1p-100f && fabsf(p.scaling) >= 0x1p-100f) {
-      const int ex = (__float_as_int(a) >> 23) - 127;
-      up = __int_as_float((127 + 9 - ex) << 23);
-      scale = fabsf(p.scaling) * 1.4426950408889634f * __int_as_float((127 - 9 + 3 + ex) << 23);
-      if (p.scaling < 0.f) up = -up;
-    }
-    float sum[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      sum[j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        f[j * 8 + i] *= up;
-        sum[j] += f[j * 8 + i];
-      }
-      const uint4 v = make_uint4(kv4_half2(f[j * 8] * 16.f, f[j * 8 + 4] * 16.f), kv4_half2(f[j * 8 + 1], f[j * 8 + 5]),
-                                 kv4_half2(f[j * 8 + 2] * 16.f, f[j * 8 + 6] * 16.f), kv4_half2(f[j * 8 + 3], f[j * 8 + 7]));
-      if (NT == 1)
+        const uint4 v = buf[j * 32 + lane];
         s.qb[0][j][0] = v.x, s.qb[0][j][1] = v.y, s.qb[0][j][2] = v.z, s.qb[0][j][3] = v.w;
-      else
-        queries[(nt * 4 + j) * 32 + lane] = v;   // read back by this lane alone
+      }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], 2);
-    // lanes c = 0, 1: the upper parts of sums 0, 1 and 2, 3; c = 2, 3: what is left of them.
-    // An eighth of the sums (exact) for m, so that -8 times it, for s, fits fp16 too.
-    const float s0 = c & 1 ? sum[2] : sum[0], s1 = c & 1 ? sum[3] : sum[1];
-    const float h0 = __half2float(__float2half_rn(s0)), h1 = __half2float(__float2half_rn(s1));
-    const float t0 = c & 2 ? s0 - h0 : h0, t1 = c & 2 ? s1 - h1 : h1;
-    s.qc[nt][0] = kv4_half2(-t0, -t1);
-    s.qc[nt][1] = kv4_half2(0.125f * t0, 0.125f * t1);
+    const uint4 v = buf[nt * kKv4QueryVecs + 128 + lane];
+    s.qc[nt][0] = v.x;
+    s.qc[nt][1] = v.y;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      s.cs[nt][u] = __shfl_sync(0xffffffffu, scale, (2 * c + u) * 4);
-      s.end[nt][u] = len - p.queries + 1 + (cb * NT * 8 + nt * 8 + 2 * c + u) / p.group;
+      s.cs[nt][u] = __uint_as_float(__shfl_sync(0xffffffffu, v.z, (2 * c + u) * 4));
+      s.end[nt][u] = len - p.queries + 1 + (first + nt * 8 + 2 * c + u) / p.group;
       s.l[nt][u] = 0.f;
       s.base[nt][u] = 0.f;
       s.thr[nt][u] = -INFINITY;
@@ -350,7 +356,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const uint4 q = NT == 1 ? make_uint4(s.qb[0][j][0], s.qb[0][j][1], s.qb[0][j][2], s.qb[0][j][3])
-                                : queries[(nt * 4 + j) * 32 + lane];
+                                : queries[nt * kKv4QueryVecs + j * 32 + lane];
         float d[4];
         kv4_mma0(d, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, q.x, q.y);
         kv4_mma(d, ua & 0x000f000fu, ub & 0x000f000fu, ua & 0x00f000f0u, ub & 0x00f000f0u, q.z, q.w);
@@ -508,48 +514,77 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     if (lane < kRing) mbar_init(&sm.full[warp][lane], MASK ? 2 : 1), mbar_init(&sm.empty[warp][lane], 1);
     if (lane < 2) sm.piece[2 * warp + lane].start = -1;
   }
+  if (tid < Smem::kShared) sm.shared_start[tid] = -1;
   fence_mbar_init();
   __syncthreads();
-  int total = 0;
+  int warps = lane <= W ? sm.scan[lane] : 0;  // tiles up to and with a warp's
 #pragma unroll
-  for (int w = 0; w <= W; ++w) {
-    if (w < warp) upto += sm.scan[w];
-    total += sm.scan[w];
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, warps, o);
+    if (lane >= o) warps += y;
   }
+  const int total = __shfl_sync(0xffffffffu, warps, W);
+  if (warp > 0) upto += __shfl_sync(0xffffffffu, warps, warp - 1);
   sm.upto[tid] = upto;
   // equal stretches, a tile a warp at least
   const int per = max((int)((unsigned)(total + gridDim.x - 1) / gridDim.x), W);
   const int c0 = (int)min((int64_t)blockIdx.x * per, (int64_t)total), c1 = min(c0 + per, total), width = c1 - c0;
   __syncthreads();
 
+  // the cursor at tile g of the line
+  auto seek = [&](int g, int left) {
+    Kv4Cursor k;
+    int lo = 0;                             // the first thread whose sequences reach beyond g
+    if (warp < W) {                         // one g for the warp
+      const unsigned beyond = __ballot_sync(0xffffffffu, lane <= W && warps > g);
+      lo = beyond ? (__ffs(beyond) - 1) * 32 : 0;
+      const unsigned in = __ballot_sync(0xffffffffu, sm.upto[lo + lane] > g);
+      lo += in ? __ffs(in) - 1 : 0;
+    } else {
+      int hi = kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sm.upto[mid] > g) hi = mid;
+        else lo = mid + 1;
+      }
+    }
+    unsigned off = g - (lo ? sm.upto[lo - 1] : 0);
+    k.b = min(lo * per_thread, p.batch - 1);
+    k.len = (int)kv4_length(p, k.b);
+    k.tiles = kv4_tiles(p, k.len);
+    while (off >= (unsigned)(k.tiles * HC) && k.b + 1 < p.batch) {
+      off -= k.tiles * HC;
+      k.len = (int)kv4_length(p, ++k.b);
+      k.tiles = kv4_tiles(p, k.len);
+    }
+    k.hc = k.tiles ? (int)(off / (unsigned)k.tiles) : 0;
+    k.t = (int)(off - (unsigned)(k.hc * k.tiles));
+    k.left = k.tiles ? left : 0;
+    return k;
+  };
   // a warp's stretch; the last warp's lanes have the stretches of the warps they serve
   const int who = min(warp < W ? warp : lane >> 1, W - 1);
   const int g0 = c0 + width / W * who + width % W * who / W;
   const int stretch = c0 + width / W * (who + 1) + width % W * (who + 1) / W - g0;
-  Kv4Cursor use;
-  int seg_start = g0;                       // first tile of the segment at hand
-  use.left = 0;
-  if (stretch > 0 && (warp < W || lane < 2 * W)) {
-    int lo = 0, hi = kThreads - 1;          // the first thread whose sequences reach beyond g0
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (sm.upto[mid] > g0) hi = mid;
-      else lo = mid + 1;
+  if (warp < W) {
+    // the queries of the CTA's first segments, a warp 8 columns of one
+    if (warp < Smem::kShared * NT && width > 0) {
+      Kv4Cursor k = seek(c0, width);
+      int start = c0 - k.t;
+      for (int i = 0; i < warp / NT && k.left > 0; ++i) {
+        start += k.tiles;
+        k.advance(p, k.here());
+      }
+      if (k.left > 0) {
+        kv4_prepare(p, sm.shared[warp / NT] + warp % NT * kKv4QueryVecs, k.b, k.hc, warp % NT, kCols, lane);
+        if (lane == 0 && warp % NT == 0) sm.shared_start[warp / NT] = start;
+      }
     }
-    unsigned off = g0 - (lo ? sm.upto[lo - 1] : 0);
-    use.b = min(lo * per_thread, p.batch - 1);
-    use.len = (int)kv4_length(p, use.b);
-    use.tiles = kv4_tiles(p, use.len);
-    while (off >= (unsigned)(use.tiles * HC) && use.b + 1 < p.batch) {
-      off -= use.tiles * HC;
-      use.len = (int)kv4_length(p, ++use.b);
-      use.tiles = kv4_tiles(p, use.len);
-    }
-    use.hc = use.tiles ? (int)(off / (unsigned)use.tiles) : 0;
-    use.t = (int)(off - (unsigned)(use.hc * use.tiles));
-    use.left = use.tiles ? stretch : 0;
-    seg_start -= use.t;
+    named_bar_sync(1, W * 32);
   }
+  Kv4Cursor use{};
+  if (stretch > 0 && (warp < W || lane < 2 * W)) use = seek(g0, stretch);
+  int seg_start = g0 - use.t;               // first tile of the segment at hand
   if (warp == W) {
     // ---- copies.  The page of a lane's next tile is looked up a turn ahead, so that the block
     // table's latency is not waited for.
@@ -564,7 +599,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       seq = use.b;
       tile = use.t & (p.pool.page_tiles - 1);
       int ord = use.t >> (p.pool.page_shift - 4);
-      if (p.pages) ord = __ldg(p.pages + ((int64_t)use.b * p.pool.heads + head) * p.num_selected + ord);
+      if (p.pages) ord = ord < p.num_selected ? __ldg(p.pages + ((int64_t)use.b * p.pool.heads + head) * p.num_selected + ord) : -1;
       const int64_t pos = ((int64_t)ord << p.pool.page_shift) + tile * kKv4Tile;
       if (ord >= 0 && pos < use.len) {      // a selected page may lie past the length, or end before it
         at = (int)pos;
@@ -626,12 +661,22 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   } else if (use.left > 0) {
     const Kv4Lane offsets(lane);
     Kv4Columns<NT> s;
-    uint4* queries = sm.queries[Smem::kQueries ? warp : 0];
     int slot = 0, parity = 0;
     bool ok = true;
     while (use.left > 0) {
       const int n = use.here();
-      kv4_begin<NT>(p, s, queries, use.b, use.hc, use.len, lane);
+      const uint4* queries = nullptr;
+#pragma unroll
+      for (int i = 0; i < Smem::kShared; ++i)
+        if (sm.shared_start[i] == seg_start) queries = sm.shared[i];
+      if (!queries) {
+        __syncwarp();                       // the segment before is done with them
+        for (int nt = 0; nt < NT; ++nt)
+          kv4_prepare(p, sm.queries[warp] + nt * kKv4QueryVecs, use.b, use.hc, nt, kCols, lane);
+        __syncwarp();
+        queries = sm.queries[warp];
+      }
+      kv4_begin<NT>(p, s, queries, use.hc, use.len, lane);
 #pragma unroll 1
       for (int i = 0; i < n; ++i) {
         // a wait that runs out is recorded; what follows waits briefly and computes on what is there
@@ -654,8 +699,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 
       // ---- end of the segment, or of the stretch
       const int r = lane >> 2, c = lane & 3;
-      const bool whole = n == use.tiles;
-      // pieces 2 w: the last of warp w, 2 w + 1: one before it.  In line order the latter comes first.
+      const int real = min(kCols, p.group * p.queries - use.hc % p.col_blocks * kCols);
+      // pieces 2 w: the last of warp w, 2 w + 1: one before it
       const int pi = 2 * warp + (use.left > n);
       float* part = piece_at(pi);
 #pragma unroll
@@ -663,43 +708,36 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int col = nt * 8 + 2 * c + u;
-          const bool real = (use.hc % p.col_blocks) * kCols + col < p.group * p.queries;
           float l = s.l[nt][u];
           l += __shfl_xor_sync(0xffffffffu, l, 4);
           l += __shfl_xor_sync(0xffffffffu, l, 8);
           l += __shfl_xor_sync(0xffffffffu, l, 16);
-          int64_t row = 0, lse_at = 0;
-          float inv = 1.f;
-          if (whole) {
-            row = kv4_out_row(p, use.b, use.hc, col, kCols, &lse_at);
-            inv = kv4_inverse(l);
-            if (row >= 0 && r == 0 && p.lse) p.lse[lse_at] = kv4_lse(s.base[nt][u], l);
-          } else if (r == 0) {
+          if (r == 0) {
             part[kCols * 128 + col] = s.thr[nt][u] == -INFINITY ? -INFINITY : s.base[nt][u];
             part[kCols * 129 + col] = l;
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float y = __shfl_sync(0xffffffffu, s.z[nt][u + 2 * (j & 1)], (j >> 1) * 4 + c);
-            const float4 v = make_float4(
-                fmaf(s.o[2 * j][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j][nt][u + 2], 0x1p20f, y) * inv,
-                fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y) * inv, fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y) * inv);
-            const int d = j * 32 + 4 * r;
-            if (!whole) {
-              if (real) *reinterpret_cast<float4*>(part + col * 128 + d) = v;
-            } else if (row >= 0) {
-              kv4_store4(p, row + d, v);
-            }
+            if (col < real)
+              *reinterpret_cast<float4*>(part + col * 128 + j * 32 + 4 * r) =
+                  make_float4(fmaf(s.o[2 * j][nt][u], 0x1p24f, y), fmaf(s.o[2 * j][nt][u + 2], 0x1p20f, y),
+                              fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y), fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y));
           }
         }
-      if (!whole) {
-        if (lane == 0) {
-          Kv4Piece& q = sm.piece[pi];
-          q.start = seg_start;
-          q.b = use.b;
-          q.hc = use.hc;
-          q.tiles = use.tiles;
-        }
+      if (n == use.tiles) {                 // the whole segment
+        __syncwarp();
+#pragma unroll 1
+        for (int col = 0; col < real; ++col)
+          kv4_store_column(p, use.b, use.hc, col, kCols, *reinterpret_cast<const float4*>(part + col * 128 + lane * 4),
+                           part[kCols * 128 + col], part[kCols * 129 + col]);
+        __syncwarp();
+      } else if (lane == 0) {
+        Kv4Piece& q = sm.piece[pi];
+        q.start = seg_start;
+        q.b = use.b;
+        q.hc = use.hc;
+        q.tiles = use.tiles;
       }
       seg_start += use.tiles;
       use.advance(p, n);
@@ -708,86 +746,98 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   // sequences without a tile: nothing to attend to
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
     if (kv4_length(p, b) == 0)
-      for (int i = tid; i < HC * kCols * 32; i += kThreads) {
-        int64_t lse_at;
-        const int64_t row = kv4_out_row(p, b, i / (kCols * 32), i / 32 % kCols, kCols, &lse_at);
-        if (row < 0) continue;
-        kv4_store4(p, row + i % 32 * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (p.lse && i % 32 == 0) p.lse[lse_at] = -INFINITY;
-      }
+#pragma unroll 1
+      for (int i = warp; i < HC * kCols; i += W + 1)
+        if ((i / kCols % p.col_blocks) * kCols + i % kCols < p.group * p.queries)
+          kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
   if (c0 >= c1) return;
   __syncthreads();
 
-  // ---- merge the pieces of each segment, in line order.  A warp takes a (segment, column): a
-  // lane a piece for the weights, then a lane 4 channels.  What is not whole here goes to the
-  // workspace: at most the CTA's first and last segment.
+  // ---- merge the pieces of each segment, in line order.  A lane has a piece, the lowest of a
+  // segment's pieces leads; a warp takes a (segment, column): a lane a piece for the weights,
+  // then a lane 4 channels.  What is not whole here goes to the workspace: at most the CTA's
+  // first and last segment.
   static_assert(2 * W <= 32, "a lane a piece");
-  const int my_start = lane < 2 * W ? sm.piece[lane].start : -1;
-  const unsigned pieces = __ballot_sync(0xffffffffu, my_start >= 0);
-  int unit = 0, cross[2] = {-1, -1};        // cross: a piece of the segments that other CTAs share
-  for (unsigned todo = pieces; todo;) {
-    const int one = __ffs(todo) - 1;
-    const Kv4Piece pc = sm.piece[one];
-    const unsigned members = __ballot_sync(0xffffffffu, my_start == pc.start);
-    todo &= ~members;
-    const bool whole = pc.start >= c0 && pc.start + pc.tiles <= c1;
-    const int side = pc.start <= c0 ? 0 : 1;
-    if (!whole) cross[side] = one;
-    float* part = p.parts + ((int64_t)blockIdx.x * 2 + side) * kKv4PartFloats;
-    const int cols = min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols);
-    for (int col = 0; col < cols; ++col) {
-      if (unit++ % (W + 1) != warp) continue;
-      const bool in = members >> lane & 1;
-      const float base = in ? piece_at(lane)[kCols * 128 + col] : -INFINITY;
-      float mx = base;
+  const Kv4Piece pc = sm.piece[min(lane, 2 * W - 1)];
+  const int my_start = lane < 2 * W ? pc.start : -1;
+  const unsigned same = __match_any_sync(0xffffffffu, my_start);
+  const bool leads = my_start >= 0 && __ffs(same) - 1 == lane;
+  const bool whole = pc.start >= c0 && pc.start + pc.tiles <= c1;
+  const int side = pc.start <= c0 ? 0 : 1;
+  const int cols = leads ? min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols) : 0;
+  int units = cols;                         // up to and with a leader's
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float w = kv4_weight(base, mx);
-      float l = in ? w * piece_at(lane)[kCols * 129 + col] : 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, units, o);
+    if (lane >= o) units += y;
+  }
+  const int all_units = __shfl_sync(0xffffffffu, units, 31);
+  int cross[2];                             // leaders of the segments that other CTAs share, or -1
+  cross[0] = __ffs(__ballot_sync(0xffffffffu, leads && !whole && side == 0)) - 1;
+  cross[1] = __ffs(__ballot_sync(0xffffffffu, leads && !whole && side == 1)) - 1;
+#pragma unroll 1
+  for (int u = warp; u < all_units; u += W + 1) {
+    const int lead = __ffs(__ballot_sync(0xffffffffu, units > u)) - 1;
+    const unsigned members = __shfl_sync(0xffffffffu, same, lead);
+    const int col = u - __shfl_sync(0xffffffffu, units - cols, lead);
+    const bool in = members >> lane & 1;
+    const float* at = piece_at(in ? lane : lead);
+    const float base = in ? at[kCols * 128 + col] : -INFINITY;
+    float mx = base, l = in ? at[kCols * 129 + col] : 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (unsigned m = members; m; m &= m - 1) {
-        const int k = __ffs(m) - 1;
-        const float wk = __shfl_sync(0xffffffffu, w, k);
-        const float4 v = *reinterpret_cast<const float4*>(piece_at(k) + col * 128 + lane * 4);
-        acc.x = fmaf(wk, v.x, acc.x), acc.y = fmaf(wk, v.y, acc.y), acc.z = fmaf(wk, v.z, acc.z), acc.w = fmaf(wk, v.w, acc.w);
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float w = kv4_weight(base, mx);
+    l *= w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (unsigned m = members; m;) {        // four pieces a turn, their loads in flight together
+      float4 v[4];
+      float wk[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = m ? __ffs(m) - 1 : lead;
+        wk[i] = __shfl_sync(0xffffffffu, w, k);
+        if (!m) wk[i] = 0.f;
+        v[i] = *reinterpret_cast<const float4*>(piece_at(k) + col * 128 + lane * 4);
+        m &= m - 1;
       }
-      if (whole) {
-        int64_t lse_at;
-        const int64_t row = kv4_out_row(p, pc.b, pc.hc, col, kCols, &lse_at);
-        const float inv = kv4_inverse(l);
-        kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-        if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
-      } else {
-        __stcg(reinterpret_cast<float4*>(part + col * 128 + lane * 4), acc);
-        if (lane == 0) {
-          __stcg(part + kCols * 128 + col, mx);
-          __stcg(part + kCols * 129 + col, l);
-        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc.x = fmaf(wk[i], v[i].x, acc.x), acc.y = fmaf(wk[i], v[i].y, acc.y), acc.z = fmaf(wk[i], v[i].z, acc.z),
+        acc.w = fmaf(wk[i], v[i].w, acc.w);
+    }
+    if (__shfl_sync(0xffffffffu, whole, lead)) {
+      kv4_store_column(p, __shfl_sync(0xffffffffu, pc.b, lead), __shfl_sync(0xffffffffu, pc.hc, lead), col, kCols, acc, mx, l);
+    } else {
+      float* part = p.parts + ((int64_t)blockIdx.x * 2 + __shfl_sync(0xffffffffu, side, lead)) * kKv4PartFloats;
+      __stcg(reinterpret_cast<float4*>(part + col * 128 + lane * 4), acc);
+      if (lane == 0) {
+        __stcg(part + kCols * 128 + col, mx);
+        __stcg(part + kCols * 129 + col, l);
       }
     }
   }
   if (cross[0] < 0 && cross[1] < 0) return; // the same for every warp
-  __threadfence();
   __syncthreads();
   if (tid < 2 && cross[tid] >= 0) {
     const Kv4Piece pc = sm.piece[cross[tid]];
     const int first = pc.start / per, n = (pc.start + pc.tiles - 1) / per - first + 1;
-    const bool last = atomicAdd(p.counters + first, 1) == n - 1;
-    sm.last[tid] = last;
-    if (last) p.counters[first] = 0;
+    // releases what the CTA wrote before the barrier, acquires what the others did
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + first) : "memory");
+    sm.last[tid] = before == n - 1;
+    if (before == n - 1) p.counters[first] = 0;
   }
   __syncthreads();
-  unit = 0;
+  int unit = 0;
 #pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    if (cross[side] < 0 || !sm.last[side]) continue;
+  for (int s = 0; s < 2; ++s) {
+    if (cross[s] < 0 || !sm.last[s]) continue;
     // every CTA's piece is there.  The segment's piece of a CTA is its first one, but for the CTA
     // in whose middle it starts
-    __threadfence();
-    const Kv4Piece pc = sm.piece[cross[side]];
+    const Kv4Piece pc = sm.piece[cross[s]];
     const int first = pc.start / per, n = (pc.start + pc.tiles - 1) / per - first + 1;
     const int skip = pc.start > first * per ? 1 : 0;
     const int cols = min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols);
@@ -795,35 +845,35 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       if (unit++ % (W + 1) != warp) continue;
       float mx = -INFINITY, l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k0 = 0; k0 < n; k0 += 32) {
-        const int k = k0 + lane;
+      for (int k0 = 0; k0 < n; k0 += 16) {  // 16 pieces a turn, their loads in flight together
+        const int k = k0 + (lane & 15);
         const float* pk = p.parts + ((int64_t)(first + k) * 2 + (k == 0 ? skip : 0)) * kKv4PartFloats;
         const float base = k < n ? __ldcg(pk + kCols * 128 + col) : -INFINITY;
         const float lk = k < n ? __ldcg(pk + kCols * 129 + col) : 0.f;
+        float4 v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          v[i] = __ldcg(reinterpret_cast<const float4*>(
+              p.parts + ((int64_t)(first + min(k0 + i, n - 1)) * 2 + (min(k0 + i, n - 1) == 0 ? skip : 0)) * kKv4PartFloats +
+              col * 128 + lane * 4));       // past the last piece: that one again, times 0
         float joint = fmaxf(mx, base);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) joint = fmaxf(joint, __shfl_xor_sync(0xffffffffu, joint, o));
+        for (int o = 8; o > 0; o >>= 1) joint = fmaxf(joint, __shfl_xor_sync(0xffffffffu, joint, o));
         const float w = kv4_weight(base, joint), old = kv4_weight(mx, joint);
         float sum = k < n ? w * lk : 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         l = l * old + sum;
         acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
         mx = joint;
-        const int count = min(32, n - k0);
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
           const float wi = __shfl_sync(0xffffffffu, w, i);
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(
-              p.parts + ((int64_t)(first + k0 + i) * 2 + (k0 + i == 0 ? skip : 0)) * kKv4PartFloats + col * 128 + lane * 4));
-          acc.x = fmaf(wi, v.x, acc.x), acc.y = fmaf(wi, v.y, acc.y), acc.z = fmaf(wi, v.z, acc.z), acc.w = fmaf(wi, v.w, acc.w);
+          acc.x = fmaf(wi, v[i].x, acc.x), acc.y = fmaf(wi, v[i].y, acc.y), acc.z = fmaf(wi, v[i].z, acc.z),
+          acc.w = fmaf(wi, v[i].w, acc.w);
         }
       }
-      int64_t lse_at;
-      const int64_t row = kv4_out_row(p, pc.b, pc.hc, col, kCols, &lse_at);
-      const float inv = kv4_inverse(l);
-      kv4_store4(p, row + lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-      if (p.lse && lane == 0) p.lse[lse_at] = kv4_lse(mx, l);
+      kv4_store_column(p, pc.b, pc.hc, col, kCols, acc, mx, l);
     }
   }
 }
