@@ -417,7 +417,9 @@ typedef struct starkv_kv4_select_args {
   int64_t table_stride;
   const int32_t* lengths;
   int32_t* pages_out;
-  float* scores;              /* scratch, (B, Hkv, table_width) */
+  void* workspace;            /* starkv_kv4_select_workspace_size bytes, the first 256 KiB zeroed before its first use (each
+                                 call leaves them zero).  One call at a time may use it. */
+  size_t workspace_bytes;
   int32_t q_dtype;
   int32_t batch;
   int32_t num_queries;
@@ -428,6 +430,7 @@ typedef struct starkv_kv4_select_args {
   int32_t num_last;           /* >= 1 */
 } starkv_kv4_select_args;
 
+int starkv_kv4_select_workspace_size(const starkv_kv4_cache* cache, int32_t batch, int32_t table_width, size_t* bytes);
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* args, starkv_stream_t stream);
 
 /* sizeof of the four structs above, in order (ABI check for bindings). */

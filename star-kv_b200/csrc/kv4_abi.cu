@@ -218,6 +218,12 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   return p.mask ? launch_attn<2, 11, true>(p, grid, st) : launch_attn<2, 11, false>(p, grid, st);
 }
 
+int starkv_kv4_select_workspace_size(const starkv_kv4_cache* cache, int32_t batch, int32_t table_width, size_t* bytes) {
+  if (!cache || !bytes || batch < 0 || table_width < 0) return host_error(STARKV_ERR_INVALID, "bad argument");
+  *bytes = kKv4MaxSegments * sizeof(int) + (size_t)batch * cache->num_kv_heads * table_width * sizeof(float);
+  return STARKV_OK;
+}
+
 int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_args* a, starkv_stream_t stream) {
   Kv4SelectParams p;
   memset(&p, 0, sizeof(p));
@@ -233,8 +239,13 @@ int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_arg
   if (a->num_first < 0 || a->num_last < 1 || (int64_t)a->num_first + a->num_last > a->num_selected)
     return host_error(STARKV_ERR_INVALID, "num_selected must hold num_first >= 0 and num_last >= 1 pages");
   if (a->batch == 0) return STARKV_OK;
-  if (!a->block_table || !a->lengths || !a->pages_out || !a->scores)
+  if (!a->block_table || !a->lengths || !a->pages_out || !a->workspace)
     return host_error(STARKV_ERR_INVALID, "null argument");
+  if ((int64_t)a->batch * p.pool.heads > kKv4MaxSegments)
+    return host_error(STARKV_ERR_UNSUPPORTED, "kv4 selection takes batch * KV heads up to 65536");
+  size_t need = 0;
+  starkv_kv4_select_workspace_size(cache, a->batch, a->table_width, &need);
+  if (a->workspace_bytes < need) return host_error(STARKV_ERR_WORKSPACE, "kv4 selection workspace too small");
   if ((rc = check_rows(a->q, a->q_strides, 2, "q rows must be 16-byte aligned"))) return rc;
   if (reinterpret_cast<uintptr_t>(p.pool.bounds) % 16)
     return host_error(STARKV_ERR_INVALID, "kv4 bounds must be 16-byte aligned");
@@ -244,7 +255,8 @@ int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_arg
   p.table_stride = a->table_stride;
   p.lengths = a->lengths;
   p.out = a->pages_out;
-  p.scores = a->scores;
+  p.counters = (int*)a->workspace;
+  p.scores = (float*)((uint8_t*)a->workspace + kKv4MaxSegments * sizeof(int));
   p.batch = a->batch;
   p.queries = a->num_queries;
   p.q_heads = a->num_q_heads;
@@ -258,15 +270,13 @@ int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_arg
   if (((int64_t)a->table_width << p.pool.page_shift) > 0x7fffff00)
     return host_error(STARKV_ERR_UNSUPPORTED, "block table of 2^31 positions or more");
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)p.pool.heads, (unsigned)p.batch);
-  if (p.width > p.keep) {                   // else no sequence has pages to drop
-    const int chunk = kKv4ScoreWarps * kKv4ScorePages;
-    kv4_score_kernel<<<dim3((unsigned)((p.width + chunk - 1) / chunk), grid.x, grid.y), kKv4ScoreWarps * 32, 0, st>>>(p);
-  }
-  if (p.width <= kKv4SelThreads * kKv4SelRegs)
-    kv4_select_kernel<true><<<grid, kKv4SelThreads, 0, st>>>(p);
+  const dim3 grid((unsigned)((p.width + kKv4ScoreChunk - 1) / kKv4ScoreChunk), (unsigned)p.pool.heads, (unsigned)p.batch);
+  if (p.width <= 8 * kKv4SelThreads)
+    kv4_select_kernel<8><<<grid, kKv4SelThreads, 0, st>>>(p);
+  else if (p.width <= 32 * kKv4SelThreads)
+    kv4_select_kernel<32><<<grid, kKv4SelThreads, 0, st>>>(p);
   else
-    kv4_select_kernel<false><<<grid, kKv4SelThreads, 0, st>>>(p);
+    kv4_select_kernel<0><<<grid, kKv4SelThreads, 0, st>>>(p);
   return host_launch_status();
 }
 

@@ -886,7 +886,8 @@ struct Kv4SelectParams {
   int64_t table_stride;
   const int* lengths;
   int* out;
-  float* scores;
+  int* counters;                            // (batch, KV heads) zero between calls
+  float* scores;                            // (batch, KV heads, width)
   int q_dtype, batch, queries, q_heads, group, width, keep, first, last;
 };
 
@@ -907,18 +908,123 @@ __device__ __forceinline__ uint32_t kv4_key_of(float s) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// ---- page scores: a warp takes 8 pages, a lane 4 channels of their bounds.  Per page and
-// column two dp4a (the positive codes against the upper bounds, the negative ones
-// against the lower) and one warp sum; bound by the bounds' bytes (256 a page and head).
-constexpr int kKv4ScoreWarps = 8, kKv4ScorePages = 8, kKv4ScoreCols = 16;
+constexpr int kKv4SelWarps = 8, kKv4SelThreads = kKv4SelWarps * 32;
+constexpr int kKv4ScorePages = 8;           // pages of a warp
+constexpr int kKv4ScoreChunk = kKv4SelWarps * kKv4ScorePages, kKv4ScoreCols = 16;
+constexpr int kKv4MaxSegments = 65536;      // (sequence, KV head) pairs the counters have room for
 
-__global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv4SelectParams p) {
-  __shared__ int pos[kKv4ScoreCols][32], neg[kKv4ScoreCols][32];
-  __shared__ float unit[kKv4ScoreCols];
+struct Kv4SelectSmem {
+  int pos[kKv4ScoreCols][32], neg[kKv4ScoreCols][32];   // positive and negative query codes, four a word
+  float unit[kKv4ScoreCols];
+  uint32_t lane[2][kKv4SelWarps];           // a value a warp, two sets in turn
+  int last;
+};
+
+// The pages to keep of one (KV head, sequence), by its last CTA: thread t has the keys of the pages
+// [t * per, (t + 1) * per) (REGS > 0: in registers), the smallest key to keep is found bit by bit
+// below the bits that all keys share, and scans put the kept pages in order.
+template <int REGS>
+__device__ __forceinline__ void kv4_choose(const Kv4SelectParams& p, Kv4SelectSmem& sm, const float* sc, int* out, int n) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (n + kKv4SelThreads - 1) / kKv4SelThreads, i0 = min(tid * per, n), mine = min(per, n - i0);
+  auto forced = [&](int i) { return i < p.first || i >= n - p.last; };
+  uint32_t held[REGS ? REGS : 1];
+  if (REGS) {
+#pragma unroll
+    for (int i = 0; i < REGS; ++i) held[i] = i < mine && !forced(i0 + i) ? kv4_key_of(__ldcg(sc + i0 + i)) : 0;
+  }
+  // f(page, key) over this thread's scored pages
+  auto each = [&](auto f) {
+    if (REGS) {
+#pragma unroll
+      for (int i = 0; i < REGS; ++i)
+        if (i < mine && !forced(i0 + i)) f(i0 + i, held[i]);
+    } else {
+      for (int i = i0; i < i0 + mine; ++i)
+        if (!forced(i)) f(i, kv4_key_of(__ldcg(sc + i)));
+    }
+  };
+  int turn = 0;
+  // one value a warp, exchanged: lane w < 8 gets warp w's
+  auto exchange = [&](uint32_t x) {
+    if (lane == 0) sm.lane[turn][warp] = x;
+    __syncthreads();
+    const uint32_t y = sm.lane[turn][lane & (kKv4SelWarps - 1)];
+    turn ^= 1;
+    return y;
+  };
+  // what all threads before this one hold, and what all hold
+  auto scan = [&](int x, int* all) {
+    int y = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    const int w = (int)exchange((uint32_t)__shfl_sync(0xffffffffu, y, 31));
+    *all = __reduce_add_sync(0xffffffffu, lane < kKv4SelWarps ? w : 0);
+    return y - x + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
+  };
+  const int need = p.keep - p.first - p.last;   // of the scored pages; there are more
+  uint32_t ones = 0xffffffffu, any = 0;
+  each([&](int, uint32_t k) { ones &= k, any |= k; });
+  ones = __reduce_and_sync(0xffffffffu, exchange(__reduce_and_sync(0xffffffffu, ones)));
+  any = __reduce_or_sync(0xffffffffu, exchange(__reduce_or_sync(0xffffffffu, any)));
+  // the largest key with at least `need` keys at or above it
+  const int top = 31 - __clz(ones ^ any);
+  uint32_t key = top < 0 ? ones : ones >> top >> 1 << top << 1;
+  bool exact = false;                       // exactly `need`
+  for (int bit = top; bit >= 0 && !exact; --bit) {
+    const uint32_t trial = key | (1u << bit);
+    int c = 0;
+    each([&](int, uint32_t k) { c += k >= trial; });
+    c = (int)exchange((uint32_t)__reduce_add_sync(0xffffffffu, c));
+    c = __reduce_add_sync(0xffffffffu, lane < kKv4SelWarps ? c : 0);
+    if (c >= need) key = trial;
+    exact = c == need;
+  }
+  int above = 0, equal = 0, total = 0, take = 0x7fffffff;
+  each([&](int, uint32_t k) { above += k > key, equal += k == key; });
+  if (!exact) {                             // of the keys equal to it only the first
+    const int before = scan(equal, &total);
+    int all_above;
+    scan(above, &all_above);
+    take = max(0, need - all_above - before);
+  }
+  take = min(equal, take);
+  int pinned = 0;
+  for (int i = i0; i < i0 + mine; ++i) pinned += forced(i);
+  int at = scan(above + take + pinned, &total);
+  if (REGS) {
+#pragma unroll
+    for (int i = 0; i < REGS; ++i)
+      if (i < mine && (forced(i0 + i) || held[i] > key || (held[i] == key && take-- > 0))) out[at++] = i0 + i;
+  } else {
+    for (int i = i0; i < i0 + mine; ++i) {
+      const uint32_t k = kv4_key_of(__ldcg(sc + i));
+      if (forced(i) || k > key || (k == key && take-- > 0)) out[at++] = i;
+    }
+  }
+}
+
+// ---- selection.  A CTA scores 64 pages of one (KV head, sequence): a warp takes 8, a lane 4
+// channels of their bounds; per page and column two dp4a (the positive codes against the
+// upper bounds, the negative ones against the lower) and one warp sum.  Bound by the bounds'
+// bytes (256 a page and head).  The CTA that is done last keeps the best pages.
+template <int REGS>
+__global__ void __launch_bounds__(kKv4SelThreads) kv4_select_kernel(const Kv4SelectParams p) {
+  __shared__ Kv4SelectSmem sm;
   const int head = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = kv4_pages(p, b), lo = p.first, hi = n - p.last;   // the pages to score
-  const int p0 = lo + (blockIdx.x * kKv4ScoreWarps + warp) * kKv4ScorePages;
-  if (n <= p.keep || lo + (int)blockIdx.x * kKv4ScoreWarps * kKv4ScorePages >= hi) return;
+  const int64_t seg = (int64_t)b * p.pool.heads + head;
+  int* out = p.out + seg * p.keep;
+  if (n <= p.keep) {
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i < p.keep; i += kKv4SelThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  if (lo + (int)blockIdx.x * kKv4ScoreChunk >= hi) return;
+  const int p0 = lo + (blockIdx.x * kKv4SelWarps + warp) * kKv4ScorePages;
   // the pages' bounds, all in flight together
   int page = -1;
   if (lane < kKv4ScorePages && p0 + lane < hi) page = kv4_page(p.pool, p.table + b * p.table_stride, p0 + lane, p.width);
@@ -941,7 +1047,7 @@ __global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv
   for (int c0 = 0; c0 < cols; c0 += kKv4ScoreCols) {
     const int nc = min(kKv4ScoreCols, cols - c0);
     if (c0) __syncthreads();
-    for (int col = warp; col < nc; col += kKv4ScoreWarps) {
+    for (int col = warp; col < nc; col += kKv4SelWarps) {
       const int gc = c0 + col;
       const int64_t at = b * p.qs[0] + (gc / p.group) * p.qs[1] + (head * p.group + gc % p.group) * p.qs[2] + lane * 4;
       const uint2 raw = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p.q) + at));
@@ -964,14 +1070,14 @@ __global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv
         wp |= (uint32_t)max(c, 0) << (8 * i);
         wn |= (uint32_t)(min(c, 0) & 255) << (8 * i);
       }
-      pos[col][lane] = (int)wp;
-      neg[col][lane] = (int)wn;
-      if (lane == 0) unit[col] = u;
+      sm.pos[col][lane] = (int)wp;
+      sm.neg[col][lane] = (int)wn;
+      if (lane == 0) sm.unit[col] = u;
     }
     __syncthreads();
     for (int col = 0; col < nc; ++col) {
-      const int wp = pos[col][lane], wn = neg[col][lane];
-      const float u = unit[col];
+      const int wp = sm.pos[col][lane], wn = sm.neg[col][lane];
+      const float u = sm.unit[col];
 #pragma unroll
       for (int i = 0; i < kKv4ScorePages; ++i) {
         const int dot = __reduce_add_sync(0xffffffffu, __dp4a(wp, up[i], __dp4a(wn, dn[i], 0)));
@@ -983,95 +1089,19 @@ __global__ void __launch_bounds__(kKv4ScoreWarps * 32) kv4_score_kernel(const Kv
 #pragma unroll
   for (int i = 0; i < kKv4ScorePages; ++i)
     if (lane == i) mine = best[i];
-  if (lane < kKv4ScorePages && p0 + lane < hi)
-    p.scores[((int64_t)b * p.pool.heads + head) * p.width + p0 + lane] = page >= 0 ? __fmul_rn(mine, scale) : -INFINITY;
-}
-
-// ---- the pages kept: one CTA per (KV head, sequence).  Thread t holds the keys of the
-// pages [t * per, (t + 1) * per) (in registers up to 8 of them), the keep-th largest key is
-// found bit by bit, and two scans put the kept pages in order.
-constexpr int kKv4SelThreads = 1024, kKv4SelRegs = 8;
-
-// Sum over the threads before this one; total: over all of them.
-__device__ __forceinline__ int kv4_scan(int x, int* warps, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int y = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int z = __shfl_up_sync(0xffffffffu, y, o);
-    if (lane >= o) y += z;
+  float* sc = p.scores + seg * p.width;
+  if (lane < kKv4ScorePages && p0 + lane < hi) __stcg(sc + p0 + lane, page >= 0 ? __fmul_rn(mine, scale) : -INFINITY);
+  const int ctas = (hi - lo + kKv4ScoreChunk - 1) / kKv4ScoreChunk;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    // releases the scores that the CTA wrote before the barrier, acquires the others'
+    int before;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + seg) : "memory");
+    sm.last = before == ctas - 1;
+    if (before == ctas - 1) p.counters[seg] = 0;
   }
   __syncthreads();
-  if (lane == 31) warps[warp] = y;
-  __syncthreads();
-  int w = warps[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int z = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += z;
-  }
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  return y - x + (warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0);
-}
-
-template <bool REGS>
-__global__ void __launch_bounds__(kKv4SelThreads) kv4_select_kernel(const Kv4SelectParams p) {
-  __shared__ int count[32], warps[32];
-  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int n = kv4_pages(p, b);
-  const int64_t seg = (int64_t)b * p.pool.heads + head;
-  int* out = p.out + seg * p.keep;
-  if (n <= p.keep) {
-    for (int i = tid; i < p.keep; i += kKv4SelThreads) out[i] = i < n ? i : -1;
-    return;
-  }
-  const float* sc = p.scores + seg * p.width;
-  const int per = (n + kKv4SelThreads - 1) / kKv4SelThreads, i0 = min(tid * per, n), mine = min(per, n - i0);
-  auto key_at = [&](int i) { return i < p.first || i >= n - p.last ? 0xffffffffu : kv4_key_of(__ldcg(sc + i)); };
-  uint32_t held[kKv4SelRegs];
-  if (REGS) {
-#pragma unroll
-    for (int i = 0; i < kKv4SelRegs; ++i) held[i] = i < mine ? key_at(i0 + i) : 0;
-  }
-  // f(i, key) over this thread's pages
-  auto each = [&](auto f) {
-    if (REGS) {
-#pragma unroll
-      for (int i = 0; i < kKv4SelRegs; ++i)
-        if (i < mine) f(i0 + i, held[i]);
-    } else {
-      for (int i = 0; i < mine; ++i) f(i0 + i, key_at(i0 + i));
-    }
-  };
-  if (tid < 32) count[tid] = 0;
-  __syncthreads();
-  uint32_t key = 0;                         // the largest key with at least `keep` keys >= it
-  bool exact = false;                       // exactly `keep`
-  for (int bit = 31; bit >= 0 && !exact; --bit) {
-    const uint32_t trial = key | (1u << bit);
-    int c = 0;
-    each([&](int, uint32_t k) { c += k >= trial; });
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((tid & 31) == 0 && c) atomicAdd(&count[bit], c);
-    __syncthreads();
-    c = count[bit];
-    if (c >= p.keep) key = trial;
-    exact = c == p.keep;
-  }
-  int above = 0, equal = 0, total = 0;
-  each([&](int, uint32_t k) { above += k > key, equal += k == key; });
-  int ties = 0x7fffffff, taken = 0;         // equal keys still to take, and those of earlier threads
-  if (!exact) {
-    taken = kv4_scan(equal, warps, &total);
-    int all_above;
-    kv4_scan(above, warps, &all_above);
-    ties = p.keep - all_above;
-  }
-  const int left = max(0, min(equal, ties - taken));
-  int at = kv4_scan(above + left, warps, &total), use = left;
-  each([&](int i, uint32_t k) {
-    if (k > key || (k == key && use-- > 0)) out[at++] = i;
-  });
+  if (sm.last) kv4_choose<REGS>(p, sm, sc, out, n);
 }
 
 }  // namespace starkv

@@ -102,7 +102,7 @@ class KV4SelectArgs(C.Structure):
     _fields_ = [
         ("q", C.c_void_p), ("q_strides", C.c_int64 * 3),
         ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("lengths", C.c_void_p),
-        ("pages_out", C.c_void_p), ("scores", C.c_void_p),
+        ("pages_out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("q_dtype", C.c_int32), ("batch", C.c_int32), ("num_queries", C.c_int32), ("num_q_heads", C.c_int32),
         ("table_width", C.c_int32), ("num_selected", C.c_int32), ("num_first", C.c_int32), ("num_last", C.c_int32),
     ]
@@ -139,6 +139,7 @@ SIGNATURES = [
     ("starkv_kv4_read", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("starkv_kv4_workspace_size", C.c_int, [C.POINTER(C.c_size_t)]),
     ("starkv_kv4_attention", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("starkv_kv4_select_workspace_size", C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
     ("starkv_kv4_select", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("starkv_last_error", C.c_char_p, []),
 ]

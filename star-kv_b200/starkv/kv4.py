@@ -35,7 +35,7 @@ from .ops import _DT
 _CACHE = struct.Struct("4P4i")
 _IO = struct.Struct("2P3q3qPq2P4i")
 _ATTENTION = struct.Struct("3P3q3qPqPP2qPPNf7i")
-_SELECT = struct.Struct("P3qPq3P8i")
+_SELECT = struct.Struct("P3qPq3PN8i")
 
 _TOKEN_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _QUERY_DTYPES = (torch.float16, torch.bfloat16)
@@ -77,26 +77,33 @@ def _output(t: torch.Tensor, name: str):
 
 
 _WORKSPACES = {}
-_workspace_bytes = 0
 
 
-def workspace(index: int, stream: int) -> torch.Tensor:
-    """Attention scratch of one stream (zeroed once; every call leaves it zeroed
-    where the next needs it).  A call under graph capture gets its own, zeroed by the
-    graph, so replays never share one with eager calls."""
-    global _workspace_bytes
-    ws = _WORKSPACES.get((index, stream))
-    capturing = torch.cuda.is_current_stream_capturing()
-    if ws is not None and not capturing:
-        return ws
-    if not _workspace_bytes:
+def _workspace(kind: str, index: int, size) -> torch.Tensor:
+    """Scratch of one kind for the current stream, of ``size()`` bytes at least (zeroed
+    when made; every call leaves zeroed what the next needs so).  A call under graph
+    capture gets its own, zeroed by the graph, so replays never share one with
+    eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(size(), dtype=torch.uint8, device=f"cuda:{index}")
+    key = (kind, index, _stream_of(index))
+    ws = _WORKSPACES.get(key)
+    need = size()
+    if ws is None or ws.numel() < need:
+        ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=f"cuda:{index}")
+    return ws
+
+
+_attention_bytes = 0
+
+
+def _attention_size() -> int:
+    global _attention_bytes
+    if not _attention_bytes:
         n = C.c_size_t(0)
         check(load().starkv_kv4_workspace_size(C.byref(n)), "starkv_kv4_workspace_size")
-        _workspace_bytes = int(n.value)
-    ws = torch.zeros(_workspace_bytes, dtype=torch.uint8, device=f"cuda:{index}")
-    if not capturing:
-        _WORKSPACES[index, stream] = ws
-    return ws
+        _attention_bytes = int(n.value)
+    return _attention_bytes
 
 
 class KV4Cache:
@@ -244,7 +251,7 @@ class KV4Cache:
             pp = _ints(pages, "pages", (B, self.num_kv_heads, n), index)
         lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
         if ws is None:
-            ws = workspace(index, _stream_of(index))
+            ws = _workspace("attention", index, _attention_size)
         elif ws.get_device() != index or not ws.is_contiguous():
             raise StarKVError(f"ws must be contiguous on {self.device}")
         a = _ATTENTION.pack(q4.data_ptr(), o4.data_ptr(), lse.data_ptr() if return_lse else 0,
@@ -270,8 +277,9 @@ class KV4Cache:
                 raise StarKVError("num_pages must be positive")
             out = torch.empty(shape, dtype=torch.int32, device=self.device)
         op = _ints(out, "out", shape, self._index)
-        scores = torch.empty(B * self.num_kv_heads * W, dtype=torch.float32, device=self.device)
-        a = _SELECT.pack(q4.data_ptr(), *qs[:3], tp, ts, lp, op, scores.data_ptr(), _DT[q.dtype], B,
+        # counters (65536 ints), then a score a page
+        ws = _workspace("select", self._index, lambda: 262144 + 4 * B * self.num_kv_heads * W)
+        a = _SELECT.pack(q4.data_ptr(), *qs[:3], tp, ts, lp, op, ws.data_ptr(), ws.numel(), _DT[q.dtype], B,
                          q4.shape[1], q4.shape[2], W, num_pages, first, last)
         self._call(self._lib.starkv_kv4_select, a, "starkv_kv4_select")
         return out
