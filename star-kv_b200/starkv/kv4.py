@@ -193,8 +193,9 @@ class KV4Cache:
                 raise StarKVError("num_tokens must not be negative")
             if dtype not in _TOKEN_DTYPES:
                 raise StarKVError(f"dtype must be one of {_TOKEN_DTYPES}, got {dtype}")
-            k, v = torch.empty((2, *shape), dtype=dtype, device=self.device).unbind(0)
-            ks = vs = k.stride()
+            B, T, H, _ = shape
+            ks = vs = (T * H * 128, H * 128, 128, 1)
+            k, v = torch.empty_strided((2, *shape), (B * ks[0], *ks), dtype=dtype, device=self.device).unbind(0)
         else:
             k, v = out
             ks = _rows(k, "out[0]", shape, _TOKEN_DTYPES, self._index)
@@ -230,8 +231,10 @@ class KV4Cache:
         index = self._index
         lp = _ints(lengths, "lengths", (B,), index)
         if out is None:
-            out = o4 = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            os_ = (Q * Hq * 128, Hq * 128, 128)
+            # empty_strided: the cheapest of torch's allocating calls
+            os_ = (Q * Hq * 128, Hq * 128, 128, 1)
+            o4 = torch.empty_strided((B, Q, Hq, 128), os_, dtype=q.dtype, device=self.device)
+            out = o4 if q4 is q else o4[:, 0]
         else:
             o4 = out.unsqueeze(1) if q.dim() == 3 and out.dim() == 3 else out
             os_ = _rows(o4, "out", q4.shape, _TOKEN_DTYPES, index)
@@ -249,7 +252,10 @@ class KV4Cache:
                 raise StarKVError("pages must be (B, num_kv_heads, n), n > 0")
             n = pages.shape[2]
             pp = _ints(pages, "pages", (B, self.num_kv_heads, n), index)
-        lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=self.device) if return_lse else None
+        lse = None
+        if return_lse:
+            lse = torch.empty_strided((B, Q, Hq), (Q * Hq, Hq, 1), dtype=torch.float32, device=self.device)
+            lse_out = lse if q4 is q else lse[:, 0]
         if ws is None:
             ws = _workspace("attention", index, _attention_size)
         elif ws.get_device() != index or not ws.is_contiguous():
@@ -258,7 +264,7 @@ class KV4Cache:
                             *qs[:3], *os_[:3], tp, ts, lp, mp, mstride, mwidth, pp, ws.data_ptr(),
                             ws.numel() * ws.element_size(), scaling, n, _DT[q.dtype], _DT[out.dtype], B, Q, Hq, W)
         self._call(self._lib.starkv_kv4_attention, a, "starkv_kv4_attention")
-        return (out, lse) if return_lse else out
+        return (out, lse_out) if return_lse else out
 
     def select(self, q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, num_pages: int,
                first: int = 1, last: int = 1, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -275,7 +281,8 @@ class KV4Cache:
         if out is None:
             if num_pages <= 0:
                 raise StarKVError("num_pages must be positive")
-            out = torch.empty(shape, dtype=torch.int32, device=self.device)
+            n = shape[2]
+            out = torch.empty_strided(shape, (self.num_kv_heads * n, n, 1), dtype=torch.int32, device=self.device)
         op = _ints(out, "out", shape, self._index)
         # counters (65536 ints), then a score a page
         ws = _workspace("select", self._index, lambda: 262144 + 4 * B * self.num_kv_heads * W)

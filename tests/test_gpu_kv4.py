@@ -359,6 +359,19 @@ def test_selection_and_attention_over_it(cuda, page, Hkv, G, Q, keep):
     check_attention(made, q, pages=pages, mask=mask)
 
 
+@pytest.mark.parametrize("pages_n", [2500, 9000])
+def test_selection_among_many_pages(cuda, pages_n):
+    """More pages than one thread's registers hold, and more than all of them do."""
+    n = pages_n * 16 - 7
+    made = Made(cuda, [n, 40 * 16], 1, 16, F16, seed=pages_n, garbage=False)
+    q = rnd((2, 1, 2, 128), F16, 92, cuda)
+    pages = made.cache.select(q, made.table, made.lengths, 33, first=2, last=3)
+    for b, m in enumerate((n, 40 * 16)):
+        want = O.select(f64(q[b]).reshape(-1, 128), made.stored(b, 0)[0], 16, 33, 2, 3)
+        assert pages[b, 0].tolist() == want
+    assert torch.equal(pages, made.cache.select(q, made.table, made.lengths, 33, first=2, last=3))
+
+
 def test_selection_first_last_and_ties(cuda):
     """Identical pages tie: the lower ones win; first / last pages are always in."""
     page, n = 16, 16 * 12
@@ -450,6 +463,17 @@ def test_bad_pages_and_positions_set_the_error_word(cuda):
     assert cache.read_error() == 0x201 and torch.equal(got, want)
     cache.read(good, ints([30, 0], cuda), 5)
     assert cache.read_error() == 0x202
+
+
+def test_single_query_shape(cuda):
+    """(B, Hq, 128) queries give (B, Hq, 128) outputs, the same as one token of (B, 1, Hq, 128)."""
+    made = Made(cuda, [100, 33], 2, 16, F16, seed=5)
+    q = rnd((2, 1, 4, 128), F16, 6, cuda)
+    a, la = made.cache.attend(q, made.table, made.lengths, SCALING, return_lse=True)
+    b, lb = made.cache.attend(q[:, 0], made.table, made.lengths, SCALING, return_lse=True)
+    assert b.shape == (2, 4, 128) and lb.shape == (2, 4)
+    assert torch.equal(a[:, 0], b) and torch.equal(la[:, 0], lb)
+    assert torch.equal(made.cache.select(q, made.table, made.lengths, 3), made.cache.select(q[:, 0], made.table, made.lengths, 3))
 
 
 def test_empty_calls(cuda):
