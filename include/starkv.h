@@ -381,8 +381,8 @@ typedef struct starkv_kv4_attention_args {
   int64_t mask_stride;
   int64_t mask_width;
   const int32_t* pages;       /* (B, Hkv, num_selected) page ordinals of the sequence, each once, -1 = none, or NULL */
-  void* workspace;            /* starkv_kv4_workspace_size bytes, zeroed before its first use; each call leaves it ready
-                                 for the next.  One call at a time may use it. */
+  void* workspace;            /* starkv_kv4_workspace_size bytes, the first 1024 zeroed before its first use (each call
+                                 leaves them zero).  One call at a time may use it. */
   size_t workspace_bytes;
   float scaling;
   int32_t num_selected;

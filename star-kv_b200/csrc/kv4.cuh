@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(256, 2) kv4_write_kernel(const Kv4IoParams p) 
   const int64_t first = base + t0 - start + tok;               // token of the lane's row in step 0
   const T* kp = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + first * p.ks[1] + head * p.ks[2] + (lane & 7) * 16;
   const T* vp = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + first * p.vs[1] + head * p.vs[2] + (lane & 7) * 16;
-  constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 1;               // steps loaded ahead; 16 bits: the whole tile
   Kv4Row<T> kx[kAhead], vx[kAhead];
   auto load = [&](int it) {
     const int t = 4 * it + tok;

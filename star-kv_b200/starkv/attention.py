@@ -80,12 +80,13 @@ class StarKVCache(_HFCache):
         self.capacity = int(capacity)
         self.quantized = bool(quantized)
         self.states: Dict[int, DecodeLayer] = {}
+        self.kv4_states: Dict[int, "KV4State"] = {}       # layers with whole heads (starkv.kv4_attention)
 
     # ---- the Cache interface the transformers model code uses
     def get_seq_length(self, layer_idx: int = 0) -> int:
-        st = self.states.get(layer_idx)
-        if st is None and self.states:
-            st = next(iter(self.states.values()))
+        st = self.states.get(layer_idx) or self.kv4_states.get(layer_idx)
+        if st is None and (self.states or self.kv4_states):
+            st = next(iter((self.states or self.kv4_states).values()))
         return 0 if st is None else st.length
 
     def get_mask_sizes(self, query_length: int, layer_idx: int = 0):
@@ -100,14 +101,14 @@ class StarKVCache(_HFCache):
 
     @property
     def is_initialized(self) -> bool:
-        return bool(self.states)
+        return bool(self.states or self.kv4_states)
 
     @property
     def is_sliding(self):
-        return [False] * max(1, len(self.states))
+        return [False] * max(1, len(self))
 
     def __len__(self):
-        return len(self.states)
+        return len(self.states) + len(self.kv4_states)
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         raise NotImplementedError("StarKVCache is written by the STAR-KV attention modules themselves "

@@ -14,7 +14,11 @@ the fused decode path per layer: ``starkv_project_append`` (latent projection +
 quantise-append) and ``starkv_decode_attention``.  The rest of each layer (norms,
 MLP, embeddings, LM head) is the transformers Llama code.
 
-    python -m starkv.e2e --context 4096 --new 128 [--layers 32] [--unquantized]
+``--kv4-layers n`` keeps the first n layers' K / V projections dense, their heads in
+the paged 4-bit cache (``starkv.kv4_attention``); ``--kv4-keep-pages p`` lets their decode
+steps attend to the p pages a score bound selects.
+
+    python -m starkv.e2e --context 4096 --new 128 [--layers 32] [--unquantized] [--kv4-layers 4]
 
 prints one JSON line: decode tokens/s (batch 1) and ms per generated token.
 """
@@ -31,12 +35,14 @@ import torch
 
 from .attention import LlamaCustomAttention, LlamaCustomAttentionQuant, StarKVCache, apply_rotary_pos_emb_custom
 from .export import BlockVProj, RaggedKProj
+from .kv4_attention import KV4Attention
 
 
 def build_model(num_layers: int = 32, hidden: int = 4096, heads: int = 32, kv_heads: int = 32, mlp: int = 11008,
                 vocab: int = 32000, k_rank_choices: Sequence[int] = (16, 32, 48),
                 v_rank_choices: Sequence[int] = (64, 128, 192), v_block_kv: int = 4, quantized: bool = True,
-                seed: int = 0, device="cuda", dtype=torch.float16, max_positions: int = 131072 + 256):
+                seed: int = 0, device="cuda", dtype=torch.float16, max_positions: int = 131072 + 256,
+              kv4_layers: Sequence[int] = (), kv4_keep_pages: int = 0):
     from transformers import LlamaConfig, LlamaForCausalLM
 
     cfg = LlamaConfig(hidden_size=hidden, num_attention_heads=heads, num_key_value_heads=kv_heads,
@@ -49,6 +55,12 @@ def build_model(num_layers: int = 32, hidden: int = 4096, heads: int = 32, kv_he
     g = torch.Generator(device=device).manual_seed(seed)
     cls = LlamaCustomAttentionQuant if quantized else LlamaCustomAttention
     for i, layer in enumerate(model.model.layers):
+        if i in kv4_layers:                              # dense K / V projections, whole heads in 4 bits
+            attn = KV4Attention(cfg, layer_idx=i, keep_pages=kv4_keep_pages)
+            for name in ("q_proj", "k_proj", "v_proj", "o_proj"):
+                setattr(attn, name, getattr(layer.self_attn, name))
+            layer.self_attn = attn
+            continue
         attn = cls(cfg, layer_idx=i, decomp_goup_num=heads)
         attn.q_proj, attn.o_proj = layer.self_attn.q_proj, layer.self_attn.o_proj
         ranks = [int(x) for x in rng.choice(k_rank_choices, size=kv_heads)]
@@ -129,7 +141,8 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     plus one graph for the token embedding and RoPE tables and one for the LM
     head and argmax.  A step is then 2 + 2L graph launches and 2L C-ABI calls
     (``starkv_project_append`` + ``starkv_decode_attention`` per layer) on the
-    current stream, all on static buffers.  Returns what ``generate`` returns,
+    current stream, all on static buffers.  Layers with whole heads (``KV4Attention``)
+    take their lengths from the GPU, so graph A_i holds their write and attention too.  Returns what ``generate`` returns,
     with the same tokens."""
     B, P = prompt.shape
     quant = getattr(model, "starkv_quantized", True)
@@ -153,9 +166,11 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     attn_s = torch.empty(B, Hq, D, dtype=dt, device=dev)
     cos_s = torch.empty(B, 1, D, dtype=dt, device=dev)
     sin_s = torch.empty_like(cos_s)
-    vs = [(l.self_attn.k_proj.VS.weight.to(dt).contiguous(), l.self_attn.v_proj.VS.weight.to(dt).contiguous())
-          for l in layers]
-    states = [cache.layer(i, l.self_attn, B, dt) for i, l in enumerate(layers)]
+    kv4 = [isinstance(l.self_attn, KV4Attention) for l in layers]
+    vs = [None if w else (l.self_attn.k_proj.VS.weight.to(dt).contiguous(), l.self_attn.v_proj.VS.weight.to(dt).contiguous())
+          for l, w in zip(layers, kv4)]
+    states = [cache.kv4_states[i] if w else cache.layer(i, l.self_attn, B, dt)
+              for i, (l, w) in enumerate(zip(layers, kv4))]
 
     def embed():
         h_s.copy_(model.model.embed_tokens(tok_s))
@@ -166,6 +181,12 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     def pre(i):
         layer = layers[i]
         x_s.copy_(layer.input_layernorm(h_s))
+        if kv4[i]:                                       # lengths live on the GPU: the whole step is in the graph
+            st = states[i]
+            q, k, v = layer.self_attn.heads(x_s, cos_s, sin_s)
+            st.append(k, v)
+            attn_s.copy_(st.attend(q, layer.self_attn.scaling, keep_pages=layer.self_attn.keep_pages)[:, 0])
+            return
         q = layer.self_attn.q_proj(x_s).view(B, 1, Hq, D).transpose(1, 2)
         q_s.copy_(apply_rotary_pos_emb_custom(q, cos_s, sin_s)[:, :, 0, :])
 
@@ -185,12 +206,21 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     saved = (tok_s.clone(), pos_s.clone())
+    held = cache.get_seq_length()
     with torch.cuda.stream(side):
         for f in fns:
             f()
     torch.cuda.current_stream().wait_stream(side)
     tok_s.copy_(saved[0])
     pos_s.copy_(saved[1])
+
+    def rewind():                                        # forget what the warm-up and the capture appended
+        for st, w in zip(states, kv4):
+            if w:
+                st.lengths.fill_(held)
+                st.length = held
+
+    rewind()
     graphs = []
     pool = None
     for f in fns:
@@ -199,8 +229,9 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
             f()
         pool = g.pool()
         graphs.append(g)
+    rewind()
     g_embed, g_pre, g_post, g_head = graphs[0], graphs[1:1 + len(layers)], graphs[1 + len(layers):-1], graphs[-1]
-    steps = [st.prepared_step(q_s, x_s, vs[i][0], vs[i][1], attn_s) for i, st in enumerate(states)]
+    steps = [None if kv4[i] else st.prepared_step(q_s, x_s, vs[i][0], vs[i][1], attn_s) for i, st in enumerate(states)]
     torch.cuda.synchronize()
     e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     e0.record()
@@ -208,10 +239,14 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
         g_embed.replay()
         for i in range(len(states)):
             g_pre[i].replay()
-            steps[i]()
+            if steps[i] is not None:
+                steps[i]()
             g_post[i].replay()
         g_head.replay()
         out.append(tok_s.clone())
+    for st, w in zip(states, kv4):
+        if w:
+            st.length = held + new_tokens - 1            # the graphs moved the GPU's count
     e1.record()
     torch.cuda.synchronize()
     per_tok = e0.elapsed_time(e1) / 1e3 / max(1, new_tokens - 1)
@@ -228,10 +263,13 @@ def main():
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--unquantized", action="store_true")
+    ap.add_argument("--kv4-layers", type=int, default=0, help="leading layers with whole heads in the 4-bit cache")
+    ap.add_argument("--kv4-keep-pages", type=int, default=0, help="pages (of 64 tokens) those attend to; 0: all")
     ap.add_argument("--no-graphs", action="store_true", help="eager per-layer decode (no CUDA graphs)")
     a = ap.parse_args()
     t0 = time.time()
-    model = build_model(num_layers=a.layers, quantized=not a.unquantized, seed=a.seed)
+    model = build_model(num_layers=a.layers, quantized=not a.unquantized, seed=a.seed,
+                        kv4_layers=range(a.kv4_layers), kv4_keep_pages=a.kv4_keep_pages)
     g = torch.Generator(device="cuda").manual_seed(a.seed + 1)
     prompt = torch.randint(0, model.config.vocab_size, (a.batch, a.context), generator=g, device="cuda")
     gen = generate if a.no_graphs else generate_graphed
@@ -240,7 +278,8 @@ def main():
     ids, per_tok = gen(model, prompt, a.new, stats=st)
     print(json.dumps({"metric": "end-to-end greedy decode (c3)", "value": a.batch / per_tok, "unit": "tokens/s",
                       "ms_per_token": per_tok * 1e3, "prompt_ms": st["prompt_s"] * 1e3, "batch": a.batch, "context": a.context, "new_tokens": a.new,
-                      "layers": a.layers, "quantized": not a.unquantized, "cuda_graphs": not a.no_graphs, "weights": "random-init fp16",
+                      "layers": a.layers, "quantized": not a.unquantized, "cuda_graphs": not a.no_graphs,
+                      **({"kv4_layers": a.kv4_layers, "kv4_keep_pages": a.kv4_keep_pages} if a.kv4_layers else {}), "weights": "random-init fp16",
                       "first_tokens": ids[0, :8].tolist(), "wall_s": time.time() - t0}))
 
 

@@ -79,18 +79,20 @@ def _output(t: torch.Tensor, name: str):
 _WORKSPACES = {}
 
 
-def _workspace(kind: str, index: int, size) -> torch.Tensor:
-    """Scratch of one kind for the current stream, of ``size()`` bytes at least (zeroed
-    when made; every call leaves zeroed what the next needs so).  A call under graph
-    capture gets its own, zeroed by the graph, so replays never share one with
-    eager calls."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(size(), dtype=torch.uint8, device=f"cuda:{index}")
+def _workspace(kind: str, index: int, size, zeroed: int) -> torch.Tensor:
+    """Scratch of one kind for the current stream, of ``size()`` bytes at least (its
+    first ``zeroed`` bytes cleared when made; every call leaves them clear for the
+    next).  A call under graph capture gets its own, cleared by the graph, so replays
+    never share one with eager calls."""
+    capturing = torch.cuda.is_current_stream_capturing()
     key = (kind, index, _stream_of(index))
-    ws = _WORKSPACES.get(key)
+    ws = None if capturing else _WORKSPACES.get(key)
     need = size()
     if ws is None or ws.numel() < need:
-        ws = _WORKSPACES[key] = torch.zeros(need, dtype=torch.uint8, device=f"cuda:{index}")
+        ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
+        ws[:zeroed].zero_()
+        if not capturing:
+            _WORKSPACES[key] = ws
     return ws
 
 
@@ -125,19 +127,43 @@ class KV4Cache:
         dev = torch.device(device)
         if dev.type != "cuda":
             raise StarKVError("KV4Cache lives on a CUDA device")
-        self.num_pages, self.num_kv_heads, self.page_size = int(num_pages), int(num_kv_heads), int(page_size)
-        self.data = torch.zeros(num_pages, num_kv_heads, page_size // 16, 2560, dtype=torch.uint8, device=dev)
-        self.device = self.data.device
-        self.bounds = self.bound_scales = None
+        data = torch.zeros(num_pages, num_kv_heads, page_size // 16, 2560, dtype=torch.uint8, device=dev)
+        bounds = scales = None
         if page_bounds:
-            self.bounds = torch.zeros(num_pages, num_kv_heads, 2, 128, dtype=torch.int8, device=dev)
-            self.bound_scales = torch.zeros(num_pages, num_kv_heads, dtype=torch.float32, device=dev)
-        self.error_word = torch.zeros(1, dtype=torch.int32, device=dev)
-        self._block = _CACHE.pack(self.data.data_ptr(), self.bounds.data_ptr() if page_bounds else 0,
-                                  self.bound_scales.data_ptr() if page_bounds else 0, self.error_word.data_ptr(),
+            bounds = torch.zeros(num_pages, num_kv_heads, 2, 128, dtype=torch.int8, device=dev)
+            scales = torch.zeros(num_pages, num_kv_heads, dtype=torch.float32, device=dev)
+        self._hold(data, bounds, scales, torch.zeros(1, dtype=torch.int32, device=dev))
+
+    @classmethod
+    def from_tensors(cls, data: torch.Tensor, bounds: Optional[torch.Tensor], bound_scales: Optional[torch.Tensor],
+                     error_word: torch.Tensor) -> "KV4Cache":
+        """A cache over the tensors of another (``data``, ``bounds``, ``bound_scales``,
+        ``error_word``), for code that passes them one by one."""
+        if data.dim() != 4 or data.shape[3] != 2560 or data.dtype != torch.uint8 or not data.is_cuda:
+            raise StarKVError("data must be a uint8 (pages, heads, page_size / 16, 2560) CUDA tensor")
+        pages, heads = data.shape[:2]
+        ok = data.is_contiguous() and data.shape[2] in (1, 2, 4, 8) and pages > 0 and heads > 0
+        ok = ok and (bounds is None) == (bound_scales is None)
+        parts = [(error_word, torch.int32, (1,))]
+        if bounds is not None:
+            parts += [(bounds, torch.int8, (pages, heads, 2, 128)), (bound_scales, torch.float32, (pages, heads))]
+        for t, dtype, shape in parts:
+            ok = ok and t.dtype == dtype and t.shape == shape and t.is_contiguous() and t.device == data.device
+        if not ok:
+            raise StarKVError("the tensors are not those of a KV4Cache")
+        self = cls.__new__(cls)
+        self._hold(data, bounds, bound_scales, error_word)
+        return self
+
+    def _hold(self, data, bounds, bound_scales, error_word):
+        self.data, self.bounds, self.bound_scales, self.error_word = data, bounds, bound_scales, error_word
+        self.num_pages, self.num_kv_heads, self.page_size = data.shape[0], data.shape[1], data.shape[2] * 16
+        self.device = data.device
+        self._index = self.device.index
+        self._block = _CACHE.pack(data.data_ptr(), 0 if bounds is None else bounds.data_ptr(),
+                                  0 if bounds is None else bound_scales.data_ptr(), error_word.data_ptr(),
                                   self.num_pages, self.num_kv_heads, self.page_size, 128)
         self._lib = load()
-        self._index = self.device.index
 
     def nbytes(self) -> int:
         """Device bytes of the pool (codes, parameters and bounds)."""
@@ -257,7 +283,7 @@ class KV4Cache:
             lse = torch.empty_strided((B, Q, Hq), (Q * Hq, Hq, 1), dtype=torch.float32, device=self.device)
             lse_out = lse if q4 is q else lse[:, 0]
         if ws is None:
-            ws = _workspace("attention", index, _attention_size)
+            ws = _workspace("attention", index, _attention_size, 1024)
         elif ws.get_device() != index or not ws.is_contiguous():
             raise StarKVError(f"ws must be contiguous on {self.device}")
         a = _ATTENTION.pack(q4.data_ptr(), o4.data_ptr(), lse.data_ptr() if return_lse else 0,
@@ -285,7 +311,7 @@ class KV4Cache:
             out = torch.empty_strided(shape, (self.num_kv_heads * n, n, 1), dtype=torch.int32, device=self.device)
         op = _ints(out, "out", shape, self._index)
         # counters (65536 ints), then a score a page
-        ws = _workspace("select", self._index, lambda: 262144 + 4 * B * self.num_kv_heads * W)
+        ws = _workspace("select", self._index, lambda: 262144 + 4 * B * self.num_kv_heads * W, 262144)
         a = _SELECT.pack(q4.data_ptr(), *qs[:3], tp, ts, lp, op, ws.data_ptr(), ws.numel(), _DT[q.dtype], B,
                          q4.shape[1], q4.shape[2], W, num_pages, first, last)
         self._call(self._lib.starkv_kv4_select, a, "starkv_kv4_select")

@@ -1,0 +1,132 @@
+"""Llama attention with whole key / value heads in the paged 4-bit cache.
+
+``KV4Attention`` stands beside the latent modules (``starkv.attention``) in one model
+and one ``StarKVCache``: layers whose learned ranks stay near the head dimension keep
+their dense ``k_proj`` / ``v_proj`` and hold their heads in 4 bits here, the others
+hold latents.  Same constructor and forward arguments as the latent modules, so
+the decoder layer's code does not change.
+
+* prompt: keys (rotated) and values are written into pages; the attention runs over
+  the exact heads with the prompt kernel (``starkv.prefill``);
+* a longer piece that continues a prompt: the history is read back from the
+  pages, attention by torch SDPA over both;
+* decode, and up to ``MAX_DRAFT`` tokens at once: write, then attention over the
+  pages; with ``keep_pages`` set, over the pages that ``KV4Cache.select`` keeps.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from . import prefill
+from .attention import LlamaCustomAttention, StarKVCache, apply_rotary_pos_emb_custom
+from .kv4 import KV4Cache
+
+MAX_DRAFT = 16
+
+
+class KV4State:
+    """One layer's pages of a fixed batch: sequence b owns ``pages_per_sequence``
+    consecutive pages of the pool.  ``lengths`` (int32, on the GPU) is what the kernels
+    read, ``length`` the same number on the host."""
+
+    def __init__(self, batch: int, capacity: int, num_kv_heads: int, page_size: int, device, page_bounds: bool):
+        self.width = -(-capacity // page_size)
+        self.cache = KV4Cache(batch * self.width, num_kv_heads, page_size, device, page_bounds)
+        self.block_table = torch.arange(batch * self.width, dtype=torch.int32, device=device).view(batch, self.width)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.length = 0
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Write k / v (B, T, Hkv, 128) behind the tokens held."""
+        if self.length + k.shape[1] > self.width * self.cache.page_size:
+            raise ValueError(f"the cache holds {self.width * self.cache.page_size} tokens")
+        self.cache.write(k, v, self.block_table, self.lengths)
+        self.lengths.add_(k.shape[1])
+        self.length += k.shape[1]
+
+    def attend(self, q: torch.Tensor, scaling: float, mask: Optional[torch.Tensor] = None,
+               keep_pages: int = 0) -> torch.Tensor:
+        """The newest tokens' queries (B, T, Hq, 128) over the pages, or over the best
+        ``keep_pages`` of them."""
+        pages = None
+        if keep_pages:
+            pages = self.cache.select(q, self.block_table, self.lengths, keep_pages)
+        return self.cache.attend(q, self.block_table, self.lengths, scaling, mask=mask, pages=pages)
+
+    def history(self, dtype: torch.dtype):
+        """All tokens held as (k, v), each (B, length, Hkv, 128)."""
+        return self.cache.read(self.block_table, torch.zeros_like(self.lengths), self.length, dtype=dtype)
+
+
+class KV4Attention(nn.Module):
+    """``keep_pages``: pages a decode step attends to (0: all of them)."""
+
+    def __init__(self, config, layer_idx: Optional[int] = None, page_size: int = 64, keep_pages: int = 0):
+        super().__init__()
+        self.layer_idx = layer_idx
+        self.num_heads = config.num_attention_heads
+        self.num_key_value_heads = config.num_key_value_heads
+        self.head_dim = config.hidden_size // config.num_attention_heads
+        if self.head_dim != 128:
+            raise ValueError("the 4-bit cache takes heads of dimension 128")
+        self.scaling = self.head_dim ** -0.5
+        self.page_size, self.keep_pages = page_size, keep_pages
+        bias = config.attention_bias
+        self.q_proj = nn.Linear(config.hidden_size, self.num_heads * 128, bias=bias)
+        self.k_proj = nn.Linear(config.hidden_size, self.num_key_value_heads * 128, bias=bias)
+        self.v_proj = nn.Linear(config.hidden_size, self.num_key_value_heads * 128, bias=bias)
+        self.o_proj = nn.Linear(self.num_heads * 128, config.hidden_size, bias=bias)
+
+    def state(self, cache: StarKVCache, batch: int, device) -> KV4State:
+        st = cache.kv4_states.get(self.layer_idx)
+        if st is None:
+            st = KV4State(batch, cache.capacity, self.num_key_value_heads, self.page_size, device, self.keep_pages > 0)
+            cache.kv4_states[self.layer_idx] = st
+        return st
+
+    def heads(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor):
+        """Rotated queries and keys and the values of x (B, T, hidden), each (B, T, heads, 128)."""
+        B, T, _ = x.shape
+        q = self.q_proj(x).view(B, T, self.num_heads, 128).transpose(1, 2)
+        k = self.k_proj(x).view(B, T, self.num_key_value_heads, 128).transpose(1, 2)
+        q = apply_rotary_pos_emb_custom(q, cos, sin)
+        k = apply_rotary_pos_emb_custom(k, cos, sin)
+        return q.transpose(1, 2), k.transpose(1, 2), self.v_proj(x).view(B, T, self.num_key_value_heads, 128)
+
+    def forward(self, hidden_states, position_embeddings, attention_mask, position_ids=None, past_key_values=None,
+                cache_position=None, past_key_values_upper=None, **kwargs):
+        cache = past_key_values if past_key_values is not None else past_key_values_upper
+        if not isinstance(cache, StarKVCache):
+            raise TypeError("KV4Attention takes a StarKVCache as past_key_values")
+        B, T, _ = hidden_states.shape
+        q, k, v = self.heads(hidden_states, *position_embeddings)
+        st = self.state(cache, B, hidden_states.device)
+        before = st.length
+        if T > MAX_DRAFT and before:
+            old_k, old_v = st.history(k.dtype)
+            keys, values = torch.cat([old_k, k], 1), torch.cat([old_v, v], 1)
+        else:
+            keys, values = k, v
+        st.append(k, v)
+        if T <= MAX_DRAFT and (before or T == 1):
+            mask = LlamaCustomAttention._decode_mask(attention_mask, B, st.length)
+            out = st.attend(q, self.scaling, mask, self.keep_pages)
+        elif attention_mask is None and not before:
+            out = prefill.prompt_attention(q.transpose(1, 2), keys.transpose(1, 2), values.transpose(1, 2), self.scaling)
+            out = out.transpose(1, 2)
+        else:
+            grp = self.num_heads // self.num_key_value_heads
+            n = keys.shape[1]
+            if attention_mask is None:
+                mask = torch.ones(T, n, dtype=torch.bool, device=q.device).tril(n - T)
+            else:
+                mask = attention_mask[:, :, :, :n]
+            out = F.scaled_dot_product_attention(q.transpose(1, 2), keys.transpose(1, 2).repeat_interleave(grp, 1),
+                                                 values.transpose(1, 2).repeat_interleave(grp, 1), attn_mask=mask,
+                                                 scale=self.scaling).transpose(1, 2)
+        return self.o_proj(out.reshape(B, T, self.num_heads * 128)), None

@@ -4,22 +4,27 @@
     torch.ops.starkv.k_attn        K logits, abx's contract (starkv_k_logits)
     torch.ops.starkv.v_attn        P . X_v in latent space, bx's contract (starkv_v_latent)
     torch.ops.starkv.quant_append  quantise + in-place cache append (starkv_append)
+    torch.ops.starkv.kv4_write     quantise whole heads into 4-bit pages (starkv_kv4_write)
+    torch.ops.starkv.kv4_read      4-bit pages back to whole heads (starkv_kv4_read)
+    torch.ops.starkv.kv4_attn      attention over 4-bit pages, with its log-sum-exp (starkv_kv4_attention)
+    torch.ops.starkv.kv4_select    the pages a score bound keeps (starkv_kv4_select)
 
 They replace the reference's kernel entry points (abx_rope_batched.abx,
 bx_quant.bx, the quantiser + ``Cache.update``) for code that dispatches
 through the torch operator registry.  A layer's ``starkv_layout`` travels as
-its raw bytes in a CPU uint8 tensor (``layout_tensor``).  No CPU kernel is
-registered: calling an op with CPU tensors raises.
+its raw bytes in a CPU uint8 tensor (``layout_tensor``), a ``KV4Cache`` as its
+tensors.  No CPU kernel is registered: calling an op with CPU tensors raises.
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from . import ops
 from ._lib import Layout
+from .kv4 import KV4Cache
 
 _LIB = "starkv"
 
@@ -99,3 +104,56 @@ def quant_append(layout: torch.Tensor, k_lat: torch.Tensor, v_lat: torch.Tensor,
 @quant_append.register_fake
 def _(layout, k_lat, v_lat, start_slot, k_cache, k_scales, v_cache, v_params):
     return None
+
+
+@torch.library.custom_op(f"{_LIB}::kv4_write", mutates_args=("data", "bounds", "bound_scales", "error_word"),
+                         device_types="cuda")
+def kv4_write(data: torch.Tensor, bounds: Optional[torch.Tensor], bound_scales: Optional[torch.Tensor],
+              error_word: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
+              start: torch.Tensor, count: Optional[torch.Tensor] = None) -> None:
+    KV4Cache.from_tensors(data, bounds, bound_scales, error_word).write(k, v, block_table, start, count)
+
+
+@kv4_write.register_fake
+def _(data, bounds, bound_scales, error_word, k, v, block_table, start, count=None):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::kv4_read", mutates_args=("error_word",), device_types="cuda")
+def kv4_read(data: torch.Tensor, error_word: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
+             num_tokens: int, dtype: torch.dtype, count: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Keys and values as one (2, B, num_tokens, heads, 128) tensor."""
+    out = torch.empty(2, block_table.shape[0], num_tokens, data.shape[1], 128, dtype=dtype, device=data.device)
+    KV4Cache.from_tensors(data, None, None, error_word).read(block_table, start, num_tokens, count, out=(out[0], out[1]))
+    return out
+
+
+@kv4_read.register_fake
+def _(data, error_word, block_table, start, num_tokens, dtype, count=None):
+    return data.new_empty((2, block_table.shape[0], num_tokens, data.shape[1], 128), dtype=dtype)
+
+
+@torch.library.custom_op(f"{_LIB}::kv4_attn", mutates_args=("error_word",), device_types="cuda")
+def kv4_attn(data: torch.Tensor, error_word: torch.Tensor, q: torch.Tensor, block_table: torch.Tensor,
+             lengths: torch.Tensor, scaling: float, mask: Optional[torch.Tensor] = None,
+             pages: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    cache = KV4Cache.from_tensors(data, None, None, error_word)
+    return cache.attend(q, block_table, lengths, scaling, mask=mask, pages=pages, return_lse=True)
+
+
+@kv4_attn.register_fake
+def _(data, error_word, q, block_table, lengths, scaling, mask=None, pages=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_LIB}::kv4_select", mutates_args=("error_word",), device_types="cuda")
+def kv4_select(data: torch.Tensor, bounds: torch.Tensor, bound_scales: torch.Tensor, error_word: torch.Tensor,
+               q: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, num_pages: int, first: int = 1,
+               last: int = 1) -> torch.Tensor:
+    cache = KV4Cache.from_tensors(data, bounds, bound_scales, error_word)
+    return cache.select(q, block_table, lengths, num_pages, first, last)
+
+
+@kv4_select.register_fake
+def _(data, bounds, bound_scales, error_word, q, block_table, lengths, num_pages, first=1, last=1):
+    return q.new_empty((block_table.shape[0], data.shape[1], num_pages), dtype=torch.int32)

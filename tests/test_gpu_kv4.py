@@ -465,6 +465,30 @@ def test_bad_pages_and_positions_set_the_error_word(cuda):
     assert cache.read_error() == 0x202
 
 
+def test_torch_ops_match_the_cache(cuda):
+    """torch.ops.starkv.kv4_* give what the KV4Cache methods give."""
+    from starkv import torch_ops  # noqa: F401
+    o = torch.ops.starkv
+    made = Made(cuda, [300, 77], 2, 32, F16, seed=13, garbage=False)
+    c, q = made.cache, rnd((2, 1, 4, 128), F16, 14, cuda)
+    other = KV4Cache(c.num_pages, 2, 32, device=cuda)
+    o.kv4_write(other.data, other.bounds, other.bound_scales, other.error_word, made.k, made.v, made.table,
+                ints([0, 0], cuda), made.lengths)
+    assert all(torch.equal(getattr(c, n), getattr(other, n)) for n in ("data", "bounds", "bound_scales"))
+    kv = o.kv4_read(c.data, c.error_word, made.table, ints([0, 5], cuda), 50, F16)
+    k, v = c.read(made.table, ints([0, 5], cuda), 50, dtype=F16)
+    assert torch.equal(kv[0], k) and torch.equal(kv[1], v)
+    pages = o.kv4_select(c.data, c.bounds, c.bound_scales, c.error_word, q, made.table, made.lengths, 4)
+    assert torch.equal(pages, c.select(q, made.table, made.lengths, 4))
+    out, lse = o.kv4_attn(c.data, c.error_word, q, made.table, made.lengths, SCALING, None, pages)
+    want, wlse = c.attend(q, made.table, made.lengths, SCALING, pages=pages, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    with pytest.raises(StarKVError):
+        KV4Cache.from_tensors(c.data[:, :1], None, None, c.error_word)
+    with pytest.raises(StarKVError):
+        KV4Cache.from_tensors(c.data, c.bounds, None, c.error_word)
+
+
 def test_single_query_shape(cuda):
     """(B, Hq, 128) queries give (B, Hq, 128) outputs, the same as one token of (B, 1, Hq, 128)."""
     made = Made(cuda, [100, 33], 2, 16, F16, seed=5)
