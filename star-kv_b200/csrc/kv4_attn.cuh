@@ -37,7 +37,7 @@
 
 namespace starkv {
 
-constexpr int kKv4PadTiles = 2;
+constexpr int kKv4PadTiles = 4;
 constexpr int kKv4MaxGrid = 160;            // CTAs the workspace has room for
 constexpr int kKv4MaxCols = 16, kKv4MaxWarps = 15;
 constexpr int kKv4PartFloats = kKv4MaxCols * 130;   // one piece: o (cols, 128), base (cols), l (cols)
@@ -64,7 +64,13 @@ struct Kv4AttnParams {
   float* heads;                             // (grid, kKv4MaxWarps, kKv4PartFloats)
   float scaling;
   int num_selected, q_dtype, out_dtype, batch, queries, q_heads, group, width, col_blocks;
+  uint64_t group_m, col_blocks_m;           // kv4_reciprocal of the two
 };
+
+// n / d for n * d < 2^38, from floor(2^38 / d) + 1 (a division of run-time integers takes some 40
+// dependent instructions, and what runs once a segment is made of such chains).
+__host__ __device__ constexpr uint64_t kv4_reciprocal(int d) { return ((uint64_t)1 << 38) / (unsigned)d + 1; }
+__device__ __forceinline__ int kv4_divide(int n, uint64_t reciprocal) { return (int)(((uint64_t)(unsigned)n * reciprocal) >> 38); }
 
 __device__ __forceinline__ void kv4_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -110,7 +116,7 @@ __device__ __forceinline__ int64_t kv4_length(const Kv4AttnParams& p, int b) {
   }
   return n < 0 ? 0 : n;
 }
-// Tiles of one of its segments, with two that hold nothing: about what a warp's change of segment
+// Tiles of one of its segments, with four that hold nothing: about what a warp's change of segment
 // costs, so that stretches with many short segments are not longer than others.
 __device__ __forceinline__ int kv4_tiles(const Kv4AttnParams& p, int64_t len) {
   if (len <= 0) return 0;
@@ -120,8 +126,8 @@ __device__ __forceinline__ int kv4_tiles(const Kv4AttnParams& p, int64_t len) {
 // Writes one column of a segment, a lane 4 channels: o / l and log(l) above the base.
 __device__ __forceinline__ void kv4_store_column(const Kv4AttnParams& p, int b, int hc, int col, int cols, float4 o, float base,
                                               float l) {
-  const int lane = threadIdx.x & 31, head = hc / p.col_blocks, gcol = (hc - head * p.col_blocks) * cols + col;
-  const int qi = gcol / p.group, qh = head * p.group + gcol - qi * p.group;
+  const int lane = threadIdx.x & 31, head = kv4_divide(hc, p.col_blocks_m), gcol = (hc - head * p.col_blocks) * cols + col;
+  const int qi = kv4_divide(gcol, p.group_m), qh = head * p.group + gcol - qi * p.group;
   const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;    // a NaN stays one
   o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
   const int64_t at = b * p.os[0] + qi * p.os[1] + qh * p.os[2] + lane * 4;
@@ -148,6 +154,12 @@ __device__ __forceinline__ void kv4_cp_async4(void* dst, const float* mask, int 
   const int bytes = i < width ? 4 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(mask + (bytes ? i : 0)), "r"(bytes)
                : "memory");
+}
+
+// The largest of a warp's values, by its order-preserving integers.
+__device__ __forceinline__ float kv4_warp_max(float x) {
+  const int u = __float_as_int(x), k = __reduce_max_sync(0xffffffffu, u ^ ((u >> 31) & 0x7fffffff));
+  return __int_as_float(k ^ ((k >> 31) & 0x7fffffff));
 }
 
 __device__ __forceinline__ uint4 kv4_lds128(uint32_t at) {
@@ -247,8 +259,8 @@ struct Kv4Columns {
 // The queries of 8 columns of a segment as the scores' operands: five vectors a lane in `buf` (32
 // vectors apart), the four groups' B operands and { sums of q for s, for m, scale, - }.
 __device__ __forceinline__ void kv4_prepare(const Kv4AttnParams& p, uint4* buf, int b, int hc, int nt, int cols, int lane) {
-  const int r = lane >> 2, c = lane & 3, head = hc / p.col_blocks;
-  const int gcol = (hc - head * p.col_blocks) * cols + nt * 8 + r, qi = gcol / p.group;
+  const int r = lane >> 2, c = lane & 3, head = kv4_divide(hc, p.col_blocks_m);
+  const int gcol = (hc - head * p.col_blocks) * cols + nt * 8 + r, qi = kv4_divide(gcol, p.group_m);
   const bool f16 = p.q_dtype == STARKV_F16;
   const int64_t at = b * p.qs[0] + qi * p.qs[1] + (head * p.group + gcol - qi * p.group) * p.qs[2] + c * 8;
   const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + at);
@@ -304,7 +316,7 @@ __device__ __forceinline__ void kv4_prepare(const Kv4AttnParams& p, uint4* buf, 
 // Takes a segment's prepared queries and clears its sums.
 template <int NT>
 __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>& s, const uint4* buf, int hc, int len, int lane) {
-  const int first = hc % p.col_blocks * (NT * 8), c = lane & 3;
+  const int first = (hc - kv4_divide(hc, p.col_blocks_m) * p.col_blocks) * (NT * 8), c = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (NT == 1) {
@@ -320,7 +332,7 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       s.cs[nt][u] = __uint_as_float(__shfl_sync(0xffffffffu, v.z, (2 * c + u) * 4));
-      s.end[nt][u] = len - p.queries + 1 + (first + nt * 8 + 2 * c + u) / p.group;
+      s.end[nt][u] = len - p.queries + 1 + kv4_divide(first + nt * 8 + 2 * c + u, p.group_m);
       s.l[nt][u] = 0.f;
       s.base[nt][u] = 0.f;
       s.thr[nt][u] = -INFINITY;
@@ -595,7 +607,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       more = use.left > 0;
       there = false;
       if (!more) return;
-      head = use.hc / p.col_blocks;
+      head = kv4_divide(use.hc, p.col_blocks_m);
       seq = use.b;
       tile = use.t & (p.pool.page_tiles - 1);
       int ord = use.t >> (p.pool.page_shift - 4);
@@ -699,7 +711,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 
       // ---- end of the segment, or of the stretch
       const int r = lane >> 2, c = lane & 3;
-      const int real = min(kCols, p.group * p.queries - use.hc % p.col_blocks * kCols);
+      const int real = min(kCols, p.group * p.queries - (use.hc - kv4_divide(use.hc, p.col_blocks_m) * p.col_blocks) * kCols);
       // pieces 2 w: the last of warp w, 2 w + 1: one before it
       const int pi = 2 * warp + (use.left > n);
       float* part = piece_at(pi);
@@ -748,7 +760,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     if (kv4_length(p, b) == 0)
 #pragma unroll 1
       for (int i = warp; i < HC * kCols; i += W + 1)
-        if ((i / kCols % p.col_blocks) * kCols + i % kCols < p.group * p.queries)
+        if ((i / kCols) % p.col_blocks * kCols + i % kCols < p.group * p.queries)
           kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
   if (c0 >= c1) return;
   __syncthreads();
@@ -764,7 +776,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   const bool leads = my_start >= 0 && __ffs(same) - 1 == lane;
   const bool whole = pc.start >= c0 && pc.start + pc.tiles <= c1;
   const int side = pc.start <= c0 ? 0 : 1;
-  const int cols = leads ? min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols) : 0;
+  const int cols = leads ? min(kCols, p.group * p.queries - (pc.hc - kv4_divide(pc.hc, p.col_blocks_m) * p.col_blocks) * kCols) : 0;
   int units = cols;                         // up to and with a leader's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -782,15 +794,10 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     const int col = u - __shfl_sync(0xffffffffu, units - cols, lead);
     const bool in = members >> lane & 1;
     const float* at = piece_at(in ? lane : lead);
-    const float base = in ? at[kCols * 128 + col] : -INFINITY;
-    float mx = base, l = in ? at[kCols * 129 + col] : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float w = kv4_weight(base, mx);
-    l *= w;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    const float base = in ? at[kCols * 128 + col] : -INFINITY, mine = in ? at[kCols * 129 + col] : 0.f;
+    const float mx = kv4_warp_max(base), w = kv4_weight(base, mx), wl = w * mine;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
 #pragma unroll 1
     for (unsigned m = members; m;) {        // four pieces a turn, their loads in flight together
       float4 v[4];
@@ -798,8 +805,10 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = m ? __ffs(m) - 1 : lead;
+        const float lk = __shfl_sync(0xffffffffu, wl, k);
         wk[i] = __shfl_sync(0xffffffffu, w, k);
-        if (!m) wk[i] = 0.f;
+        l += m ? lk : 0.f;
+        wk[i] = m ? wk[i] : 0.f;
         v[i] = *reinterpret_cast<const float4*>(piece_at(k) + col * 128 + lane * 4);
         m &= m - 1;
       }
@@ -840,7 +849,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     const Kv4Piece pc = sm.piece[cross[s]];
     const int first = pc.start / per, n = (pc.start + pc.tiles - 1) / per - first + 1;
     const int skip = pc.start > first * per ? 1 : 0;
-    const int cols = min(kCols, p.group * p.queries - pc.hc % p.col_blocks * kCols);
+    const int cols = min(kCols, p.group * p.queries - (pc.hc - kv4_divide(pc.hc, p.col_blocks_m) * p.col_blocks) * kCols);
     for (int col = 0; col < cols; ++col) {
       if (unit++ % (W + 1) != warp) continue;
       float mx = -INFINITY, l = 0.f;
@@ -856,19 +865,15 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
           v[i] = __ldcg(reinterpret_cast<const float4*>(
               p.parts + ((int64_t)(first + min(k0 + i, n - 1)) * 2 + (min(k0 + i, n - 1) == 0 ? skip : 0)) * kKv4PartFloats +
               col * 128 + lane * 4));       // past the last piece: that one again, times 0
-        float joint = fmaxf(mx, base);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) joint = fmaxf(joint, __shfl_xor_sync(0xffffffffu, joint, o));
-        const float w = kv4_weight(base, joint), old = kv4_weight(mx, joint);
-        float sum = k < n ? w * lk : 0.f;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        l = l * old + sum;
+        const float joint = fmaxf(mx, kv4_warp_max(base)), old = kv4_weight(mx, joint);
+        const float w = kv4_weight(base, joint), wl = w * lk;
+        l *= old;
         acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
         mx = joint;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float wi = __shfl_sync(0xffffffffu, w, i);
+          l += __shfl_sync(0xffffffffu, wl, i);
           acc.x = fmaf(wi, v[i].x, acc.x), acc.y = fmaf(wi, v[i].y, acc.y), acc.z = fmaf(wi, v[i].z, acc.z),
           acc.w = fmaf(wi, v[i].w, acc.w);
         }
