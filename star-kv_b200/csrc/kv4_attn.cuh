@@ -21,7 +21,9 @@
 //     operand: the running sums stay centred, so that the truncating fp32 additions
 //     of the tensor cores do not act on sums 8 s times as large (measured at 32K
 //     tokens: relative error 1.5e-3 when the -8 is taken at the end instead).
-//     The centres add sum w m_g.
+//     The centres add sum w m_g, and a row of ones sums the rounded weights: dividing by
+//     that sum takes their rounding out of what they have in common (one key that
+//     outweighs the rest has no error from it).  The log-sum-exp has the sum in fp32.
 //     w is 2^(x - m + 11 - e): m a running maximum that may trail by 2^4, e >= 0 the
 //     exponent that keeps every s_g so far <= 2^e, so neither small weights nor
 //     large s leave fp16.
@@ -39,13 +41,18 @@ namespace starkv {
 
 constexpr int kKv4PadTiles = 4;
 constexpr int kKv4MaxGrid = 160;            // CTAs the workspace has room for
-constexpr int kKv4MaxCols = 16, kKv4MaxWarps = 15;
-constexpr int kKv4PartFloats = kKv4MaxCols * 130;   // one piece: o (cols, 128), base (cols), l (cols)
+constexpr int kKv4MaxCols = 16;
+// One piece of a segment: o (cols, 128), then per column the base, the sum of the weights and the
+// sum of the weights as rounded to fp16.
+constexpr int kKv4PieceRows = 131;
+constexpr int kKv4PartFloats = kKv4MaxCols * kKv4PieceRows;
+// Two pieces a warp: up to 15 warps of 8 columns or 11 of 16.
+constexpr int kKv4HeadFloats = 2 * 11 * 16 * kKv4PieceRows;
 constexpr size_t kKv4CounterBytes = 1024;
 static_assert(kKv4MaxGrid * sizeof(int) <= kKv4CounterBytes, "a counter a CTA");
-// counters, two pieces a CTA for other CTAs, one a warp
+// counters, two pieces a CTA for other CTAs, two a warp
 constexpr size_t kKv4WorkspaceBytes =
-    kKv4CounterBytes + (size_t)kKv4MaxGrid * (2 + kKv4MaxWarps) * kKv4PartFloats * sizeof(float);
+    kKv4CounterBytes + (size_t)kKv4MaxGrid * (2 * kKv4PartFloats + kKv4HeadFloats) * sizeof(float);
 
 struct Kv4AttnParams {
   Kv4Pool pool;
@@ -61,7 +68,7 @@ struct Kv4AttnParams {
   const int* pages;
   int* counters;                            // (kKv4MaxGrid) zero between calls
   float* parts;                             // (grid, 2, kKv4PartFloats)
-  float* heads;                             // (grid, kKv4MaxWarps, kKv4PartFloats)
+  float* heads;                             // (grid, kKv4HeadFloats)
   float scaling;
   int num_selected, q_dtype, out_dtype, batch, queries, q_heads, group, width, col_blocks;
   uint64_t group_m, col_blocks_m;           // kv4_reciprocal of the two
@@ -123,12 +130,12 @@ __device__ __forceinline__ int kv4_tiles(const Kv4AttnParams& p, int64_t len) {
   return (p.pages ? p.num_selected * p.pool.page_tiles : (int)((len + kKv4Tile - 1) >> 4)) + kKv4PadTiles;
 }
 
-// Writes one column of a segment, a lane 4 channels: o / l and log(l) above the base.
+// Writes one column of a segment, a lane 4 channels: o over the rounded weights' sum, log(l) above the base.
 __device__ __forceinline__ void kv4_store_column(const Kv4AttnParams& p, int b, int hc, int col, int cols, float4 o, float base,
-                                              float l) {
+                                              float l, float rounded) {
   const int lane = threadIdx.x & 31, head = kv4_divide(hc, p.col_blocks_m), gcol = (hc - head * p.col_blocks) * cols + col;
   const int qi = kv4_divide(gcol, p.group_m), qh = head * p.group + gcol - qi * p.group;
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;    // a NaN stays one
+  const float inv = l == 0.f ? 0.f : 1.f / rounded;   // a NaN stays one
   o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
   const int64_t at = b * p.os[0] + qi * p.os[1] + qh * p.os[2] + lane * 4;
   if (p.out_dtype == STARKV_F32) {
@@ -251,7 +258,7 @@ struct Kv4Columns {
   float cs[NT][2];                          // a column's scores, as computed (an eighth), to the log2 domain
   int end[NT][2];                           // first position a column does not attend to
   float o[8][NT][4], l[NT][2];
-  float z[NT][4];                           // sum w m: group j in rows j / 2 (and every second one) and j / 2 + 8
+  float z[NT][4];                           // sum w m: group j in rows j / 2 and j / 2 + 8; sum w in row 2
   float base[NT][2], thr[NT][2];            // w = 2^(x - base); x beyond thr moves the base
   int e;
 };
@@ -458,6 +465,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
   const uint4 va = kv4_lds128(tl + at.code + kKv4VCodes), vb = kv4_lds128(tl + at.code + kKv4VCodes + 512);
   uint2 ma = kv4_lds64(tl + at.vmid), mb = kv4_lds64(tl + at.vmid + 128);
   if (MASK || EDGE) ma.x &= la, ma.y &= la, mb.x &= lb, mb.y &= lb;
+  if (lane >> 2 == 2) ma.x = mb.x = 0x3c003c00u;   // row 2: ones
   uint32_t p0[NT], p1[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -502,11 +510,14 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int HC = p.pool.heads * p.col_blocks;
-  // piece i of the CTA: o (cols, 128), base (cols), l (cols).  A warp's last piece lies over its ring,
-  // one before it (the end of a segment that an earlier warp began) in the workspace.
+  // piece i of the CTA (see kKv4PieceRows): 2 w is the last of warp w and lies over its ring, 2 w + 1 is
+  // the end of a segment that an earlier warp began and lies in the workspace
+  constexpr int kPiece = kCols * kKv4PieceRows;
+  static_assert(2 * W * kPiece <= kKv4HeadFloats && kPiece <= kKv4PartFloats, "room in the workspace");
+  static_assert(kPiece * sizeof(float) <= sizeof(sm.ring[0]), "room over the ring");
+  float* const heads = p.heads + (int64_t)blockIdx.x * kKv4HeadFloats;
   auto piece_at = [&](int i) {
-    return i & 1 ? p.heads + ((int64_t)blockIdx.x * kKv4MaxWarps + (i >> 1)) * kKv4PartFloats
-                 : reinterpret_cast<float*>(sm.ring[i >> 1][0]);
+    return i & 1 ? heads + (i >> 1) * kPiece : reinterpret_cast<float*>(sm.ring[i >> 1][0]);
   };
 
   // ---- the line of tiles: total, this CTA's stretch, the warps' first sequences
@@ -712,9 +723,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       // ---- end of the segment, or of the stretch
       const int r = lane >> 2, c = lane & 3;
       const int real = min(kCols, p.group * p.queries - (use.hc - kv4_divide(use.hc, p.col_blocks_m) * p.col_blocks) * kCols);
-      // pieces 2 w: the last of warp w, 2 w + 1: one before it
+      // a whole segment that is not the stretch's last goes through a place of its own: the ring is
+      // in use, and the piece before it waits for the merge
+      const bool whole = n == use.tiles;
       const int pi = 2 * warp + (use.left > n);
-      float* part = piece_at(pi);
+      float* part = whole && use.left > n ? heads + (W + warp) * kPiece : piece_at(pi);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -728,6 +741,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
             part[kCols * 128 + col] = s.thr[nt][u] == -INFINITY ? -INFINITY : s.base[nt][u];
             part[kCols * 129 + col] = l;
           }
+          if (r == 2) part[kCols * 130 + col] = s.z[nt][u];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float y = __shfl_sync(0xffffffffu, s.z[nt][u + 2 * (j & 1)], (j >> 1) * 4 + c);
@@ -737,12 +751,12 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
                               fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y), fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y));
           }
         }
-      if (n == use.tiles) {                 // the whole segment
+      if (whole) {
         __syncwarp();
 #pragma unroll 1
         for (int col = 0; col < real; ++col)
           kv4_store_column(p, use.b, use.hc, col, kCols, *reinterpret_cast<const float4*>(part + col * 128 + lane * 4),
-                           part[kCols * 128 + col], part[kCols * 129 + col]);
+                           part[kCols * 128 + col], part[kCols * 129 + col], part[kCols * 130 + col]);
         __syncwarp();
       } else if (lane == 0) {
         Kv4Piece& q = sm.piece[pi];
@@ -761,7 +775,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 #pragma unroll 1
       for (int i = warp; i < HC * kCols; i += W + 1)
         if ((i / kCols) % p.col_blocks * kCols + i % kCols < p.group * p.queries)
-          kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+          kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f, 0.f);
   if (c0 >= c1) return;
   __syncthreads();
 
@@ -794,10 +808,11 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     const int col = u - __shfl_sync(0xffffffffu, units - cols, lead);
     const bool in = members >> lane & 1;
     const float* at = piece_at(in ? lane : lead);
-    const float base = in ? at[kCols * 128 + col] : -INFINITY, mine = in ? at[kCols * 129 + col] : 0.f;
-    const float mx = kv4_warp_max(base), w = kv4_weight(base, mx), wl = w * mine;
+    const float base = in ? at[kCols * 128 + col] : -INFINITY;
+    const float mx = kv4_warp_max(base), w = kv4_weight(base, mx);
+    const float wl = in ? w * at[kCols * 129 + col] : 0.f, wr = in ? w * at[kCols * 130 + col] : 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
+    float l = 0.f, rounded = 0.f;
 #pragma unroll 1
     for (unsigned m = members; m;) {        // four pieces a turn, their loads in flight together
       float4 v[4];
@@ -805,9 +820,10 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int k = m ? __ffs(m) - 1 : lead;
-        const float lk = __shfl_sync(0xffffffffu, wl, k);
+        const float lk = __shfl_sync(0xffffffffu, wl, k), rk = __shfl_sync(0xffffffffu, wr, k);
         wk[i] = __shfl_sync(0xffffffffu, w, k);
         l += m ? lk : 0.f;
+        rounded += m ? rk : 0.f;
         wk[i] = m ? wk[i] : 0.f;
         v[i] = *reinterpret_cast<const float4*>(piece_at(k) + col * 128 + lane * 4);
         m &= m - 1;
@@ -818,13 +834,15 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
         acc.w = fmaf(wk[i], v[i].w, acc.w);
     }
     if (__shfl_sync(0xffffffffu, whole, lead)) {
-      kv4_store_column(p, __shfl_sync(0xffffffffu, pc.b, lead), __shfl_sync(0xffffffffu, pc.hc, lead), col, kCols, acc, mx, l);
+      kv4_store_column(p, __shfl_sync(0xffffffffu, pc.b, lead), __shfl_sync(0xffffffffu, pc.hc, lead), col, kCols, acc, mx, l,
+                       rounded);
     } else {
       float* part = p.parts + ((int64_t)blockIdx.x * 2 + __shfl_sync(0xffffffffu, side, lead)) * kKv4PartFloats;
       __stcg(reinterpret_cast<float4*>(part + col * 128 + lane * 4), acc);
       if (lane == 0) {
         __stcg(part + kCols * 128 + col, mx);
         __stcg(part + kCols * 129 + col, l);
+        __stcg(part + kCols * 130 + col, rounded);
       }
     }
   }
@@ -852,13 +870,13 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     const int cols = min(kCols, p.group * p.queries - (pc.hc - kv4_divide(pc.hc, p.col_blocks_m) * p.col_blocks) * kCols);
     for (int col = 0; col < cols; ++col) {
       if (unit++ % (W + 1) != warp) continue;
-      float mx = -INFINITY, l = 0.f;
+      float mx = -INFINITY, l = 0.f, rounded = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k0 = 0; k0 < n; k0 += 16) {  // 16 pieces a turn, their loads in flight together
         const int k = k0 + (lane & 15);
         const float* pk = p.parts + ((int64_t)(first + k) * 2 + (k == 0 ? skip : 0)) * kKv4PartFloats;
         const float base = k < n ? __ldcg(pk + kCols * 128 + col) : -INFINITY;
-        const float lk = k < n ? __ldcg(pk + kCols * 129 + col) : 0.f;
+        const float lk = k < n ? __ldcg(pk + kCols * 129 + col) : 0.f, rk = k < n ? __ldcg(pk + kCols * 130 + col) : 0.f;
         float4 v[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -866,19 +884,21 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
               p.parts + ((int64_t)(first + min(k0 + i, n - 1)) * 2 + (min(k0 + i, n - 1) == 0 ? skip : 0)) * kKv4PartFloats +
               col * 128 + lane * 4));       // past the last piece: that one again, times 0
         const float joint = fmaxf(mx, kv4_warp_max(base)), old = kv4_weight(mx, joint);
-        const float w = kv4_weight(base, joint), wl = w * lk;
+        const float w = kv4_weight(base, joint), wl = w * lk, wr = w * rk;
         l *= old;
+        rounded *= old;
         acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
         mx = joint;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float wi = __shfl_sync(0xffffffffu, w, i);
           l += __shfl_sync(0xffffffffu, wl, i);
+          rounded += __shfl_sync(0xffffffffu, wr, i);
           acc.x = fmaf(wi, v[i].x, acc.x), acc.y = fmaf(wi, v[i].y, acc.y), acc.z = fmaf(wi, v[i].z, acc.z),
           acc.w = fmaf(wi, v[i].w, acc.w);
         }
       }
-      kv4_store_column(p, pc.b, pc.hc, col, kCols, acc, mx, l);
+      kv4_store_column(p, pc.b, pc.hc, col, kCols, acc, mx, l, rounded);
     }
   }
 }

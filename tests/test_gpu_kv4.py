@@ -212,6 +212,15 @@ def test_attention_split_over_the_machine(cuda, lens, Hkv, G, Q):
     check_attention(made, rnd((len(lens), Q, Hkv * G, 128), F16, 6, cuda))
 
 
+@pytest.mark.parametrize("B,Hkv,G,Q,top", [(300, 8, 4, 1, 130), (500, 4, 1, 1, 60), (200, 4, 4, 4, 90), (64, 8, 4, 1, 700)])
+def test_attention_many_short_sequences(cuda, B, Hkv, G, Q, top):
+    """Stretches that hold the end of one sequence, several whole ones and the start of another."""
+    rng = np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(0, top, B)]
+    made = Made(cuda, lens, Hkv, 16, F16, seed=B)
+    check_attention(made, rnd((B, Q, Hkv * G, 128), F16, 7, cuda))
+
+
 @pytest.mark.parametrize("out_dtype", [F16, BF16])
 def test_attention_output_types(cuda, out_dtype):
     made = Made(cuda, [100, 40], 2, 32, F16, seed=8)
