@@ -363,10 +363,15 @@ __global__ void __launch_bounds__(256, 2) kv4_write_kernel(const Kv4IoParams p) 
   bd[32 + lane] = code(dn.x, false) | code(dn.y, false) << 8 | code(dn.z, false) << 16 | code(dn.w, false) << 24;
 }
 
-// A lane's 8 channels from 8 nibbles in channel order.
+// A lane's 8 channels from 8 nibbles in channel order.  A nibble becomes a float by standing in the
+// low byte of 2^23 (one byte permute), and the offset 2^23 + 8 comes off exactly.
 __device__ __forceinline__ void kv4_values8(uint32_t w, float s, float m, float* f) {
+  const uint32_t even = w & 0x0f0f0f0fu, odd = w >> 4 & 0x0f0f0f0fu;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __fmaf_rn(s, (float)((int)((w >> (4 * i)) & 15u) - 8), m);
+  for (int i = 0; i < 8; ++i) {
+    const float c = __uint_as_float(__byte_perm(i & 1 ? odd : even, 0x4b000000u, 0x7440 + (i >> 1)));
+    f[i] = __fmaf_rn(s, c - 8388616.f, m);
+  }
 }
 
 template <typename T>
@@ -421,28 +426,35 @@ __global__ void __launch_bounds__(kKv4ReadWarps * 32) kv4_read_kernel(const Kv4I
   }
   const uint8_t* tile = buf[warp];
   const int c = l16 & 3, g = l16 >> 2;
-  T* kp = reinterpret_cast<T*>(const_cast<void*>(p.k)) + b * p.ks[0] + head * p.ks[2] + l16 * 8;
-  T* vp = reinterpret_cast<T*>(const_cast<void*>(p.v)) + b * p.vs[0] + head * p.vs[2] + l16 * 8;
+  T* kp = reinterpret_cast<T*>(const_cast<void*>(p.k)) + b * p.ks[0] + head * p.ks[2] + l16 * 8 + (i0 + half) * p.ks[1];
+  T* vp = reinterpret_cast<T*>(const_cast<void*>(p.v)) + b * p.vs[0] + head * p.vs[2] + l16 * 8 + (i0 + half) * p.vs[1];
+  // rows of the tile that are written, and those that hold tokens
+  const int first = i0 < 0 ? (int)-i0 : 0, rows = (int)min((int64_t)kKv4Tile, p.num_tokens - i0);
+  const int live = page >= 0 ? (int)min((int64_t)kKv4Tile, count - i0) : 0;
 #pragma unroll
   for (int it = 0; it < 8; ++it) {
     const int tt = 2 * it + half;
-    const int64_t i = i0 + tt;
-    if (i < 0 || i >= p.num_tokens) continue;
-    float fk[8], fv[8];
-    if (page >= 0 && i < count) {
-      const __half* kpar = reinterpret_cast<const __half*>(tile + kv4_kparam(tt, g));
-      kv4_values8(*reinterpret_cast<const uint32_t*>(tile + tt * 64 + c * 16 + g * 4), __half2float(kpar[0]),
-                  __half2float(kpar[4]), fk);
-      const uint32_t w = (uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_vcode(tt, g, 2 * c)) |
-                         ((uint32_t)*reinterpret_cast<const uint16_t*>(tile + kv4_vcode(tt, g, 2 * c + 1)) << 16);
-      const __half* vpar = reinterpret_cast<const __half*>(tile + kv4_vparam(tt, g));
-      kv4_values8(w, __half2float(vpar[0]), __half2float(vpar[8]), fv);
-    } else {
+    if (tt >= first && tt < rows) {
+      float fk[8], fv[8];
+      if (tt < live) {
+        // the lane's part of an offset is the same in every step, the step's part a constant
+        const __half* kpar = reinterpret_cast<const __half*>(tile + kv4_kparam(half, g) + kv4_kparam(2 * it, 0) - kKv4KParams);
+        kv4_values8(*reinterpret_cast<const uint32_t*>(tile + half * 64 + c * 16 + g * 4 + it * 128), __half2float(kpar[0]),
+                    __half2float(kpar[4]), fk);
+        const uint8_t* quads = tile + kv4_vcode(half, g, 2 * c) + kv4_vcode(2 * it, 0, 0) - kKv4VCodes;
+        const uint32_t w = (uint32_t)*reinterpret_cast<const uint16_t*>(quads) |
+                           ((uint32_t)*reinterpret_cast<const uint16_t*>(quads + 64) << 16);
+        const __half* vpar = reinterpret_cast<const __half*>(tile + kv4_vparam(half, g) + it * 32);
+        kv4_values8(w, __half2float(vpar[0]), __half2float(vpar[8]), fv);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) fk[j] = fv[j] = 0.f;
+        for (int j = 0; j < 8; ++j) fk[j] = fv[j] = 0.f;
+      }
+      kv4_store8(kp, fk);
+      kv4_store8(vp, fv);
     }
-    kv4_store8(kp + i * p.ks[1], fk);
-    kv4_store8(vp + i * p.vs[1], fv);
+    kp += 2 * p.ks[1];
+    vp += 2 * p.vs[1];
   }
 }
 
