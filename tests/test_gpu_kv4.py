@@ -212,7 +212,7 @@ def test_attention_split_over_the_machine(cuda, lens, Hkv, G, Q):
     check_attention(made, rnd((len(lens), Q, Hkv * G, 128), F16, 6, cuda))
 
 
-@pytest.mark.parametrize("B,Hkv,G,Q,top", [(300, 8, 4, 1, 130), (500, 4, 1, 1, 60), (200, 4, 4, 4, 90), (64, 8, 4, 1, 700)])
+@pytest.mark.parametrize("B,Hkv,G,Q,top", [(300, 8, 4, 1, 130), (500, 4, 1, 1, 60), (200, 4, 4, 4, 90), (64, 8, 4, 1, 700), (1300, 1, 2, 1, 40)])
 def test_attention_many_short_sequences(cuda, B, Hkv, G, Q, top):
     """Stretches that hold the end of one sequence, several whole ones and the start of another."""
     rng = np.random.default_rng(B)
