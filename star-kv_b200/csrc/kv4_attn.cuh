@@ -441,6 +441,15 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
   const uint32_t big = __vimax3_u16x2(__vimax3_u16x2(ta.x, ta.y, ta.z), __vimax3_u16x2(ta.w, tb.x, tb.y),
                                       __vimax3_u16x2(tb.z, tb.w, lim));
   over |= big != lim;
+  // With 16 columns the value codes come in before the vote (53 -> 50 us for 4 drafts; there are fewer
+  // warps to hide the loads), with 8 after it (their registers are needed for it: 2 % slower before).
+  uint4 va, vb;
+  uint2 ma, mb;
+  auto load_values = [&]() {
+    va = kv4_lds128(tl + at.code + kKv4VCodes), vb = kv4_lds128(tl + at.code + kKv4VCodes + 512);
+    ma = kv4_lds64(tl + at.vmid), mb = kv4_lds64(tl + at.vmid + 128);
+  };
+  if (NT > 1) load_values();
   // ---- a score or an s that the base does not cover
   if (__any_sync(0xffffffffu, over)) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
@@ -471,8 +480,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
     s.e = e_new;
   }
   // ---- weights and values
-  const uint4 va = kv4_lds128(tl + at.code + kKv4VCodes), vb = kv4_lds128(tl + at.code + kKv4VCodes + 512);
-  uint2 ma = kv4_lds64(tl + at.vmid), mb = kv4_lds64(tl + at.vmid + 128);
+  if (NT == 1) load_values();
   if (MASK || EDGE) ma.x &= la, ma.y &= la, mb.x &= lb, mb.y &= lb;
   if (lane >> 2 == 2) ma.x = mb.x = 0x3c003c00u;   // row 2: ones
   uint32_t p0[NT], p1[NT];
