@@ -234,6 +234,7 @@ struct Kv4AttnSmem {
   int scan[W + 1];
   int upto[(W + 1) * 32];                   // tiles of the sequences up to and with a thread's
   int last[2];
+  int empties;                              // there are sequences of no tokens
 };
 
 __device__ __forceinline__ uint2 kv4_lds64(uint32_t at) {
@@ -542,7 +543,12 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   const int per_thread = (p.batch + kThreads - 1) / kThreads;
   const int b_lo = tid * per_thread, b_hi = min(b_lo + per_thread, p.batch);
   int mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += kv4_tiles(p, kv4_length(p, b)) * HC;
+  bool empty = false;                       // a sequence of no tokens
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int t = kv4_tiles(p, kv4_length(p, b));
+    mine += t * HC;
+    empty |= t == 0;
+  }
   int upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -556,7 +562,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   }
   if (tid < Smem::kShared) sm.shared_start[tid] = -1;
   fence_mbar_init();
-  __syncthreads();
+  const int empties = __syncthreads_or(empty);
+  if (tid == 0) sm.empties = empties;       // kept there: it would take a register all along
   int warps = lane <= W ? sm.scan[lane] : 0;  // tiles up to and with a warp's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -786,13 +793,19 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       use.advance(p, n);
     }
   }
-  // sequences without a tile: nothing to attend to
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x)
-    if (kv4_length(p, b) == 0)
+  // sequences of no tokens: zeros, the columns of each spread over the grid's warps
+  if (sm.empties) {
 #pragma unroll 1
-      for (int i = warp; i < HC * kCols; i += W + 1)
-        if ((i / kCols) % p.col_blocks * kCols + i % kCols < p.group * p.queries)
-          kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f, 0.f);
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      unsigned none = __ballot_sync(0xffffffffu, b0 + lane < p.batch && kv4_length(p, min(b0 + lane, p.batch - 1)) == 0);
+      for (; none; none &= none - 1) {
+        const int b = b0 + __ffs(none) - 1;
+        for (int i = ((blockIdx.x + b) % gridDim.x) * (W + 1) + warp; i < HC * kCols; i += gridDim.x * (W + 1))
+          if ((i / kCols) % p.col_blocks * kCols + i % kCols < p.group * p.queries)
+            kv4_store_column(p, b, i / kCols, i % kCols, kCols, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f, 0.f);
+      }
+    }
+  }
   if (c0 >= c1) return;
   __syncthreads();
 
