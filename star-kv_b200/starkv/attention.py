@@ -58,6 +58,14 @@ def apply_rotary_pos_emb_custom(x, cos, sin, unsqueeze_dim=1):
     return (x * cos) + (rotate_half(x) * sin)
 
 
+def additive_mask(mask: torch.Tensor) -> torch.Tensor:
+    """A mask in fp32 to be added to scores: boolean and whole-number masks keep (0) what
+    is not zero and drop (-inf) the rest, floating masks stay as they are."""
+    if mask.is_floating_point():
+        return mask.to(torch.float32)
+    return torch.zeros(mask.shape, dtype=torch.float32, device=mask.device).masked_fill_(mask == 0, float("-inf"))
+
+
 try:                                                    # transformers' cache base class (the model code's type)
     from transformers.cache_utils import Cache as _HFCache
 except Exception:                                       # pragma: no cover - transformers absent
@@ -245,10 +253,14 @@ class LlamaCustomAttention(nn.Module):
     # ---- helpers
     @staticmethod
     def _decode_mask(attention_mask, B, L):
+        """The newest token's mask as the kernels take it, additive fp32 (B, L): the last
+        row of a (B, 1, q, L) mask, or a (B, L) one.  A boolean or whole-number mask says
+        which positions count (transformers' masks for its default SDPA attention and
+        its 2-D padding masks), a floating one is added to the scores."""
         if attention_mask is None:
             return None
         m = attention_mask[:, 0, -1, :L] if attention_mask.dim() == 4 else attention_mask[:, :L]
-        return m.to(torch.float32).expand(B, L).contiguous()
+        return additive_mask(m).expand(B, L).contiguous()
 
     def _decode_on_tensors(self, q_rot, keys, values, attention_mask):
         """Decode over an HF cache's latent tensors (B, Hkv, L, r) / (B, L, rv) in place."""

@@ -83,3 +83,20 @@ def test_oracle_attention_is_softmax():
     assert (w[0][:, 8] == 0).all() and np.allclose(w.sum(-1), 1)
     out, lse, _ = O.attend(q, k[:1], v[:1], 0.1)                # one token, two queries: the first sees nothing
     assert (out[0] == 0).all() and np.isneginf(lse[0]).all() and np.allclose(out[1], v[:1])
+
+
+def test_decode_masks_of_every_kind():
+    """Boolean and whole-number masks keep or drop positions; floating masks are added."""
+    from starkv.attention import LlamaCustomAttention as A
+    inf = float("inf")
+    keep = torch.tensor([[False, True, True, True, True], [True, True, True, False, True]])
+    want = torch.tensor([[-inf, 0, 0, 0], [0, 0, 0, -inf]])
+    rows = torch.stack([torch.ones_like(keep), keep], 1)[:, None]      # (2, 1, 2, 5): the last row counts
+    for m in (keep, keep.long(), keep.to(torch.uint8), rows, rows.int()):
+        got = A._decode_mask(m, 2, 4)
+        assert got.dtype == torch.float32 and got.is_contiguous() and torch.equal(got, want)
+    assert torch.equal(A._decode_mask(keep[:1], 2, 4), want[:1].expand(2, 4))
+    add = torch.tensor([[-inf, 0.5, -65504.0, 1.0]], dtype=torch.float16)
+    for m in (add, add[:, None, None]):
+        assert torch.equal(A._decode_mask(m, 2, 4), add.float().expand(2, 4))
+    assert A._decode_mask(None, 2, 4) is None
