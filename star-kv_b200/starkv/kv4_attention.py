@@ -12,6 +12,10 @@ the decoder layer's code does not change.
   pages, attention by torch SDPA over both;
 * decode, and up to ``MAX_DRAFT`` tokens at once: write, then attention over the
   pages; with ``keep_pages`` set, over the pages that ``KV4Cache.select`` keeps.
+
+The kernel takes one mask row a sequence and is causal by itself.  A mask with a row for
+each of several tokens goes to it in one call where the rows differ by causality only,
+and a token at a time where they do not (a draft's tree).
 """
 
 from __future__ import annotations
@@ -23,10 +27,20 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import prefill
-from .attention import LlamaCustomAttention, StarKVCache, apply_rotary_pos_emb_custom
+from .attention import LlamaCustomAttention, StarKVCache, additive_mask, apply_rotary_pos_emb_custom
 from .kv4 import KV4Cache
 
 MAX_DRAFT = 16
+
+
+def causal_rows(mask: torch.Tensor, n: int) -> bool:
+    """Whether the rows of mask (B, 1, T, >= n) are its last one with the positions behind
+    each token dropped (-inf, or the lowest number of the mask's type).  Synchronises."""
+    T = mask.shape[2]
+    rows = additive_mask(mask[:, 0, :, :n])
+    seen = torch.ones(T, n, dtype=torch.bool, device=mask.device).tril(n - T)
+    low = torch.finfo(mask.dtype).min if mask.is_floating_point() else float("-inf")
+    return bool(torch.where(seen, rows == rows[:, -1:], rows <= low).all())
 
 
 class KV4State:
@@ -57,6 +71,12 @@ class KV4State:
         if keep_pages:
             pages = self.cache.select(q, self.block_table, self.lengths, keep_pages)
         return self.cache.attend(q, self.block_table, self.lengths, scaling, mask=mask, pages=pages)
+
+    def attend_rows(self, q: torch.Tensor, scaling: float, rows: torch.Tensor, keep_pages: int = 0) -> torch.Tensor:
+        """``attend`` with a mask row for each token, rows (B, T, length): a call a token, in
+        which its row says what it attends to, the newer tokens too."""
+        return torch.stack([self.attend(q[:, i:i + 1], scaling, rows[:, i], keep_pages)[:, 0]
+                            for i in range(q.shape[1])], 1)
 
     def history(self, dtype: torch.dtype):
         """All tokens held as (k, v), each (B, length, Hkv, 128)."""
@@ -114,8 +134,14 @@ class KV4Attention(nn.Module):
             keys, values = k, v
         st.append(k, v)
         if T <= MAX_DRAFT and (before or T == 1):
-            mask = LlamaCustomAttention._decode_mask(attention_mask, B, st.length)
-            out = st.attend(q, self.scaling, mask, self.keep_pages)
+            by_row = attention_mask is not None and attention_mask.dim() == 4 and attention_mask.shape[2] == T > 1
+            # a graph cannot ask what the mask holds
+            if by_row and (torch.cuda.is_current_stream_capturing() or not causal_rows(attention_mask, st.length)):
+                rows = additive_mask(attention_mask[:, 0, :, :st.length]).expand(B, T, st.length)
+                out = st.attend_rows(q, self.scaling, rows, self.keep_pages)
+            else:
+                mask = LlamaCustomAttention._decode_mask(attention_mask, B, st.length)
+                out = st.attend(q, self.scaling, mask, self.keep_pages)
         elif attention_mask is None and not before:
             out = prefill.prompt_attention(q.transpose(1, 2), keys.transpose(1, 2), values.transpose(1, 2), self.scaling)
             out = out.transpose(1, 2)

@@ -105,3 +105,56 @@ def test_latent_layers_take_boolean_masks(cuda, quantized):
         attn = model.model.layers[0].self_attn
         outs.append(attn(x, (cos, sin), mask, **({"past_key_values_upper": cache} if quantized else {"past_key_values": cache}))[0])
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("kind", ["2d", "additive"])
+def test_drafts(cuda, kind):
+    check_padded(cuda, (3, 1, 4), kind)
+
+
+def with_rows(q, k, v, rows, scaling):
+    """64-bit attention of q (B, T, Hq, 128) over k / v (B, n, Hkv, 128) with the additive mask rows (B, T, n)."""
+    q, k, v = (t.double().transpose(1, 2) for t in (q, k, v))
+    grp = q.shape[1] // k.shape[1]
+    s = q @ k.repeat_interleave(grp, 1).transpose(-1, -2) * scaling + rows[:, None].double()
+    return (torch.softmax(s, -1) @ v.repeat_interleave(grp, 1)).transpose(1, 2)
+
+
+@pytest.mark.parametrize("kind", ["bool", "additive", "later"])
+@torch.no_grad()
+def test_draft_masks_whose_rows_differ(cuda, kind):
+    """A draft's tree: a token attends to the history and its own ancestors; ``later``: and a
+    token that comes after it.  Within 2e-3 as in test_gpu_kv4_attention.py."""
+    attn = small_model(cuda, (0, 1)).model.layers[0].self_attn
+    attn.o_proj = torch.nn.Identity()
+    B, P, T = 2, 90, 5
+    g = torch.Generator(device=cuda).manual_seed(14)
+    x = torch.randn(B, P + T, 512, generator=g, device=cuda).half() * 20
+    one = torch.ones(B, 1, 128, device=cuda, dtype=torch.float16)     # no rotation
+    pos = (one, one * 0)
+    cache = StarKVCache(128)
+    attn(x[:, :P], pos, None, past_key_values=cache)
+    keep = torch.ones(B, 1, T, P + T, dtype=torch.bool, device=cuda)
+    keep[0, ..., :33] = False                                         # padding
+    tree = torch.tensor([[1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 0, 1, 0, 0], [1, 1, 0, 1, 0], [1, 0, 1, 0, 1]], device=cuda).bool()
+    if kind == "later":
+        tree[1, 4] = True
+    keep[..., P:] = tree
+    rows = torch.zeros(keep.shape, dtype=torch.float16, device=cuda).masked_fill_(~keep, float("-inf"))
+    out, _ = attn(x[:, P:], pos, keep if kind == "bool" else rows, past_key_values=cache)
+    q, _, _ = attn.heads(x[:, P:], *pos)
+    want = with_rows(q, *cache.kv4_states[0].history(torch.float32), rows[:, 0], attn.scaling)
+    assert rel(out, want.flatten(2)) <= 2e-3
+    # the same rows from a CUDA graph, which cannot look at them
+    state, held = cache.kv4_states[0], P
+    def again():
+        state.lengths.fill_(held)
+        state.length = held
+        return attn(x[:, P:], pos, keep, past_key_values=cache)[0]
+    if kind == "bool":
+        again()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = again()
+        graph.replay()
+        assert torch.equal(got, out)

@@ -100,3 +100,25 @@ def test_decode_masks_of_every_kind():
     for m in (add, add[:, None, None]):
         assert torch.equal(A._decode_mask(m, 2, 4), add.float().expand(2, 4))
     assert A._decode_mask(None, 2, 4) is None
+
+
+def test_rows_that_differ_by_causality_only():
+    from starkv.kv4_attention import causal_rows
+    B, T, n = 2, 4, 9
+    pad = torch.ones(B, 1, 1, n, dtype=torch.bool)
+    pad[0, ..., :3] = False
+    keep = pad & torch.ones(T, n, dtype=torch.bool).tril(n - T)
+    wide = torch.cat([keep, torch.ones(B, 1, T, 2, dtype=torch.bool)], -1)     # columns past n do not count
+    for dtype in (torch.bool, torch.float16, torch.float32):
+        for m in (keep, wide):
+            add = m if dtype == torch.bool else torch.zeros(m.shape, dtype=dtype).masked_fill(~m, torch.finfo(dtype).min)
+            assert causal_rows(add, n)
+    inf = torch.zeros(keep.shape).masked_fill(~keep, float("-inf"))
+    assert causal_rows(inf, n)
+    for at in ((0, 0, 1, 5), (1, 0, 0, 8), (0, 0, 0, 0)):         # a dropped one, a newer one seen, padding seen
+        for m in (keep.clone(), inf.clone()):
+            m[at] = not keep[at] if m.dtype == torch.bool else (float("-inf") if keep[at] else 0.0)
+            assert not causal_rows(m, n)
+    bias = inf.clone()
+    bias[1, 0, 2, 4] = 0.5
+    assert not causal_rows(bias, n)
