@@ -63,20 +63,31 @@ class KV4State:
         self.lengths.add_(k.shape[1])
         self.length += k.shape[1]
 
+    def select(self, q: torch.Tensor, keep_pages: int, newest: Optional[int] = None) -> torch.Tensor:
+        """The pages (``KV4Cache.select``) of queries q (B, T, Hq, 128) among the ``newest``
+        tokens (T of them when None).  The first page and those that may hold the newest
+        tokens, whose own positions they are, always count; more than ``keep_pages`` where
+        those alone are more."""
+        newest = newest or q.shape[1]
+        last = 1 + -(-(newest - 1) // self.cache.page_size)
+        return self.cache.select(q, self.block_table, self.lengths, max(keep_pages, 1 + last), 1, last)
+
     def attend(self, q: torch.Tensor, scaling: float, mask: Optional[torch.Tensor] = None,
                keep_pages: int = 0) -> torch.Tensor:
         """The newest tokens' queries (B, T, Hq, 128) over the pages, or over the best
         ``keep_pages`` of them."""
-        pages = None
-        if keep_pages:
-            pages = self.cache.select(q, self.block_table, self.lengths, keep_pages)
+        pages = self.select(q, keep_pages) if keep_pages else None
         return self.cache.attend(q, self.block_table, self.lengths, scaling, mask=mask, pages=pages)
 
     def attend_rows(self, q: torch.Tensor, scaling: float, rows: torch.Tensor, keep_pages: int = 0) -> torch.Tensor:
         """``attend`` with a mask row for each token, rows (B, T, length): a call a token, in
         which its row says what it attends to, the newer tokens too."""
-        return torch.stack([self.attend(q[:, i:i + 1], scaling, rows[:, i], keep_pages)[:, 0]
-                            for i in range(q.shape[1])], 1)
+        out = []
+        for i in range(q.shape[1]):
+            qi = q[:, i:i + 1]
+            pages = self.select(qi, keep_pages, newest=q.shape[1]) if keep_pages else None
+            out.append(self.cache.attend(qi, self.block_table, self.lengths, scaling, mask=rows[:, i], pages=pages))
+        return torch.cat(out, 1)
 
     def history(self, dtype: torch.dtype):
         """All tokens held as (k, v), each (B, length, Hkv, 128)."""
@@ -84,7 +95,8 @@ class KV4State:
 
 
 class KV4Attention(nn.Module):
-    """``keep_pages``: pages a decode step attends to (0: all of them)."""
+    """``keep_pages``: pages a decode step attends to (0: all of them; from 2 on, the first and
+    the newest token's are always among them)."""
 
     def __init__(self, config, layer_idx: Optional[int] = None, page_size: int = 64, keep_pages: int = 0):
         super().__init__()
@@ -94,6 +106,8 @@ class KV4Attention(nn.Module):
         self.head_dim = config.hidden_size // config.num_attention_heads
         if self.head_dim != 128:
             raise ValueError("the 4-bit cache takes heads of dimension 128")
+        if keep_pages < 0 or keep_pages == 1:
+            raise ValueError("keep_pages must be 0, or 2 and more (the first page and the newest token's)")
         self.scaling = self.head_dim ** -0.5
         self.page_size, self.keep_pages = page_size, keep_pages
         bias = config.attention_bias

@@ -158,3 +158,60 @@ def test_draft_masks_whose_rows_differ(cuda, kind):
             got = again()
         graph.replay()
         assert torch.equal(got, out)
+
+
+def state_of(cuda, n, page=64, B=1, seed=15):
+    """A KV4State with n random tokens a sequence, 2 KV heads."""
+    from starkv.kv4_attention import KV4State
+    st = KV4State(B, n + 64, 2, page, cuda, page_bounds=True)
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    draw = lambda *s: torch.randn(*s, generator=g, device=cuda).half()  # noqa: E731
+    st.append(draw(B, n, 2, 128), draw(B, n, 2, 128))
+    return st, draw
+
+
+@pytest.mark.parametrize("page,T,over", [(64, 4, 1), (64, 16, 1), (64, 16, 15), (64, 16, 0), (16, 16, 1), (16, 5, 4), (32, 2, 1), (128, 1, 5)])
+def test_kept_pages_hold_the_drafts_themselves(cuda, page, T, over):
+    """T drafts whose newest `over` tokens are in the last page: every query's own position is
+    among the pages kept, whatever the others score and however few are asked for."""
+    n = page * 20 + over
+    st, draw = state_of(cuda, n, page)
+    for keep in (1, 2, 8):
+        q = draw(1, T, 8, 128)
+        pages = st.select(q, keep)
+        own = set(range((n - T) // page, (n - 1) // page + 1))
+        for h in range(2):
+            got = [p for p in pages[0, h].tolist() if p >= 0]
+            assert own <= set(got) and 0 in got and len(got) == len(set(got)) and len(got) >= keep
+        # rows that see everything up to themselves, one by one over the same pages
+        rows = torch.where(torch.ones(T, n, device=cuda).tril(n - T) > 0, 0.0, float("-inf"))[None]
+        a, b = st.attend(q, 128 ** -0.5, keep_pages=keep), st.attend_rows(q, 128 ** -0.5, rows, keep_pages=keep)
+        hide = torch.full((1, T, n), float("-inf"), device=cuda)
+        k, v = st.history(torch.float32)
+        for h in range(2):
+            kept = torch.isin(torch.arange(n, device=cuda) // page, pages[0, h])
+            want = with_rows(q[:, :, 4 * h:4 * h + 4], k[:, :, h:h + 1], v[:, :, h:h + 1], torch.where(kept, rows, hide), 128 ** -0.5)
+            assert rel(a[:, :, 4 * h:4 * h + 4], want) <= 2e-3
+        assert torch.isfinite(b).all()
+        if T == 1:
+            assert rel(b, a) <= 2e-3
+
+
+@torch.no_grad()
+def test_module_drafts_with_kept_pages(cuda):
+    """Fewest pages, drafts over the end of a page: the first page and the drafts' own."""
+    attn = small_model(cuda, (0, 1), kv4_keep_pages=2).model.layers[0].self_attn
+    attn.o_proj = torch.nn.Identity()
+    P, T = 64 * 6 - 3, 5
+    g = torch.Generator(device=cuda).manual_seed(16)
+    x = torch.randn(1, P + T, 512, generator=g, device=cuda).half() * 20
+    one = torch.ones(1, 1, 128, device=cuda, dtype=torch.float16)
+    cache = StarKVCache(512)
+    attn(x[:, :P], (one, one * 0), None, past_key_values=cache)
+    out, _ = attn(x[:, P:], (one, one * 0), None, past_key_values=cache)
+    n = P + T
+    at = torch.arange(n, device=cuda)
+    ok = (at[None] <= torch.arange(P, n, device=cuda)[:, None]) & ((at < 64) | (at >= 64 * 5))
+    q, _, _ = attn.heads(x[:, P:], one, one * 0)
+    want = with_rows(q, *cache.kv4_states[0].history(torch.float32), torch.where(ok, 0.0, float("-inf"))[None], attn.scaling)
+    assert rel(out, want.flatten(2)) <= 2e-3

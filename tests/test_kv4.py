@@ -122,3 +122,13 @@ def test_rows_that_differ_by_causality_only():
     bias = inf.clone()
     bias[1, 0, 2, 4] = 0.5
     assert not causal_rows(bias, n)
+
+
+def test_keep_pages_that_cannot_hold_the_first_and_the_newest():
+    from types import SimpleNamespace
+    from starkv.kv4_attention import KV4Attention
+    cfg = SimpleNamespace(hidden_size=256, num_attention_heads=2, num_key_value_heads=1, attention_bias=False)
+    for keep in (1, -1):
+        with pytest.raises(ValueError):
+            KV4Attention(cfg, keep_pages=keep)
+    assert [KV4Attention(cfg, keep_pages=k).keep_pages for k in (0, 2, 64)] == [0, 2, 64]
