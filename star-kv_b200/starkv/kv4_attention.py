@@ -63,20 +63,35 @@ class KV4State:
         self.lengths.add_(k.shape[1])
         self.length += k.shape[1]
 
-    def select(self, q: torch.Tensor, keep_pages: int, newest: Optional[int] = None) -> torch.Tensor:
+    def select(self, q: torch.Tensor, keep_pages: int, mask: Optional[torch.Tensor] = None,
+               newest: Optional[int] = None) -> torch.Tensor:
         """The pages (``KV4Cache.select``) of queries q (B, T, Hq, 128) among the ``newest``
         tokens (T of them when None).  The first page and those that may hold the newest
         tokens, whose own positions they are, always count; more than ``keep_pages`` where
-        those alone are more."""
+        those alone are more.
+
+        With an additive mask (B, L) a sequence begins at the first position that it does not
+        drop (-inf, or at most fp16's lowest number): pages of left padding are neither the
+        first page nor scored."""
         newest = newest or q.shape[1]
-        last = 1 + -(-(newest - 1) // self.cache.page_size)
-        return self.cache.select(q, self.block_table, self.lengths, max(keep_pages, 1 + last), 1, last)
+        page = self.cache.page_size
+        last = 1 + -(-(newest - 1) // page)
+        keep = max(keep_pages, 1 + last)
+        if mask is None:
+            return self.cache.select(q, self.block_table, self.lengths, keep, 1, last)
+        live = mask > torch.finfo(torch.float16).min
+        lead = torch.where(live.any(1), live.int().argmax(1), mask.shape[1])
+        skip = torch.minimum(lead, self.lengths - 1).clamp_(min=0) // page
+        at = (skip[:, None] + torch.arange(self.width, device=skip.device)).clamp_(max=self.width - 1)
+        skip = skip.int()
+        pages = self.cache.select(q, self.block_table.gather(1, at), self.lengths - skip * page, keep, 1, last)
+        return torch.where(pages >= 0, pages + skip[:, None, None], pages)
 
     def attend(self, q: torch.Tensor, scaling: float, mask: Optional[torch.Tensor] = None,
                keep_pages: int = 0) -> torch.Tensor:
         """The newest tokens' queries (B, T, Hq, 128) over the pages, or over the best
         ``keep_pages`` of them."""
-        pages = self.select(q, keep_pages) if keep_pages else None
+        pages = self.select(q, keep_pages, mask) if keep_pages else None
         return self.cache.attend(q, self.block_table, self.lengths, scaling, mask=mask, pages=pages)
 
     def attend_rows(self, q: torch.Tensor, scaling: float, rows: torch.Tensor, keep_pages: int = 0) -> torch.Tensor:
@@ -85,7 +100,7 @@ class KV4State:
         out = []
         for i in range(q.shape[1]):
             qi = q[:, i:i + 1]
-            pages = self.select(qi, keep_pages, newest=q.shape[1]) if keep_pages else None
+            pages = self.select(qi, keep_pages, rows[:, i], newest=q.shape[1]) if keep_pages else None
             out.append(self.cache.attend(qi, self.block_table, self.lengths, scaling, mask=rows[:, i], pages=pages))
         return torch.cat(out, 1)
 

@@ -215,3 +215,47 @@ def test_module_drafts_with_kept_pages(cuda):
     q, _, _ = attn.heads(x[:, P:], one, one * 0)
     want = with_rows(q, *cache.kv4_states[0].history(torch.float32), torch.where(ok, 0.0, float("-inf"))[None], attn.scaling)
     assert rel(out, want.flatten(2)) <= 2e-3
+
+
+@pytest.mark.parametrize("low", [float("-inf"), torch.finfo(torch.float16).min, torch.finfo(torch.float32).min])
+def test_kept_pages_leave_padding_out(cuda, low):
+    """A sequence behind whole pages of padding keeps the pages it keeps alone; padding that ends
+    inside a page, a sequence that is all padding, and a mask narrower than the sequence."""
+    from starkv.kv4_attention import KV4State
+    page, n, pads = 64, 64 * 16 + 9, (64 * 7, 0, 64 * 3 + 10, 64 * 16 + 9, 64 * 15)
+    st, draw = state_of(cuda, n, page, B=5)
+    q = draw(5, 2, 8, 128)
+    mask = torch.zeros(5, n, device=cuda)
+    for b, m in enumerate(pads):
+        mask[b, :m] = low
+    pages = st.select(q, 5, mask)
+    k, v = st.history(torch.float16)
+    out = st.attend(q, 128 ** -0.5, mask, keep_pages=5)
+    for b in (0, 1):
+        alone = KV4State(1, n + 64, 2, page, cuda, page_bounds=True)
+        alone.append(k[b:b + 1, pads[b]:], v[b:b + 1, pads[b]:])
+        # stored values quantise to other codes than the tokens did: the same pool is needed for the same bounds
+        alone.cache.data[:st.width - pads[b] // page].copy_(st.cache.data[b * st.width + pads[b] // page:(b + 1) * st.width])
+        alone.cache.bounds[:st.width - pads[b] // page].copy_(st.cache.bounds[b * st.width + pads[b] // page:(b + 1) * st.width])
+        alone.cache.bound_scales[:st.width - pads[b] // page].copy_(st.cache.bound_scales[b * st.width + pads[b] // page:(b + 1) * st.width])
+        assert torch.equal(alone.select(q[b:b + 1], 5) + pads[b] // page, pages[b:b + 1])
+        want = alone.attend(q[b:b + 1], 128 ** -0.5, keep_pages=5)
+        assert rel(out[b:b + 1], want) <= 2e-3
+    assert (pages[2, :, 0] == 3).all() and (pages[2].amin() >= 3) and (pages[2, :, -2:].cpu() == torch.tensor([15, 16])).all()
+    assert (pages[4].cpu() == torch.tensor([15, 16, -1, -1, -1])).all()
+    assert (pages[3, :, 0] == 16).all() and st.cache.read_error() == 0
+    if low == float("-inf"):
+        assert (out[3] == 0).all()
+    # positions past the mask count
+    assert torch.equal(st.select(q, 5, mask[:, :64 * 7]), st.select(q, 5, torch.cat([mask[:, :64 * 7], torch.zeros_like(mask[:, 64 * 7:])], 1)))
+
+
+@torch.no_grad()
+def test_padded_batch_with_kept_pages(cuda):
+    """Through transformers' code: a short sequence beside a long one keeps all its own pages,
+    as it does alone."""
+    seqs = sequences(cuda, (400, 160), 2)
+    got = run_padded(small_model(cuda, (0, 1), kv4_keep_pages=4), seqs, (1, 1), "2d")
+    alone = run_padded(small_model(cuda, (0, 1), kv4_keep_pages=4), seqs[1:], (1, 1), "2d")
+    for x, y in zip(got[1:], alone[1:]):
+        assert rel(x[1], y[0]) <= TOLERANCE
