@@ -134,7 +134,8 @@ class KV4Attention(nn.Module):
     def state(self, cache: StarKVCache, batch: int, device) -> KV4State:
         st = cache.kv4_states.get(self.layer_idx)
         if st is None:
-            st = KV4State(batch, cache.capacity, self.num_key_value_heads, self.page_size, device, self.keep_pages > 0)
+            # with bounds (2.5 % of the pool) whatever keep_pages is: it may be set later
+            st = KV4State(batch, cache.capacity, self.num_key_value_heads, self.page_size, device, True)
             cache.kv4_states[self.layer_idx] = st
         return st
 

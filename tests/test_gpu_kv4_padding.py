@@ -259,3 +259,19 @@ def test_padded_batch_with_kept_pages(cuda):
     alone = run_padded(small_model(cuda, (0, 1), kv4_keep_pages=4), seqs[1:], (1, 1), "2d")
     for x, y in zip(got[1:], alone[1:]):
         assert rel(x[1], y[0]) <= TOLERANCE
+
+
+@torch.no_grad()
+def test_keep_pages_set_after_the_prompt(cuda):
+    """keep_pages may change from step to step."""
+    outs = []
+    for late in (False, True):
+        attn = small_model(cuda, (0, 1), kv4_keep_pages=0 if late else 3).model.layers[0].self_attn
+        g = torch.Generator(device=cuda).manual_seed(17)
+        x = torch.randn(1, 401, 512, generator=g, device=cuda).half() * 20
+        one = torch.ones(1, 1, 128, device=cuda, dtype=torch.float16)
+        cache = StarKVCache(512)
+        attn(x[:, :400], (one, one * 0), None, past_key_values=cache)
+        attn.keep_pages = 3
+        outs.append(attn(x[:, 400:], (one, one * 0), None, past_key_values=cache)[0])
+    assert torch.equal(*outs)
