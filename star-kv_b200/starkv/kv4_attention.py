@@ -3,8 +3,9 @@
 ``KV4Attention`` stands beside the latent modules (``starkv.attention``) in one model
 and one ``StarKVCache``: layers whose learned ranks stay near the head dimension keep
 their dense ``k_proj`` / ``v_proj`` and hold their heads in 4 bits here, the others
-hold latents.  Same constructor and forward arguments as the latent modules, so
-the decoder layer's code does not change.
+hold latents.  The latent modules' constructor arguments (its own by keyword) and
+attributes, and either's forward arguments by keyword, so the decoder layer's code does
+not change.
 
 * prompt: keys (rotated) and values are written into pages; the attention runs over
   the exact heads with the prompt kernel (``starkv.prefill``);
@@ -113,12 +114,19 @@ class KV4Attention(nn.Module):
     """``keep_pages``: pages a decode step attends to (0: all of them; from 2 on, the first and
     the newest token's are always among them)."""
 
-    def __init__(self, config, layer_idx: Optional[int] = None, page_size: int = 64, keep_pages: int = 0):
+    def __init__(self, config, layer_idx: Optional[int] = None, decomp_goup_num: Optional[int] = 1, *,
+                 page_size: int = 64, keep_pages: int = 0):
         super().__init__()
+        self.config = config
         self.layer_idx = layer_idx
+        self.attention_dropout = getattr(config, "attention_dropout", 0.0)
+        self.hidden_size = config.hidden_size
         self.num_heads = config.num_attention_heads
         self.num_key_value_heads = config.num_key_value_heads
+        self.num_key_value_groups = self.num_heads // self.num_key_value_heads
         self.head_dim = config.hidden_size // config.num_attention_heads
+        self.is_causal = True
+        self.decomp_goup_num = decomp_goup_num           # nothing is factored here
         if self.head_dim != 128:
             raise ValueError("the 4-bit cache takes heads of dimension 128")
         if keep_pages < 0 or keep_pages == 1:
@@ -176,7 +184,7 @@ class KV4Attention(nn.Module):
             out = prefill.prompt_attention(q.transpose(1, 2), keys.transpose(1, 2), values.transpose(1, 2), self.scaling)
             out = out.transpose(1, 2)
         else:
-            grp = self.num_heads // self.num_key_value_heads
+            grp = self.num_key_value_groups
             n = keys.shape[1]
             if attention_mask is None:
                 mask = torch.ones(T, n, dtype=torch.bool, device=q.device).tril(n - T)

@@ -132,3 +132,19 @@ def test_keep_pages_that_cannot_hold_the_first_and_the_newest():
         with pytest.raises(ValueError):
             KV4Attention(cfg, keep_pages=keep)
     assert [KV4Attention(cfg, keep_pages=k).keep_pages for k in (0, 2, 64)] == [0, 2, 64]
+
+
+def test_module_is_built_like_the_latent_ones():
+    """The positional arguments mean the same in both, and the attributes that model code reads are there."""
+    from transformers import LlamaConfig
+    from starkv.attention import LlamaCustomAttention
+    from starkv.kv4_attention import KV4Attention
+    cfg = LlamaConfig(hidden_size=512, num_attention_heads=4, num_key_value_heads=2, attention_bias=False)
+    a, b = LlamaCustomAttention(cfg, 3, 32), KV4Attention(cfg, 3, 32, keep_pages=2)
+    for name in ("config", "layer_idx", "attention_dropout", "hidden_size", "num_heads", "num_key_value_heads",
+                 "num_key_value_groups", "head_dim", "is_causal", "scaling", "decomp_goup_num"):
+        assert getattr(a, name) == getattr(b, name), name
+    assert b.page_size == 64 and b.keep_pages == 2
+    assert KV4Attention(cfg, 3, page_size=32).page_size == 32
+    with pytest.raises(TypeError):
+        KV4Attention(cfg, 3, 1, 32)
