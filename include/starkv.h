@@ -323,7 +323,7 @@ int starkv_prefill_attention(const starkv_prefill_args* args, starkv_stream_t st
  */
 typedef struct starkv_kv4_cache {
   void* data;               /* 16-byte aligned */
-  void* bounds;
+  void* bounds;             /* 16-byte aligned */
   float* bound_scales;
   int32_t* error_word;      /* device int, set to a code when a kernel meets a bad page or position */
   int32_t num_pages;
@@ -381,8 +381,8 @@ typedef struct starkv_kv4_attention_args {
   int64_t mask_stride;
   int64_t mask_width;
   const int32_t* pages;       /* (B, Hkv, num_selected) page ordinals of the sequence, each once, -1 = none, or NULL */
-  void* workspace;            /* starkv_kv4_workspace_size bytes, the first 1024 zeroed before its first use (each call
-                                 leaves them zero).  One call at a time may use it. */
+  void* workspace;            /* starkv_kv4_workspace_size bytes, 16-byte aligned, the first 1024 zeroed before its first
+                                 use (each call leaves them zero).  One call at a time may use it. */
   size_t workspace_bytes;
   float scaling;
   int32_t num_selected;
@@ -417,8 +417,8 @@ typedef struct starkv_kv4_select_args {
   int64_t table_stride;
   const int32_t* lengths;
   int32_t* pages_out;
-  void* workspace;            /* starkv_kv4_select_workspace_size bytes, the first 256 KiB zeroed before its first use (each
-                                 call leaves them zero).  One call at a time may use it. */
+  void* workspace;            /* starkv_kv4_select_workspace_size bytes, 4-byte aligned, the first 256 KiB zeroed before its
+                                 first use (each call leaves them zero).  One call at a time may use it. */
   size_t workspace_bytes;
   int32_t q_dtype;
   int32_t batch;

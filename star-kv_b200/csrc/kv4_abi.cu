@@ -14,6 +14,12 @@ using namespace starkv;
 
 namespace {
 
+// Whether every address is a multiple of `bytes` (null is).
+template <typename... P>
+bool aligned(size_t bytes, P... ptrs) {
+  return ((reinterpret_cast<uintptr_t>(ptrs) | ...) & (bytes - 1)) == 0;
+}
+
 int check_pool(const starkv_kv4_cache* c, Kv4Pool* pool) {
   if (!c || !c->data) return host_error(STARKV_ERR_INVALID, "null cache");
   if (c->head_dim != 128) return host_error(STARKV_ERR_UNSUPPORTED, "kv4 caches take head_dim 128");
@@ -21,7 +27,8 @@ int check_pool(const starkv_kv4_cache* c, Kv4Pool* pool) {
     return host_error(STARKV_ERR_UNSUPPORTED, "kv4 page_size must be 16, 32, 64 or 128");
   if (c->num_pages <= 0 || c->num_kv_heads <= 0 || c->num_kv_heads > 65535)
     return host_error(STARKV_ERR_INVALID, "kv4 cache needs pages and KV heads (at most 65535)");
-  if (reinterpret_cast<uintptr_t>(c->data) % 16) return host_error(STARKV_ERR_INVALID, "kv4 data must be 16-byte aligned");
+  if (!aligned(16, c->data, c->bounds) || !aligned(4, c->bound_scales, c->error_word))
+    return host_error(STARKV_ERR_INVALID, "kv4 data and bounds must be 16-byte aligned, scales and error word 4-byte");
   if ((c->bounds == nullptr) != (c->bound_scales == nullptr))
     return host_error(STARKV_ERR_INVALID, "kv4 bounds and bound_scales go together");
   pool->data = (uint8_t*)c->data;
@@ -57,6 +64,7 @@ int io_params(const starkv_kv4_cache* cache, const starkv_kv4_io_args* a, Kv4IoP
     return host_error(STARKV_ERR_INVALID, "bad batch (at most 65535), token count or block table");
   if (a->batch == 0 || a->num_tokens == 0) return STARKV_OK;
   if (!a->block_table || !a->start) return host_error(STARKV_ERR_INVALID, "null argument");
+  if (!aligned(4, a->block_table, a->start, a->count)) return host_error(STARKV_ERR_INVALID, "int32 arguments must be 4-byte aligned");
   if ((rc = check_rows(a->k, a->k_strides, eb, "k rows must be 16-byte aligned")) ||
       (rc = check_rows(a->v, a->v_strides, eb, "v rows must be 16-byte aligned")))
     return rc;
@@ -170,6 +178,9 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   size_t need = 0;
   starkv_kv4_workspace_size(&need);
   if (a->workspace_bytes < need) return host_error(STARKV_ERR_WORKSPACE, "kv4 attention workspace too small");
+  if (!aligned(16, a->workspace)) return host_error(STARKV_ERR_WORKSPACE, "kv4 attention workspace must be 16-byte aligned");
+  if (!aligned(4, a->block_table, a->lengths, a->pages, a->mask, a->lse))
+    return host_error(STARKV_ERR_INVALID, "int32 and fp32 arguments must be 4-byte aligned");
   if ((rc = check_rows(a->q, a->q_strides, 2, "q rows must be 16-byte aligned")) ||
       (rc = check_rows(a->out, a->out_strides, ob, "out rows must be 16-byte aligned")))
     return rc;
@@ -248,9 +259,10 @@ int starkv_kv4_select(const starkv_kv4_cache* cache, const starkv_kv4_select_arg
   size_t need = 0;
   starkv_kv4_select_workspace_size(cache, a->batch, a->table_width, &need);
   if (a->workspace_bytes < need) return host_error(STARKV_ERR_WORKSPACE, "kv4 selection workspace too small");
+  if (!aligned(4, a->workspace)) return host_error(STARKV_ERR_WORKSPACE, "kv4 selection workspace must be 4-byte aligned");
+  if (!aligned(4, a->block_table, a->lengths, a->pages_out))
+    return host_error(STARKV_ERR_INVALID, "int32 arguments must be 4-byte aligned");
   if ((rc = check_rows(a->q, a->q_strides, 2, "q rows must be 16-byte aligned"))) return rc;
-  if (reinterpret_cast<uintptr_t>(p.pool.bounds) % 16)
-    return host_error(STARKV_ERR_INVALID, "kv4 bounds must be 16-byte aligned");
   p.q = a->q;
   memcpy(p.qs, a->q_strides, sizeof(p.qs));
   p.table = a->block_table;

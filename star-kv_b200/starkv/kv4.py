@@ -250,7 +250,8 @@ class KV4Cache:
         num_kv_heads, n) page ordinals to attend within (``select``).  Returns out of
         q's shape and dtype (or in ``out``), and with ``return_lse`` the fp32 log-sum-exp
         (q's shape without the channels); a query with nothing to attend to gets 0 and
-        -inf."""
+        -inf.  ws: scratch of one's own, ``starkv_kv4_workspace_size`` bytes on a 16-byte
+        boundary, its first 1024 zeroed before its first use (each call leaves them zero)."""
         B, W, tp, ts = self._table(block_table)
         q4, qs = self._queries(q, B)
         Q, Hq = q4.shape[1], q4.shape[2]

@@ -519,3 +519,33 @@ def test_empty_calls(cuda):
     assert cache.attend(torch.zeros(0, 1, 2, 128, dtype=F16, device=cuda), none, z, 1.0).shape == (0, 1, 2, 128)
     assert cache.select(torch.zeros(0, 2, 128, dtype=F16, device=cuda), none, z, 2).shape == (0, 1, 2)
     assert cache.read_error() == 0
+
+
+def test_unaligned_workspaces_are_refused(cuda):
+    """The kernels read and write 16 bytes at a time in the attention's workspace, 4 in the selection's."""
+    import ctypes as C
+    from starkv import _lib, kv4
+    lib = _lib.load()
+    cache = KV4Cache(4, 2, page_size=32, device=cuda)
+    table, lengths = table_of(2, 2, cuda), ints([40, 3], cuda)
+    q = torch.zeros(2, 1, 4, 128, dtype=F16, device=cuda)
+    need = kv4._attention_size()
+    room = torch.zeros(need + 64, dtype=torch.uint8, device=cuda)
+    base = -room.data_ptr() % 16
+    for off in (1, 2, 4, 8, 15):
+        with pytest.raises(StarKVError):
+            cache.attend(q, table, lengths, SCALING, ws=room[base + off:])
+    got = cache.attend(q, table, lengths, SCALING, ws=room[base + 16:])
+    assert torch.equal(got, cache.attend(q, table, lengths, SCALING))
+    n = C.c_size_t(0)
+    assert lib.starkv_kv4_select_workspace_size(cache._block, 2, 2, C.byref(n)) == 0
+    room = torch.zeros(n.value + 64, dtype=torch.uint8, device=cuda)
+    out = torch.empty(2, 2, 2, dtype=torch.int32, device=cuda)
+    for off, status in ((1, 4), (2, 4), (3, 4), (4, 0)):
+        a = _lib.KV4SelectArgs(q=q.data_ptr(), q_strides=q.stride()[:3], block_table=table.data_ptr(), table_stride=2,
+                               lengths=lengths.data_ptr(), pages_out=out.data_ptr(), workspace=room.data_ptr() + off,
+                               workspace_bytes=n.value, q_dtype=1, batch=2, num_queries=1, num_q_heads=4, table_width=2,
+                               num_selected=2, num_first=1, num_last=1)
+        assert lib.starkv_kv4_select(cache._block, C.byref(a), None) == status
+    torch.cuda.synchronize()
+    assert out.cpu()[0, 0].tolist() == [0, 1]

@@ -148,3 +148,16 @@ def test_module_is_built_like_the_latent_ones():
     assert KV4Attention(cfg, 3, page_size=32).page_size == 32
     with pytest.raises(TypeError):
         KV4Attention(cfg, 3, 1, 32)
+
+
+@pytest.mark.parametrize("field,value", [("bounds", 264), ("bounds", 257), ("bound_scales", 258), ("error_word", 257)])
+def test_pool_alignment(field, value):
+    """The kernels store words of 16 and 4 bytes there."""
+    c = _lib.KV4Cache(data=256, bounds=256, bound_scales=256, error_word=256, num_pages=4, num_kv_heads=2,
+                      page_size=64, head_dim=128)
+    setattr(c, field, value)
+    lib = _lib.load()
+    for fn, a in ((lib.starkv_kv4_write, _lib.KV4IoArgs()), (lib.starkv_kv4_read, _lib.KV4IoArgs()),
+                  (lib.starkv_kv4_attention, _lib.KV4AttentionArgs()), (lib.starkv_kv4_select, _lib.KV4SelectArgs())):
+        assert fn(C.byref(c), C.byref(a), None) == 1
+        assert b"aligned" in lib.starkv_last_error()
