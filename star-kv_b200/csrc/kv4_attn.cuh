@@ -176,6 +176,13 @@ __device__ __forceinline__ void kv4_cp_async4(void* dst, const float* mask, int 
                : "memory");
 }
 
+// An additive mask's value for the log2 domain.  Beyond -2.3e38 the product would leave fp32; -inf
+// and NaN stay what they are.
+__device__ __forceinline__ float kv4_mask_log2(float a) {
+  const float low = a == -INFINITY ? a : -2.3e38f * 1.4426950408889634f;
+  return a < -2.3e38f ? low : a * 1.4426950408889634f;
+}
+
 // The largest of a warp's values, by its order-preserving integers.
 __device__ __forceinline__ float kv4_warp_max(float x) {
   const int u = __float_as_int(x), k = __reduce_max_sync(0xffffffffu, u ^ ((u >> 31) & 0x7fffffff));
@@ -404,9 +411,8 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
   if (MASK) {
     add0 = __uint_as_float(kv4_lds32(mk + at.row));
     add1 = __uint_as_float(kv4_lds32(mk + at.row + 32));
-    // beyond -2.3e38 the sum would leave fp32 in the log2 domain
-    add0 = add0 == -INFINITY ? add0 : fmaxf(add0, -2.3e38f) * 1.4426950408889634f;
-    add1 = add1 == -INFINITY ? add1 : fmaxf(add1, -2.3e38f) * 1.4426950408889634f;
+    add0 = kv4_mask_log2(add0);
+    add1 = kv4_mask_log2(add1);
   }
   bool over = false;
 #pragma unroll

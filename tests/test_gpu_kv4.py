@@ -549,3 +549,25 @@ def test_unaligned_workspaces_are_refused(cuda):
         assert lib.starkv_kv4_select(cache._block, C.byref(a), None) == status
     torch.cuda.synchronize()
     assert out.cpu()[0, 0].tolist() == [0, 1]
+
+
+@pytest.mark.parametrize("Q,G", [(1, 1), (1, 4), (3, 8)])
+def test_nan_in_a_mask(cuda, Q, G):
+    """A NaN in a mask is added like any number: the queries that may attend there are NaN, and only they."""
+    lens = [300, 300, 70]
+    made = Made(cuda, lens, 2, 64, F16, seed=23, garbage=False)
+    q = rnd((3, Q, 2 * G, 128), F16, 24, cuda)
+    clean = torch.zeros(3, 300, device=cuda)
+    clean[1, 290:] = float("-inf")
+    mask = clean.clone()
+    mask[0, 17] = mask[1, 280] = float("nan")
+    mask[2, 70:] = float("nan")                               # past the length
+    want, wlse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=clean, return_lse=True)
+    out, lse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask, return_lse=True)
+    assert torch.isnan(out[:2]).all() and torch.isnan(lse[:2]).all()
+    assert torch.equal(out[2], want[2]) and torch.equal(lse[2], wlse[2])
+    if Q > 1:                                                 # where only the newest query attends
+        mask = clean.clone()
+        mask[0, 299] = float("nan")
+        out, lse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask, return_lse=True)
+        assert torch.isnan(out[0, -1]).all() and torch.equal(out[0, :-1], want[0, :-1]) and torch.equal(lse[0, :-1], wlse[0, :-1])
