@@ -143,6 +143,20 @@ __device__ __forceinline__ int kv4_tiles(const Kv4AttnParams& p, int64_t len) {
   return (p.pages ? p.num_selected * p.pool.page_tiles : (int)((len + kKv4Tile - 1) >> 4)) + kKv4PadTiles;
 }
 
+// An additive mask's value for the log2 domain: times log2 e.  Beyond 1e38 in magnitude, where the
+// product would soon leave fp32, the slope is 3/4: numbers stay apart and in order (so far out any
+// two weigh as 0 and 1), the type's lowest becomes -3.24e38, infinities and NaN stay.  kv4_lse is the way back.
+constexpr float kKv4MaskKnee = 1e38f, kKv4Log2e = 1.4426950408889634f;
+__device__ __forceinline__ float kv4_mask_log2(float a) {
+  const float t = fminf(fmaxf(a, -kKv4MaskKnee), kKv4MaskKnee);
+  return fmaf(a - t, 0.75f, t * kKv4Log2e);
+}
+__device__ __forceinline__ float kv4_lse(float x) {
+  const float t = fminf(fmaxf(x, -kKv4MaskKnee * kKv4Log2e), kKv4MaskKnee * kKv4Log2e);
+  const float y = fmaf(x - t, 1.f / 0.75f, t * 0.69314718055994531f);
+  return fabsf(y) == INFINITY && fabsf(x) != INFINITY ? copysignf(3.402823466e38f, y) : y;   // a rounding past the end
+}
+
 // Writes one column of a segment, a lane 4 channels: o over the rounded weights' sum, log(l) above the base.
 __device__ __forceinline__ void kv4_store_column(const Kv4AttnParams& p, int b, int hc, int col, int cols, float4 o, float base,
                                               float l, float rounded) {
@@ -161,7 +175,7 @@ __device__ __forceinline__ void kv4_store_column(const Kv4AttnParams& p, int b, 
   }
   if (p.lse && lane == 0)
     p.lse[((int64_t)b * p.queries + qi) * p.q_heads + qh] =
-        l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718055994531f;
+        l == 0.f ? -INFINITY : kv4_lse(base + log2f(l));
 }
 
 // Weight of a piece against the joint base.
@@ -174,13 +188,6 @@ __device__ __forceinline__ void kv4_cp_async4(void* dst, const float* mask, int 
   const int bytes = i < width ? 4 : 0;
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(mask + (bytes ? i : 0)), "r"(bytes)
                : "memory");
-}
-
-// An additive mask's value for the log2 domain.  Beyond -2.3e38 the product would leave fp32; -inf
-// and NaN stay what they are.
-__device__ __forceinline__ float kv4_mask_log2(float a) {
-  const float low = a == -INFINITY ? a : -2.3e38f * 1.4426950408889634f;
-  return a < -2.3e38f ? low : a * 1.4426950408889634f;
 }
 
 // The largest of a warp's values, by its order-preserving integers.

@@ -571,3 +571,30 @@ def test_nan_in_a_mask(cuda, Q, G):
         mask[0, 299] = float("nan")
         out, lse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask, return_lse=True)
         assert torch.isnan(out[0, -1]).all() and torch.equal(out[0, :-1], want[0, :-1]) and torch.equal(lse[0, :-1], wlse[0, :-1])
+
+
+@pytest.mark.parametrize("Q,G", [(1, 1), (1, 4), (3, 8)])
+def test_masks_of_the_largest_magnitudes(cuda, Q, G):
+    """Numbers near the ends of fp32 are kept apart: positions at -3e38 weigh nothing beside one at
+    -2.5e38, which weighs nothing beside 0, and the log-sum-exp is the largest of them."""
+    low = torch.finfo(F32).min
+    made = Made(cuda, [300] * 7, 2, 64, F16, seed=25)
+    q = rnd((7, Q, 2 * G, 128), F16, 26, cuda)
+    mask = torch.full((7, 300), low, device=cuda)
+    mask[1, 40] = -3e38
+    mask[2, 40] = -2.5e38
+    mask[2, 41:] = -3.3e38
+    mask[3, :], mask[3, 40] = torch.finfo(BF16).min, -1e38
+    mask[4, :], mask[4, 40] = -1e38, 2.5e38
+    mask[5, :], mask[5, 40], mask[5, 41] = 0, 1e38, 3e38
+    mask[6, 40] = -9e37
+    out = torch.empty(q.shape, device=cuda)
+    _, lse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask, out=out, return_lse=True)
+    want = [low, -3e38, -2.5e38, -1e38, 2.5e38, 3e38, -9e37]
+    assert np.abs(f64(lse) / np.array(want)[:, None, None] - 1).max() <= 2.0 ** -20
+    for b in range(1, 7):                                     # one position takes all: its value, rounded twice at most
+        for h in range(2):
+            v = O.values(f64(made.v[b, 41 if b == 5 else 40, h]))
+            _, s, m = O.quantise(f64(made.v[b, 41 if b == 5 else 40, h]))
+            tol = 2 * U * (8 * s + np.abs(m)).repeat(32)
+            assert (np.abs(f64(out[b, :, h * G:(h + 1) * G]) - v) <= tol).all(), b
