@@ -313,12 +313,16 @@ __device__ __forceinline__ void kv4_prepare(const Kv4AttnParams& p, uint4* buf, 
   big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
   const float a = f16 ? kv4_halves(big).x : __uint_as_float(big << 16);
   // q scaled by a power of two to [512, 1024) in magnitude, the scaling's sign with it; a column
-  // whose scores vanish (q or scaling below 2^-100) becomes zero
+  // whose scores vanish (q below 2^-117, or q times scaling below 2^-110: `up` or `scale` would leave
+  // fp32) becomes zero; one with a NaN for a scaling becomes NaN
   float up = 0.f, scale = 1.f;
-  if (!(a < 0x1p-100f) && fabsf(p.scaling) >= 0x1p-100f) {
+  const float size = fabsf(p.scaling);
+  if (size != size) {
+    up = size;
+  } else if (!(a < 0x1p-117f) && !(a * size < 0x1p-110f)) {
     const int ex = (__float_as_int(a) >> 23) - 127;
     up = __int_as_float((127 + 9 - ex) << 23);
-    scale = fabsf(p.scaling) * 1.4426950408889634f * __int_as_float((127 - 9 + 3 + ex) << 23);
+    scale = size * kKv4Log2e * __int_as_float((127 - 9 + 3 + ex) << 23);
     if (p.scaling < 0.f) up = -up;
   }
   float sum[4];

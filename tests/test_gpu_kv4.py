@@ -598,3 +598,34 @@ def test_masks_of_the_largest_magnitudes(cuda, Q, G):
             _, s, m = O.quantise(f64(made.v[b, 41 if b == 5 else 40, h]))
             tol = 2 * U * (8 * s + np.abs(m)).repeat(32)
             assert (np.abs(f64(out[b, :, h * G:(h + 1) * G]) - v) <= tol).all(), b
+
+
+@pytest.mark.parametrize("scaling,size", [(1e-25, 1e-20), (-1e-30, 1e-12), (1e-38, 1.0), (0.0, 1.0), (1e-35, 1e30), (1e20, 1e-25)])
+def test_scalings_of_any_size(cuda, scaling, size):
+    """Products of queries and scaling below fp32's range leave the mean of the values, the others their softmax."""
+    lens, Q, G = [77, 5, 0, 333], 2, 4
+    made = Made(cuda, lens, 1, 64, BF16, seed=27)
+    q = (rnd((4, Q, G, 128), BF16, 28, cuda).float() * size).to(BF16)
+    mask = torch.zeros(4, 333, device=cuda)
+    mask[3, :100] = float("-inf")
+    for m in (None, mask):
+        out = torch.empty(q.shape, device=cuda)
+        _, lse = made.cache.attend(q, made.table, made.lengths, scaling, mask=m, out=out, return_lse=True)
+        for b, n in enumerate(lens):
+            k, v = made.stored(b, 0)
+            ref, rlse, w = O.attend(f64(q[b]), k, v, float(np.float32(scaling)), None, None if m is None else f64(m[b]))
+            empty = np.isneginf(rlse)
+            assert (f64(out[b])[empty] == 0).all() and np.isneginf(f64(lse[b])[empty]).all()
+            if n:                                             # scores are below 0.1: 2^-15 of that does not show
+                _, s, mm = O.quantise(f64(made.v[b, :n, 0]))
+                big = (8 * s + np.abs(mm)).max()
+                assert np.abs(f64(out[b]) - ref).max() <= (2 * U + 2.0 ** -15) * big
+                assert np.abs(f64(lse[b])[~empty] - rlse[~empty]).max() <= 2.0 ** -15
+
+
+def test_nan_scaling(cuda):
+    made = Made(cuda, [77, 1, 0], 1, 64, F16, seed=29)
+    q = rnd((3, 2, 4, 128), F16, 30, cuda)
+    out, lse = made.cache.attend(q, made.table, made.lengths, float("nan"), return_lse=True)
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all() and torch.isnan(out[1, 1]).all()
+    assert (out[1, 0] == 0).all() and (out[2] == 0).all() and torch.isneginf(lse[2]).all()
