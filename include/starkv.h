@@ -365,8 +365,9 @@ int starkv_kv4_read(const starkv_kv4_cache* cache, const starkv_kv4_io_args* arg
  * query i of sequence b sits at position lengths[b] - num_queries + i and attends
  * to positions [0, that], within the pages of `pages` when given.  x = scaling *
  * q.k + mask; out = softmax(x) V; lse = log(sum exp(x)).  A query that attends to
- * nothing (no length, mask -inf everywhere) gets out = 0, lse = -inf; what the
- * cache holds at positions past the length or masked by -inf does not matter.
+ * nothing (no length, mask -inf everywhere) gets out = 0, lse = -inf.  What the
+ * cache holds at positions that a query does not attend to (past the length, newer
+ * than the query, masked by -inf) does not matter to it, NaN included.
  */
 typedef struct starkv_kv4_attention_args {
   const void* q;              /* (B, num_queries, Hq, 128), fp16 / bf16 */

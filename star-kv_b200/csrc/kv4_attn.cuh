@@ -126,6 +126,12 @@ __device__ __forceinline__ uint32_t kv4_hmul2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 0xffff for each of a word's two fp16 numbers that is a NaN.
+__device__ __forceinline__ uint32_t kv4_nans(uint32_t a) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&a);
+  return __hneu2_mask(h, h);
+}
+
 // Tokens of a sequence, within the block table.
 __device__ __forceinline__ int64_t kv4_length(const Kv4AttnParams& p, int b) {
   const int64_t cap = (int64_t)p.width << p.pool.page_shift;
@@ -504,6 +510,26 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
   // ---- weights and values
   if (NT == 1) load_values();
   if (MASK || EDGE) ma.x &= la, ma.y &= la, mb.x &= lb, mb.y &= lb;
+  if (EDGE) {
+    // A group that holds a NaN has one for m.  Here not every column attends to its token, and 0 times
+    // it must not reach those that do not: the centres go on without it, and one more product says
+    // which columns' sums it belongs to.
+    const uint32_t na = kv4_nans(ma.x), nb = kv4_nans(ma.y), nc = kv4_nans(mb.x), nd = kv4_nans(mb.y);
+    if (__any_sync(0xffffffffu, na | nb | nc | nd)) {
+      ma.x &= ~na, ma.y &= ~nb, mb.x &= ~nc, mb.y &= ~nd;
+      const uint32_t one = lane >> 2 == 2 ? 0u : 0x3c003c00u;   // row 2 is the weights' sum
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        auto seen = [&](int u) { return x[nt][u] == -INFINITY ? 0.f : 1.f; };
+        float d[4];
+        kv4_mma0(d, na & one, nb & 0x3c003c00u, nc & one, nd & 0x3c003c00u, kv4_transpose(kv4_half2(seen(0), seen(1))),
+                 kv4_transpose(kv4_half2(seen(2), seen(3))));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (d[u] > 0.f) s.z[nt][u] = __int_as_float(0x7fffffff);
+      }
+    }
+  }
   if (lane >> 2 == 2) ma.x = mb.x = 0x3c003c00u;   // row 2: ones
   uint32_t p0[NT], p1[NT];
 #pragma unroll

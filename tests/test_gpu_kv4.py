@@ -629,3 +629,33 @@ def test_nan_scaling(cuda):
     out, lse = made.cache.attend(q, made.table, made.lengths, float("nan"), return_lse=True)
     assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all() and torch.isnan(out[1, 1]).all()
     assert (out[1, 0] == 0).all() and (out[2] == 0).all() and torch.isneginf(lse[2]).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Hkv,G,Q,n", [(1, 4, 2, 77), (2, 1, 4, 33), (1, 4, 4, 16), (1, 3, 5, 130), (2, 8, 6, 64), (1, 2, 3, 3)])
+def test_nan_in_newer_tokens_does_not_reach_older_queries(cuda, dtype, Hkv, G, Q, n):
+    """A NaN key or value of a newer draft is the newer queries' alone, and a value's only in its 32 channels."""
+    made = Made(cuda, [n, n], Hkv, 16, F32, seed=33, garbage=False)
+    made.k, made.v = made.k.clamp(-3, 3), made.v.clamp(-3, 3)         # scales below 1: no other exponent without one
+    made.cache.write(made.k, made.v, made.table, ints([0, 0], cuda))
+    q = rnd((2, Q, Hkv * G, 128), dtype, 34, cuda)
+    mask = torch.zeros(2, n, device=cuda)
+    for m in (None, mask):
+        want, wlse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=m, return_lse=True)
+        for i in range(1, Q):                                         # position of query i
+            k, v = made.k.clone(), made.v.clone()
+            v[0, n - Q + i, :, 70] = float("nan")
+            k[1, n - Q + i, :, 5] = float("nan")
+            made.cache.write(k, v, made.table, ints([0, 0], cuda))
+            out, lse = made.cache.attend(q, made.table, made.lengths, SCALING, mask=m, return_lse=True)
+            assert torch.equal(out[:, :i], want[:, :i]) and torch.equal(lse[:, :i], wlse[:, :i])
+            bad = torch.isnan(out[0, i:])
+            assert bad[..., 64:96].all() and not bad[..., :64].any() and not bad[..., 96:].any()
+            assert torch.equal(lse[0], wlse[0]) and torch.isnan(lse[1, i:]).all() and torch.isnan(out[1, i:]).all()
+        made.cache.write(made.k, made.v, made.table, ints([0, 0], cuda))
+    mask[:, n - 1] = float("-inf")                                    # masked for all: nobody's
+    want = made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask)
+    v = made.v.clone()
+    v[:, n - 1] = float("nan")
+    made.cache.write(made.k, v, made.table, ints([0, 0], cuda))
+    assert torch.equal(want, made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask))
