@@ -246,10 +246,11 @@ int starkv_quantize_split(const void* x, int32_t dtype, int64_t rows, int32_t r,
 /*
  * Test hooks for the device-side failure path (no counterpart in the
  * reference): wait_limit_ns (> 0; 0 restores the default 2 s) bounds every
- * mbarrier wait of the K kernel; skip_copy_unit >= 0 makes the K kernel's
- * first CTA (split 0, head group 0, sequence 0) never issue that unit's staging
- * copy, so that its consumers' waits
- * run out, record an error code in the workspace's first word and return.
+ * mbarrier wait of the K kernel and of the 4-bit attention; skip_copy_unit >= 0
+ * makes the K kernel's first CTA (split 0, head group 0, sequence 0) never issue
+ * that unit's staging copy, and the 4-bit attention's first warp that of its tile
+ * of that number, so that the waits for it run out, record an error code (in the
+ * workspace's first word, in the cache's error word) and return.
  * (0, -1) restores normal operation.  Not for production use.
  */
 int starkv_set_test_hooks(int64_t wait_limit_ns, int32_t skip_copy_unit);

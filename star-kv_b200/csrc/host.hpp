@@ -11,5 +11,8 @@ int host_error(int code, const char* msg);
 int host_launch_status();
 // STARKV_OK when the current device is an sm_100 GPU; *sms gets its SM count.
 int host_device(int* sms);
+// Time limit of one device-side wait, and the copy that a test withholds (-1: none).
+unsigned long long host_wait_limit();
+int host_skip_unit();
 
 }  // namespace starkv

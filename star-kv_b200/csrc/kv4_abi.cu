@@ -217,6 +217,8 @@ int starkv_kv4_attention(const starkv_kv4_cache* cache, const starkv_kv4_attenti
   const int64_t tiles = (a->pages ? (int64_t)a->num_selected : (int64_t)a->table_width) * p.pool.page_tiles + kKv4PadTiles;
   if ((double)tiles * p.pool.heads * p.col_blocks * a->batch > 2.0e9)
     return host_error(STARKV_ERR_UNSUPPORTED, "batch * KV heads * tiles of a block table row must stay below 2e9");
+  p.wait_ns = host_wait_limit();
+  p.skip_copy = host_skip_unit();
   p.group_m = kv4_reciprocal(p.group);
   p.col_blocks_m = kv4_reciprocal(p.col_blocks);
   int sms = 0;

@@ -85,6 +85,8 @@ struct Kv4AttnParams {
   float scaling;
   int num_selected, q_dtype, out_dtype, batch, queries, q_heads, group, width, col_blocks;
   uint64_t group_m, col_blocks_m;           // kv4_reciprocal of the two
+  unsigned long long wait_ns;               // limit of one wait
+  int skip_copy;                            // tests: tile of the first warp whose copy is withheld, or -1
 };
 
 // n / d for n * d < 2^38, from floor(2^38 / d) + 1 (a division of run-time integers takes some 40
@@ -259,6 +261,8 @@ struct Kv4AttnSmem {
   int upto[(W + 1) * 32];                   // tiles of the sequences up to and with a thread's
   int last[2];
   int empties;                              // there are sequences of no tokens
+  int stop, done;                           // a wait ran out; no more copies will be started
+  int issued[32];                           // tiles that a lane of the copying warp started, once it is done
 };
 
 __device__ __forceinline__ uint2 kv4_lds64(uint32_t at) {
@@ -283,6 +287,30 @@ struct Kv4Lane {
     asm volatile("" : "+r"(code), "+r"(kpar), "+r"(kown), "+r"(vpar), "+r"(vmid));
   }
 };
+
+// A flag in shared memory from one warp to the others, with what its lane wrote before.
+__device__ __forceinline__ void kv4_raise(int* flag) {
+  __threadfence_block();
+  *(volatile int*)flag = 1;
+}
+__device__ __forceinline__ bool kv4_raised(const int* flag) {
+  const bool up = *(const volatile int*)flag != 0;
+  __threadfence_block();
+  return up;
+}
+
+// Waits for a tile, the same answer for the whole warp: false when limit_ns pass first or `stop` is raised.
+// (The vote costs 1-2 % of a long call; what comes after a wait has to be one path for all lanes.)
+__device__ __forceinline__ bool kv4_wait_tile(uint64_t* bar, uint32_t parity, unsigned long long limit_ns, const int* stop) {
+  bool there = mbar_try_wait_plain(bar, parity);
+  if (!there) {
+    const unsigned long long t0 = global_timer_ns();
+#pragma unroll 1
+    while (!(there = mbar_try_wait_plain(bar, parity)))
+      if (kv4_raised(stop) || global_timer_ns() - t0 > limit_ns) break;
+  }
+  return __all_sync(0xffffffffu, there);
+}
 
 // The columns of one segment in a warp's registers.
 template <int NT>
@@ -610,7 +638,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
   if (tid < Smem::kShared) sm.shared_start[tid] = -1;
   fence_mbar_init();
   const int empties = __syncthreads_or(empty);
-  if (tid == 0) sm.empties = empties;       // kept there: it would take a register all along
+  if (tid == 0) sm.empties = empties, sm.stop = sm.done = 0;   // kept there: it would take a register all along
   int warps = lane <= W ? sm.scan[lane] : 0;  // tiles up to and with a warp's
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -706,15 +734,18 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
     if ((lane & 1) && use.left > 0) use.advance(p, 1);
     look();
     unsigned long long idle_since = 0;
+    int issued = 0;
     while (__any_sync(0xffffffffu, more)) {
       const bool go = more && mbar_test_wait(&sm.empty[who][slot], parity);
       if (!__any_sync(0xffffffffu, go)) {
         const unsigned long long now = global_timer_ns();
         if (idle_since == 0) idle_since = now;
-        if (now - idle_since > kWaitLimitNs) {
-          if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
-          break;
+        const bool late = __any_sync(0xffffffffu, now - idle_since > p.wait_ns);
+        if (late && lane == 0) {
+          record_error(p.pool.err, kDevWaitCopy);
+          kv4_raise(&sm.stop);
         }
+        if (late || __any_sync(0xffffffffu, kv4_raised(&sm.stop))) break;
         __nanosleep(40);
         continue;
       }
@@ -728,7 +759,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
         uint64_t* bar = &sm.full[who][slot];
         if (there) {
           mbar_arrive_expect_tx(bar, kKv4TileBytes);
-          bulk_g2s(sm.ring[who][slot], p.pool.tile(page, head, tile), kKv4TileBytes, bar);
+          if (blockIdx.x || who || 2 * issued + (lane & 1) != p.skip_copy)
+            bulk_g2s(sm.ring[who][slot], p.pool.tile(page, head, tile), kKv4TileBytes, bar);
         } else {
           mbar_arrive(bar);
         }
@@ -747,16 +779,20 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
             mbar_arrive(bar);
           }
         }
+        ++issued;
         slot += 2;
         if (slot >= kRing) slot -= kRing, parity ^= 1;
         look();
       }
     }
+    sm.issued[lane] = issued;
+    __syncwarp();
+    if (lane == 0) kv4_raise(&sm.done);
   } else if (use.left > 0) {
     const Kv4Lane offsets(lane);
     Kv4Columns<NT> s;
     int slot = 0, parity = 0;
-    bool ok = true;
+    bool failed = false;
     while (use.left > 0) {
       const int n = use.here();
       const uint4* queries = nullptr;
@@ -772,11 +808,26 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       }
       kv4_begin<NT>(p, s, queries, use.hc, use.len, lane);
 #pragma unroll 1
-      for (int i = 0; i < n; ++i) {
-        // a wait that runs out is recorded; what follows waits briefly and computes on what is there
-        if (!mbar_wait(&sm.full[warp][slot], parity, ok ? kWaitLimitNs : 1000000ull)) {
-          ok = false;
-          if (lane == 0) record_error(p.pool.err, kDevWaitCopy);
+      for (int i = 0; i < n && !failed; ++i) {
+        if (!kv4_wait_tile(&sm.full[warp][slot], parity, p.wait_ns, &sm.stop)) {
+          // A wait ran out: reported, and no result of this call counts.  No slot is given back, the copying
+          // warp stops, and this one waits for its own copies in flight before its pieces go over the
+          // ring; they are merged and counted as ever, so that the workspace is left clear.
+          failed = true;
+          if (lane == 0) {
+            record_error(p.pool.err, kDevWaitCopy);
+            kv4_raise(&sm.stop);
+          }
+          const unsigned long long since = global_timer_ns();
+          while (!kv4_raised(&sm.done) && global_timer_ns() - since < p.wait_ns) __nanosleep(200);
+          __syncwarp();
+          for (int j = stretch - use.left + i, k = 0; k < kRing; ++j, ++k) {
+            if ((j >> 1) < *(volatile int*)&sm.issued[2 * warp + (j & 1)])
+              mbar_wait(&sm.full[warp][slot], parity, p.wait_ns);
+            if (++slot == kRing) slot = 0, parity ^= 1;
+          }
+          __syncwarp();
+          break;
         }
         const int pos = sm.pos[warp][slot];
         if (pos >= 0) {

@@ -23,7 +23,7 @@ namespace {
 
 thread_local char g_last_error[256] = "";
 // Test hooks (starkv_set_test_hooks): time limit of one device-side wait and a
-// K-kernel stage whose copy is never issued.
+// K-kernel stage, or 4-bit attention tile, whose copy is never issued.
 unsigned long long g_wait_ns = kWaitLimitNs;
 int g_skip_unit = -1;
 #ifdef STARKV_KTRACE
@@ -477,6 +477,8 @@ int host_device(int* sms) {
   if (!rc && sms) *sms = device_sm_count(nullptr);
   return rc;
 }
+unsigned long long host_wait_limit() { return g_wait_ns; }
+int host_skip_unit() { return g_skip_unit; }
 
 }  // namespace starkv
 
