@@ -76,7 +76,16 @@ def _output(t: torch.Tensor, name: str):
         raise StarKVError(f"{name} must not repeat elements (stride 0)")
 
 
+# The newest few streams' scratch: an attention workspace is 32 MB, and programs go through many
+# streams.  What is dropped goes back to its own stream's pool of torch's allocator, which hands
+# it out behind the work that still uses it.
 _WORKSPACES = {}
+_MAX_WORKSPACES = 8
+
+
+def release_workspaces() -> None:
+    """Give the scratch of all streams back to torch's allocator."""
+    _WORKSPACES.clear()
 
 
 def _workspace(kind: str, index: int, size, zeroed: int) -> torch.Tensor:
@@ -92,6 +101,10 @@ def _workspace(kind: str, index: int, size, zeroed: int) -> torch.Tensor:
         ws = torch.empty(need, dtype=torch.uint8, device=f"cuda:{index}")
         ws[:zeroed].zero_()
         if not capturing:
+            _WORKSPACES.pop(key, None)
+            held = [k for k in list(_WORKSPACES) if k[0] == kind]
+            for k in held[:max(0, len(held) + 1 - _MAX_WORKSPACES)]:
+                _WORKSPACES.pop(k, None)
             _WORKSPACES[key] = ws
     return ws
 

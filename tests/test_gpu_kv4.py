@@ -659,3 +659,30 @@ def test_nan_in_newer_tokens_does_not_reach_older_queries(cuda, dtype, Hkv, G, Q
     v[:, n - 1] = float("nan")
     made.cache.write(made.k, v, made.table, ints([0, 0], cuda))
     assert torch.equal(want, made.cache.attend(q, made.table, made.lengths, SCALING, mask=mask))
+
+
+def test_workspaces_of_many_streams_are_bounded(cuda):
+    """The scratch of a few streams is kept, whichever come, and can be let go."""
+    from starkv import kv4
+    made = Made(cuda, [3000, 17, 1024], 2, 64, F16, seed=63)
+    q = rnd((3, 1, 8, 128), F16, 64, cuda)
+    want = made.cache.attend(q, made.table, made.lengths, SCALING)
+    pages = made.cache.select(q, made.table, made.lengths, 4)
+    torch.cuda.synchronize()
+    kv4.release_workspaces()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    streams = [torch.cuda.Stream() for _ in range(20)]
+    got = []
+    for _ in range(2):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append((made.cache.attend(q, made.table, made.lengths, SCALING), made.cache.select(q, made.table, made.lengths, 4)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, pages) for a, b in got)
+    assert len({s.cuda_stream for s in streams}) > 10 >= kv4._MAX_WORKSPACES
+    assert torch.cuda.memory_allocated() - before <= kv4._MAX_WORKSPACES * (kv4._attention_size() + (1 << 20)) + (4 << 20)
+    kv4.release_workspaces()
+    del got
+    assert torch.cuda.memory_allocated() - before <= 1 << 20
+    assert torch.equal(want, made.cache.attend(q, made.table, made.lengths, SCALING))
