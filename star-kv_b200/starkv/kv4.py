@@ -20,6 +20,7 @@ the layout and the arithmetic); there is no CPU path.
 
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import struct
 from typing import Optional, Tuple
@@ -177,6 +178,14 @@ class KV4Cache:
                                   0 if bounds is None else bound_scales.data_ptr(), error_word.data_ptr(),
                                   self.num_pages, self.num_kv_heads, self.page_size, 128)
         self._lib = load()
+
+    def __deepcopy__(self, memo) -> "KV4Cache":
+        """A pool of its own with the same contents (the argument block holds addresses)."""
+        parts = (self.data, self.bounds, self.bound_scales, self.error_word)
+        return self.from_tensors(*[copy.deepcopy(t, memo) for t in parts])
+
+    def __reduce__(self):
+        return self.from_tensors, (self.data, self.bounds, self.bound_scales, self.error_word)
 
     def nbytes(self) -> int:
         """Device bytes of the pool (codes, parameters and bounds)."""

@@ -686,3 +686,34 @@ def test_workspaces_of_many_streams_are_bounded(cuda):
     del got
     assert torch.cuda.memory_allocated() - before <= 1 << 20
     assert torch.equal(want, made.cache.attend(q, made.table, made.lengths, SCALING))
+
+
+def test_copies_have_pools_of_their_own(cuda):
+    """copy.deepcopy (a prompt's cache reused) and pickling: the copy holds the same tokens, and
+    writing into one leaves the other as it is; a shallow copy shares the pool."""
+    import copy
+    import pickle
+    from starkv.attention import StarKVCache
+    from starkv.kv4_attention import KV4State
+    made = Made(cuda, [300, 77], 2, 64, F16, seed=65, garbage=False)
+    q = rnd((2, 1, 8, 128), F16, 66, cuda)
+    want = made.cache.attend(q, made.table, made.lengths, SCALING)
+    whole = StarKVCache(400)
+    whole.kv4_states[0] = KV4State(2, 400, 2, 64, cuda, page_bounds=True)
+    whole.kv4_states[0].append(made.k, made.v)
+    other = copy.deepcopy(whole)
+    new = rnd((2, 1, 2, 128), F16, 67, cuda)
+    before = [t.clone() for t in whole.kv4_states[0].history(F32)]
+    other.kv4_states[0].append(new, new)
+    assert (other.get_seq_length(), whole.get_seq_length()) == (301, 300)
+    assert all(torch.equal(a, b) for a, b in zip(before, whole.kv4_states[0].history(F32)))
+    assert all(torch.equal(a, b[:, :300]) for a, b in zip(before, other.kv4_states[0].history(F32)))
+    for twin in (copy.deepcopy(made.cache), pickle.loads(pickle.dumps(made.cache))):
+        assert twin.data.data_ptr() != made.cache.data.data_ptr() and torch.equal(twin.bounds, made.cache.bounds)
+        twin.write(new, new, made.table, ints([0, 0], cuda))
+        assert not torch.equal(twin.attend(q, made.table, made.lengths, SCALING), want)
+        assert torch.equal(made.cache.attend(q, made.table, made.lengths, SCALING), want)
+    bare = copy.deepcopy(KV4Cache(3, 1, page_bounds=False, device=cuda))
+    assert bare.bounds is None and bare.num_pages == 3
+    shared = copy.copy(made.cache)
+    assert shared.data is made.cache.data and torch.equal(shared.attend(q, made.table, made.lengths, SCALING), want)
