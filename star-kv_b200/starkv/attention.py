@@ -118,6 +118,17 @@ class StarKVCache(_HFCache):
     def __len__(self):
         return len(self.states) + len(self.kv4_states)
 
+    def crop(self, max_length: int) -> None:
+        """Forgets the tokens from ``max_length`` on (negative: that many of the newest), as
+        transformers' assisted generation does with drafts that were not accepted."""
+        for st in (*self.states.values(), *self.kv4_states.values()):
+            keep = max_length if max_length >= 0 else max(0, st.length + max_length)
+            if keep < st.length:
+                st.crop(keep)
+
+    def reset(self) -> None:
+        self.crop(0)
+
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         raise NotImplementedError("StarKVCache is written by the STAR-KV attention modules themselves "
                                   "(latents appended in place by the decode kernels)")

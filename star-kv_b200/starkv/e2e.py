@@ -217,8 +217,7 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     def rewind():                                        # forget what the warm-up and the capture appended
         for st, w in zip(states, kv4):
             if w:
-                st.lengths.fill_(held)
-                st.length = held
+                st.crop(held)
 
     rewind()
     graphs = []

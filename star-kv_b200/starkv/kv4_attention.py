@@ -64,6 +64,11 @@ class KV4State:
         self.lengths.add_(k.shape[1])
         self.length += k.shape[1]
 
+    def crop(self, length: int) -> None:
+        """Forgets the tokens from ``length`` on; their slots are written anew."""
+        self.lengths.fill_(length)
+        self.length = length
+
     def select(self, q: torch.Tensor, keep_pages: int, mask: Optional[torch.Tensor] = None,
                newest: Optional[int] = None) -> torch.Tensor:
         """The pages (``KV4Cache.select``) of queries q (B, T, Hq, 128) among the ``newest``

@@ -45,6 +45,10 @@ class DecodeLayer:
     def length(self) -> int:
         return self.cache.length
 
+    def crop(self, length: int) -> None:
+        """Forgets the tokens from ``length`` on; their slots are written anew."""
+        self.cache.length = length
+
     def prefill(self, k_lat: torch.Tensor, v_lat: torch.Tensor):
         self.cache.prefill(k_lat.contiguous(), v_lat.contiguous())
 

@@ -275,3 +275,39 @@ def test_keep_pages_set_after_the_prompt(cuda):
         attn.keep_pages = 3
         outs.append(attn(x[:, 400:], (one, one * 0), None, past_key_values=cache)[0])
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("kv4_layers", [(0, 1), (0,), ()])
+@torch.no_grad()
+def test_rejected_drafts_are_forgotten(cuda, kv4_layers):
+    """StarKVCache.crop: drafts (single tokens where a layer holds latents) that are taken back leave
+    no trace, over a page's end, with page bounds and after a reset."""
+    model = small_model(cuda, kv4_layers, kv4_keep_pages=3)
+    from starkv.e2e import forward_tokens
+    model.starkv_quantized = False
+    g = torch.Generator(device=cuda).manual_seed(18)
+    ids = torch.randint(0, 1000, (2, 230), generator=g, device=cuda)
+    P = 62
+    step = 6 if kv4_layers == (0, 1) else 1
+    plain, cache = StarKVCache(256), StarKVCache(256)
+    for c in (plain, cache):
+        forward_tokens(model, ids[:, :P], 0, c)
+    for turn in range(2):
+        wrong = torch.randint(0, 1000, (2, 2 * step), generator=g, device=cuda)
+        for i in range(2):
+            forward_tokens(model, wrong[:, i * step:(i + 1) * step], P + i * step, cache)
+        assert cache.get_seq_length() == P + 2 * step
+        cache.crop(P + 1 if turn else -2 * step)
+        if turn:
+            cache.crop(P)
+        assert all(cache.get_seq_length(i) == P for i in range(2))
+        for i in range(70):
+            a = forward_tokens(model, ids[:, P + i:P + i + 1], P + i, cache)
+            b = forward_tokens(model, ids[:, P + i:P + i + 1], P + i, plain)
+            assert torch.equal(a, b), i
+        P += 70
+    cache.crop(1000)
+    assert cache.get_seq_length() == P
+    cache.reset()
+    assert cache.get_seq_length() == 0
+    assert torch.equal(forward_tokens(model, ids[:, :100], 0, cache), forward_tokens(model, ids[:, :100], 0, StarKVCache(256)))
