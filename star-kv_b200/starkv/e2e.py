@@ -154,6 +154,11 @@ def generate_graphed(model, prompt: torch.Tensor, new_tokens: int, capacity: int
     p1.record()
     tok = logits.argmax(-1, keepdim=True)
     out: List[torch.Tensor] = [tok]
+    if new_tokens <= 1:                                  # no step to capture, and no room asked for one
+        torch.cuda.synchronize()
+        if stats is not None:
+            stats["prompt_s"] = p0.elapsed_time(p1) / 1e3
+        return tok, 0.0
     layers = model.model.layers
     dt = model.model.embed_tokens.weight.dtype
     attn0 = layers[0].self_attn

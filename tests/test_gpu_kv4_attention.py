@@ -145,3 +145,18 @@ def test_mixed_layers_decode_matches_recompute(cuda):
     got = forward_tokens(model, seq[:, -1:], 80, cache)
     want = forward_tokens(model, seq, 0, StarKVCache(90))
     assert rel(got.float(), want.double()) <= 0.2
+
+
+@pytest.mark.parametrize("kv4_layers", [(0,), (0, 1), ()])
+def test_graphed_loop_with_a_cache_that_the_prompt_fills(cuda, kv4_layers):
+    """One new token needs no slot: the loop from graphs gives the eager loop's, as it does where the
+    last step fills the cache."""
+    model = build_model(num_layers=2, hidden=512, heads=4, kv_heads=2, mlp=1024, vocab=1000, v_block_kv=2,
+                        quantized=False, seed=3, device=cuda, max_positions=512, kv4_layers=kv4_layers)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    prompt = torch.randint(0, 1000, (2, 64), generator=g, device=cuda)
+    for new, capacity in ((1, 64), (1, 65), (65, 128)):
+        a, b = {}, {}
+        want, _ = generate(model, prompt, new, capacity, a)
+        got, per = generate_graphed(model, prompt, new, capacity, b)
+        assert torch.equal(want, got) and got.shape == (2, new) and per >= 0 and b["prompt_s"] > 0
