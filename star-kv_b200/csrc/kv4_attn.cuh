@@ -28,9 +28,10 @@
 //     The centres add sum w m_g, and a row of ones sums the rounded weights: dividing by
 //     that sum takes their rounding out of what they have in common (one key that
 //     outweighs the rest has no error from it).  The log-sum-exp has the sum in fp32.
-//     w is 2^(x - m + 11 - e): m a running maximum that may trail by 2^4, e >= 0 the
-//     exponent that keeps every s_g so far <= 2^e, so neither small weights nor
-//     large s leave fp16.
+//     w is 2^(x - m + 11 - max(e, 0)): m a running maximum that may trail by 2^4, 2^e the
+//     least of 2^-14, 2^-7 and 2^0, 2^1 .. that no s_g so far is above; with e < 0 the
+//     factors are w (s_g 2^-e).  So no factor passes 2^15, and a weight 2^-20 of the
+//     largest still has 8 bits or more where all s are alike, whatever their size.
 //
 // Work split.  All (sequence, KV head, column block) segments form one line of
 // tiles; CTA i of a grid of one CTA per SM takes an equal stretch of it, its warps
@@ -322,7 +323,7 @@ struct Kv4Columns {
   float o[8][NT][4], l[NT][2];
   float z[NT][4];                           // sum w m: group j in rows j / 2 and j / 2 + 8; sum w in row 2
   float base[NT][2], thr[NT][2];            // w = 2^(x - base); x beyond thr moves the base
-  int e;
+  int e;                                    // no s so far is above 2^e: -14, -7 or >= 0; o is in units of 2^min(e, 0)
 };
 
 // The queries of 8 columns of a segment as the scores' operands: five vectors a lane in `buf` (32
@@ -417,7 +418,7 @@ __device__ __forceinline__ void kv4_begin(const Kv4AttnParams& p, Kv4Columns<NT>
       for (int mt = 0; mt < 8; ++mt) s.o[mt][nt][i] = 0.f;
     }
   }
-  s.e = 0;
+  s.e = -14;
 }
 
 // One tile at shared address tl.  MASK: its additive mask at shared address mk.  EDGE: some of its
@@ -509,7 +510,9 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
   // ---- a score or an s that the base does not cover
   if (__any_sync(0xffffffffu, over)) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(big & 0xffffu, big >> 16));
-    const int e_new = (int)((top + 0x3ffu) >> 10) - 15;
+    int e_new = (int)((top + 0x3ffu) >> 10) - 15;
+    if (e_new < 0) e_new = e_new <= -14 ? -14 : e_new <= -7 ? -7 : 0;
+    const float unit_o = __int_as_float((127 + min(s.e, 0) - min(e_new, 0)) << 23);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -521,9 +524,9 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
         const float unit = MASK ? 1.f : s.cs[nt][u];
         t *= unit;
         const bool before = s.thr[nt][u] != -INFINITY;
-        const float m = before ? fmaxf(t, s.base[nt][u] + (float)(11 - s.e)) : t;
+        const float m = before ? fmaxf(t, s.base[nt][u] + (float)(11 - max(s.e, 0))) : t;
         if (m == -INFINITY) continue;
-        const float moved = m + (float)(e_new - 11);
+        const float moved = m + (float)(max(e_new, 0) - 11);
         const float f = before ? kv4_exp2(s.base[nt][u] - moved) : 0.f;
         s.base[nt][u] = moved;
         s.thr[nt][u] = (m + 4.f) / unit;
@@ -531,9 +534,14 @@ __device__ __forceinline__ void kv4_tile(Kv4Columns<NT>& s, const uint4* queries
         s.z[nt][u] *= f;
         s.z[nt][u + 2] *= f;
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) s.o[mt][nt][u] *= f, s.o[mt][nt][u + 2] *= f;
+        for (int mt = 0; mt < 8; ++mt) s.o[mt][nt][u] *= f * unit_o, s.o[mt][nt][u + 2] *= f * unit_o;
       }
     s.e = e_new;
+  }
+  if (s.e < 0) {                            // values far below one
+    const uint32_t up = (uint32_t)(15 - s.e) * 0x04000400u;
+    ta.x = kv4_hmul2(ta.x, up), ta.y = kv4_hmul2(ta.y, up), ta.z = kv4_hmul2(ta.z, up), ta.w = kv4_hmul2(ta.w, up);
+    tb.x = kv4_hmul2(tb.x, up), tb.y = kv4_hmul2(tb.y, up), tb.z = kv4_hmul2(tb.z, up), tb.w = kv4_hmul2(tb.w, up);
   }
   // ---- weights and values
   if (NT == 1) load_values();
@@ -850,6 +858,7 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
       const bool whole = n == use.tiles;
       const int pi = 2 * warp + (use.left > n);
       float* part = whole && use.left > n ? heads + (W + warp) * kPiece : piece_at(pi);
+      const float u24 = __int_as_float((127 + 24 + min(s.e, 0)) << 23), u20 = u24 * 0x1p-4f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -869,8 +878,8 @@ __global__ void __launch_bounds__((W + 1) * 32, 1) kv4_attn_kernel(const Kv4Attn
             const float y = __shfl_sync(0xffffffffu, s.z[nt][u + 2 * (j & 1)], (j >> 1) * 4 + c);
             if (col < real)
               *reinterpret_cast<float4*>(part + col * 128 + j * 32 + 4 * r) =
-                  make_float4(fmaf(s.o[2 * j][nt][u], 0x1p24f, y), fmaf(s.o[2 * j][nt][u + 2], 0x1p20f, y),
-                              fmaf(s.o[2 * j + 1][nt][u], 0x1p24f, y), fmaf(s.o[2 * j + 1][nt][u + 2], 0x1p20f, y));
+                  make_float4(fmaf(s.o[2 * j][nt][u], u24, y), fmaf(s.o[2 * j][nt][u + 2], u20, y),
+                              fmaf(s.o[2 * j + 1][nt][u], u24, y), fmaf(s.o[2 * j + 1][nt][u + 2], u20, y));
           }
         }
       if (whole) {

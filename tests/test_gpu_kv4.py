@@ -717,3 +717,34 @@ def test_copies_have_pools_of_their_own(cuda):
     assert bare.bounds is None and bare.num_pages == 3
     shared = copy.copy(made.cache)
     assert shared.data is made.cache.data and torch.equal(shared.attend(q, made.table, made.lengths, SCALING), want)
+
+
+@pytest.mark.parametrize("scale,grow", [(1e-5, 1), (1e-4, 1), (1e-3, 1), (1e-2, 1), (1.0, 1), (1e-5, 40), (1e-5, 3000), (1e-4, 100), (0.05, 40)])
+def test_attention_to_many_small_values_behind_one_peak(cuda, scale, grow):
+    """One key holds nearly all the weight, the others 2^-20 of its weight each, so many in a warp's
+    stretch that together they are some hundredths; the values may be far below one and grow on the
+    way.  The bound at the head of this file without its absolute part: what the small weights add is
+    not lost below fp16's range."""
+    B, H, page, n = 8, 32, 128, 131072
+    W = n // page
+    k = rnd((1, n, 1, 128), F16, 71, cuda)
+    v = rnd((1, n, 1, 128), F32, 72, cuda).clamp(-3, 3)
+    v[..., ::32] = 4.0                                        # code 7 in every token: losses do not average out
+    at = torch.arange(n, device=cuda)[None, :, None, None] / 128 % 100 / 100    # again and again within a stretch's length
+    v = v * scale * torch.where(at > 0.6, float(grow), torch.where(at > 0.3, grow ** 0.5, 1.0))
+    cache = KV4Cache(B * W, H, page_size=page, device=cuda, page_bounds=False)
+    table = table_of(B, W, cuda, 5)
+    cache.write(k.float().expand(B, n, H, 128), v.expand(B, n, H, 128), table, ints([0] * B, cuda))
+    mask = torch.full((B, n), -14.0, device=cuda)
+    mask[:, 37] = 0
+    q = torch.zeros(B, 1, H, 128, dtype=F16, device=cuda)
+    out = torch.empty(q.shape, device=cuda)
+    cache.attend(q, table, ints([n] * B, cuda), SCALING, mask=mask, out=out)
+    vals = O.values(f64(v[0, :, 0]))
+    c, s, m = O.quantise(f64(v[0, :, 0]))
+    w = np.exp(f64(mask[0]))
+    w /= w.sum()
+    size = (np.abs(s[..., None] * c) + np.abs(m)[..., None]).reshape(n, 128)
+    tol = (2 * U * (1 + 2 * U) + 2.0 ** -18) * (w @ size)
+    err = np.abs(f64(out[:, 0]) - w @ vals)                   # the same tokens in every sequence and head
+    assert (err <= tol).all(), (err / tol).max()
