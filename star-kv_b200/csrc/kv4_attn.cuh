@@ -22,9 +22,9 @@
 //     of the tensor cores do not act on sums 8 s times as large (measured at 32K
 //     tokens: relative error 1.5e-3 when the -8 is taken at the end instead).
 //     Where one channel of a group is many times the others, s c and m nearly cancel for
-//     those and the rounding of w s_g shows: relative error of an fp16 output up to
-//     3.3e-4, against 2.1e-4 of the exact one rounded (bf16: 1.6e-3 to
-//     1.7e-3, against 1.6e-3).
+//     those and the rounding of w s_g shows: relative error of an fp16 output 2.1e-4 to
+//     4.1e-4, against 2.0e-4 of the exact one rounded (bf16: a few percent more than
+//     that).  The rest of w s_g as a second operand would cost an estimated eighth more.
 //     The centres add sum w m_g, and a row of ones sums the rounded weights: dividing by
 //     that sum takes their rounding out of what they have in common (one key that
 //     outweighs the rest has no error from it).  The log-sum-exp has the sum in fp32.
@@ -40,20 +40,20 @@
 // and what a CTA does not hold whole goes to the workspace, where the CTA that
 // arrives last merges it in CTA order (the same result every time).
 //
-// Measured on a B200 (copy: 6.45 TB/s): 16 sequences of 32768 tokens, 32 KV heads, one
-// query head each (2.7 GB): 508 us, 5.3 TB/s; 64 sequences of up to 8192, 8 KV heads of 4,
-// pages of 16: 82 us, 4.2 TB/s; one sequence of 32769, 8 of 4: 22.5 us; 8 sequences of up to
-// 16384, 8 of 4, 4 query tokens, masked: 50 us.  Long contexts are bound by issue and
-// dependent latencies: 246 warp instructions a tile (80 of them the nibbles' masks and
-// shifts, 26 matrix instructions of 8 cycles), 122 cycles a tile and SM without the copies
-// where HBM takes 111 for its 2560 bytes.  Short ones by the chain of start (lengths,
-// queries, block table, first tile: 5 us) and merge (6 us).
+// Measured on a B200 (copy: 6.45 TB/s), device time with the L2 flushed: 16 sequences of 32768
+// tokens, 32 KV heads, one query head each (2.7 GB): 510 us, 5.3 TB/s (call after call at the power
+// cap 532-561 us); 64 sequences of up to 8192, 8 KV heads of 4, pages of 16: 88 us; one sequence of
+// 32769, 8 of 4: 28 us (23 with the L2 warm); 8 sequences of up to 16384, 8 of 4, 4 query tokens,
+// masked: 53 us.  Long contexts are bound by issue and dependent latencies: 274 warp instructions a
+// tile (80 of them the nibbles' masks and shifts, 26 matrix instructions of 8 cycles), about 140
+// cycles a tile and SM where HBM takes 115 for its 2560 bytes.  Short ones by the chain of start
+// (lengths, queries, block table, first tile: 5 us) and merge (6 us).
 #pragma once
 #include "kv4.cuh"
 
 namespace starkv {
 
-constexpr int kKv4PadTiles = 4;             // see kv4_tiles; 64 mixed sequences: 115 us with 0, 85 with 2, 82 with 4 or 7
+constexpr int kKv4PadTiles = 4;             // see kv4_tiles; 64 mixed sequences, when chosen: 115 us with 0, 85 with 2, 82 with 4 or 7
 constexpr int kKv4MaxGrid = 160;            // CTAs the workspace has room for
 constexpr int kKv4MaxCols = 16;
 // One piece of a segment: o (cols, 128), then per column the base, the sum of the weights and the
