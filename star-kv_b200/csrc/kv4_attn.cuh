@@ -31,7 +31,7 @@
 //     w is 2^(x - m + 11 - max(e, 0)): m a running maximum that may trail by 2^4, 2^e the
 //     least of 2^-14, 2^-7 and 2^0, 2^1 .. that no s_g so far is above; with e < 0 the
 //     factors are w (s_g 2^-e).  So no factor passes 2^15, and a weight 2^-20 of the
-//     largest still has 8 bits or more where all s are alike, whatever their size.
+//     largest still has 8 bits or more where all s are alike, for any s from 2^-21 up.
 //
 // Work split.  All (sequence, KV head, column block) segments form one line of
 // tiles; CTA i of a grid of one CTA per SM takes an equal stretch of it, its warps
