@@ -114,12 +114,14 @@ static_assert(kPkSmemBytes <= 227 * 1024, "shared memory of one SM");
 
 __device__ __forceinline__ PkSeq pk_seq(const PackedParams& p, int b) {
   const int q0 = p.q_start[b], q1 = p.q_end[b], k0 = p.k_start[b], k1 = p.k_end[b];
+  // ends are held within the tensors before any difference is taken: one far below zero would wrap around
   PkSeq s;
   s.q0 = min(max(q0, 0), p.total_q);
-  s.qn = max(min(q1, p.total_q) - s.q0, 0);
   s.k0 = min(max(k0, 0), p.total_k);
-  s.kn = max(min(k1, p.total_k) - s.k0, 0);
-  if (s.q0 != q0 || s.k0 != k0 || s.q0 + s.qn != q1 || s.k0 + s.kn != k1) record_error(p.err, kDevBadRange);
+  const int qe = min(max(q1, s.q0), p.total_q), ke = min(max(k1, s.k0), p.total_k);
+  s.qn = qe - s.q0;
+  s.kn = ke - s.k0;
+  if (s.q0 != q0 || s.k0 != k0 || qe != q1 || ke != k1) record_error(p.err, kDevBadRange);
   return s;
 }
 

@@ -324,3 +324,25 @@ def test_timed_out_copy(cuda, skip, nq, nk):
     for _ in range(3):
         assert torch.equal(packed_attention(q, k, v, cq, ck, SCALE, error_word=err), want)
     assert int(err) == 0
+
+
+@pytest.mark.parametrize("batch", [4, 300, 1500])
+def test_ends_far_below_zero(cuda, batch):
+    """Ends near -2^31 behind starts inside the tensors: such a sequence has no rows and the error word says
+    so, in the table of up to 256 sequences and beyond; the others are what they are without it."""
+    q, k, v = make((2 * batch, 2, 128), torch.float16), make((2 * batch, 1, 128), torch.float16, 1), make((2 * batch, 1, 128), torch.float16, 2)
+    starts = torch.arange(batch, dtype=torch.int32, device="cuda") * 2
+    pairs = [(2 * b, 2 * b + 2) for b in range(0, batch, 2)]
+    live = torch.zeros(2 * batch, dtype=torch.bool, device="cuda")
+    live.view(-1, 4)[:, :2] = True
+    want = [t[live] for t in reference(q, k, v, pairs, pairs)]
+    for low in (-2 ** 31, -2 ** 31 + 1, -2 ** 31 + batch, -1):
+        for which in ("q", "k"):
+            ends = {"q": starts + 2, "k": starts + 2}
+            ends[which][1::2] = low
+            out, err = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+            packed_attention(q, k, v, (starts, ends["q"]), (starts, ends["k"]), SCALE, out=out, error_word=err)
+            assert int(err) == 0x203
+            close(out[live], None, want, torch.float16, 2)
+            # without queries rows are left alone, without keys they are 0
+            assert bool((out[~live] == (7.0 if which == "q" else 0.0)).all())
