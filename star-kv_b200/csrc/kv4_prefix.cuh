@@ -591,6 +591,7 @@ __global__ void __launch_bounds__(kKvpThreads, 1) kv4_prefix_kernel(const __grid
       for (int piece = blockIdx.x; ok && piece < pieces; piece += gridDim.x, ++round) {
         const int split = piece / p.blocks % splits, n = first_step(split + 1) - first_step(split);
         const int ahead = halves ? 2 : 1;                   // a tile's next step
+        if (n == 0) continue;                               // an empty prefix: no piece has a step
         for (int x = 0; ok && x < 2; ++x) wait(&sm.q_full[x], round & 1, kDevWaitCopy);
         if (!ok) break;
         // step u of the piece is step g + u of all; with halves tile u & 1 takes it, else both do
@@ -696,7 +697,9 @@ __global__ void __launch_bounds__(kKvpThreads, 1) kv4_prefix_kernel(const __grid
       const int u0 = first_step(split), n = first_step(split + 1) - u0;
       const int row_id = block * 256 + (halves ? 0 : x * 128) + r;
       PkRow row = {-INFINITY, 0.f, false};
-      {
+      // Queries are laid out for products only: without a step nothing holds the rows back, and a tile's
+      // would arrive for their next piece while the issuer still waits for the other tile's first.
+      if (n > 0) {
         const KvpRow at = kvp_row(p, kvh, row_id);
         const int k = kvp_query(p.s.q, p.s.q_dtype, at.q, at.live, Qs + x * kPkTileBytes, Qm + x * kKvpSumBytes, r);
         fence_proxy_async_smem();
