@@ -34,7 +34,7 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
     scaling: None, or a model configuration's ``rope_scaling`` / ``rope_parameters``, of
     ``rope_type`` "default", "linear" (factor), "llama3" (factor, low_freq_factor,
     high_freq_factor, original_max_position_embeddings) or "yarn" (factor,
-    original_max_position_embeddings, beta_fast, beta_slow, attention_factor); a
+    original_max_position_embeddings, beta_fast, beta_slow, truncate, attention_factor); a
     ``rope_theta`` in it is the base."""
     s = dict(scaling or {})
     base = float(s.get("rope_theta", base))
@@ -67,8 +67,10 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
         old = number("original_max_position_embeddings")
         # the pair that makes n turns over the original context
         pair = lambda n: rotary_dim * math.log(old / (2.0 * math.pi * n)) / (2.0 * math.log(base))  # noqa: E731
-        lo = max(math.floor(pair(number("beta_fast", 32.0))), 0)
-        hi = min(math.ceil(pair(number("beta_slow", 1.0))), rotary_dim - 1)
+        lo, hi = pair(number("beta_fast", 32.0)), pair(number("beta_slow", 1.0))
+        if s.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         for i, x in enumerate(f):
             e = min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001)))
             f[i] = (1.0 - e) * x + e * x / factor

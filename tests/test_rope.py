@@ -87,3 +87,12 @@ def test_c_negative_strides_refused():
     a.x_strides[0][1] = -128
     assert _lib.load().starkv_rope(C.byref(a), None) == 1
     assert _lib.load().starkv_rope(None, None) == 1
+
+
+@pytest.mark.parametrize("dim,base,scaling", [(64, 150000.0, dict(YARN, truncate=False)), (64, 150000.0, dict(YARN, truncate=True)),
+                                              (64, 150000.0, dict(YARN, truncate=None)), (128, 10000.0, dict(YARN, truncate=False, beta_fast=16.0)),
+                                              (128, 1000000.0, dict(YARN, truncate=False, factor=4.0, beta_slow=2.0)),
+                                              (64, 500000.0, dict(LLAMA3, truncate=False))])
+def test_truncate(dim, base, scaling):
+    """Whether yarn's ramp begins and ends on whole pairs."""
+    test_frequencies_are_those_of_transformers(dim, base, scaling)
