@@ -94,5 +94,16 @@ def test_c_negative_strides_refused():
                                               (128, 1000000.0, dict(YARN, truncate=False, factor=4.0, beta_slow=2.0)),
                                               (64, 500000.0, dict(LLAMA3, truncate=False))])
 def test_truncate(dim, base, scaling):
-    """Whether yarn's ramp begins and ends on whole pairs."""
-    test_frequencies_are_those_of_transformers(dim, base, scaling)
+    """Whether yarn's ramp begins and ends on whole pairs.  Theirs is fp32, off by 16 u (u = 2^-24) as above;
+    and its ramp e = (i - lo) / (hi - lo) by u for the rounding of each end, u lo / (hi - lo) and
+    u hi / (hi - lo), and for the subtraction, the division and 1 - e: 8 u where lo + hi <= 5 (hi - lo), as
+    it is here.  The ramp is multiplied by the unscaled frequency, which is up to `factor` times the result."""
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    got, factor = rope_frequencies(dim, base, scaling)
+    cfg = LlamaConfig(hidden_size=dim, num_attention_heads=1, head_dim=dim, max_position_embeddings=131072,
+                      rope_parameters=dict(scaling, rope_theta=base))
+    want, wf = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")
+    assert factor == pytest.approx(wf, rel=1e-6) and len(want) == len(got)
+    for i, (a, b) in enumerate(zip(got, want.tolist())):
+        assert abs(a - b) <= 2.0 ** -24 * (16 * b + 8 * base ** (-2 * i / dim))
