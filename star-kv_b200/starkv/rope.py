@@ -35,7 +35,8 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
     ``rope_type`` "default", "linear" (factor), "llama3" (factor, low_freq_factor,
     high_freq_factor, original_max_position_embeddings) or "yarn" (factor,
     original_max_position_embeddings, beta_fast, beta_slow, truncate, attention_factor); a
-    ``rope_theta`` in it is the base."""
+    ``rope_theta`` in it is the base; of a ``partial_rotary_factor`` rotary_dim is the outcome (``Rope``
+    works it out)."""
     s = dict(scaling or {})
     base = float(s.get("rope_theta", base))
     kind = s.get("rope_type", s.get("type", "default"))
@@ -81,9 +82,26 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
     raise StarKVError(f"unknown rope_type {kind!r}")
 
 
+def rotary_channels(head_dim: int, rotary_dim: Optional[int] = None, scaling: Optional[dict] = None) -> int:
+    """How many channels of a head turn: ``rotary_dim``, or the part of head_dim that scaling's
+    ``partial_rotary_factor`` says, or all."""
+    part = (scaling or {}).get("partial_rotary_factor")
+    if part is not None:
+        if not 0 < float(part) <= 1:
+            raise StarKVError(f"partial_rotary_factor must be above 0 and at most 1, got {part}")
+        part = int(head_dim * float(part))
+        if rotary_dim is not None and rotary_dim != part:
+            raise StarKVError(f"rotary_dim {rotary_dim} is not the scaling's partial_rotary_factor of head_dim, {part}")
+        rotary_dim = part
+    rotary_dim = head_dim if rotary_dim is None else rotary_dim
+    if rotary_dim <= 0 or rotary_dim % 2 or rotary_dim > head_dim:
+        raise StarKVError(f"rotary_dim must be even, positive and at most head_dim {head_dim}, got {rotary_dim}")
+    return rotary_dim
+
+
 class Rope:
-    """Rotary positions of heads of ``head_dim``, of which the first ``rotary_dim`` channels (all by
-    default) turn: pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with ``interleaved``.
+    """Rotary positions of heads of ``head_dim``, of which the first ``rotary_dim`` channels (by default
+    all, or ``scaling``'s ``partial_rotary_factor`` of them) turn: pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with ``interleaved``.
 
     Frequencies come from ``base`` and ``scaling`` (``rope_frequencies``), or are given:
     ``frequencies`` (rotary_dim / 2 numbers, e.g. a model's ``inv_freq``) and ``factor``."""
@@ -91,9 +109,7 @@ class Rope:
     def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: Optional[int] = None, interleaved: bool = False,
                  scaling: Optional[dict] = None, frequencies: Optional[Union[Sequence[float], torch.Tensor]] = None,
                  factor: float = 1.0, device="cuda"):
-        rotary_dim = head_dim if rotary_dim is None else rotary_dim
-        if rotary_dim <= 0 or rotary_dim % 2 or rotary_dim > head_dim:
-            raise StarKVError(f"rotary_dim must be even, positive and at most head_dim {head_dim}, got {rotary_dim}")
+        rotary_dim = rotary_channels(head_dim, rotary_dim, scaling)
         if frequencies is None:
             frequencies, factor = rope_frequencies(rotary_dim, base, scaling)
         elif scaling is not None:

@@ -226,3 +226,13 @@ def test_refusals(cuda):
                 lambda: rope.apply(q, q.clone(), pos, out=(q, q))):
         with pytest.raises(StarKVError):
             bad()
+
+
+def test_part_of_a_head_from_the_scaling(cuda):
+    """The constructor takes the turned channels from partial_rotary_factor."""
+    rope = Rope(128, scaling=dict(YARN, rope_theta=500000.0, truncate=False, partial_rotary_factor=0.25))
+    assert rope.rotary_dim == 32
+    q, pos = make((9, 3, 128), torch.float32), torch.arange(9, device=cuda) * 1000
+    got = rope.apply(q, None, pos)
+    close(got, *reference(rope, q, pos))
+    assert torch.equal(got[..., 32:], q[..., 32:])

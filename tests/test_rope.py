@@ -6,7 +6,7 @@ import math
 import pytest
 
 from starkv import _lib, rope
-from starkv.rope import rope_frequencies, turns_of
+from starkv.rope import rope_frequencies, rotary_channels, turns_of
 
 LLAMA3 = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192)
 YARN = dict(rope_type="yarn", factor=32.0, original_max_position_embeddings=4096)
@@ -107,3 +107,33 @@ def test_truncate(dim, base, scaling):
     assert factor == pytest.approx(wf, rel=1e-6) and len(want) == len(got)
     for i, (a, b) in enumerate(zip(got, want.tolist())):
         assert abs(a - b) <= 2.0 ** -24 * (16 * b + 8 * base ** (-2 * i / dim))
+
+
+@pytest.mark.parametrize("head,part", [(64, 0.5), (128, 0.25), (80, 0.4), (96, 1.0)])
+@pytest.mark.parametrize("scaling", [dict(rope_type="default"), LLAMA3, YARN, dict(rope_type="linear", factor=4.0)])
+def test_part_of_a_head(head, part, scaling):
+    """A configuration's partial_rotary_factor says how many channels turn, as in transformers."""
+    scaling = dict(scaling, partial_rotary_factor=part, rope_theta=500000.0)
+    n = rotary_channels(head, None, scaling)
+    assert n == int(head * part) == rotary_channels(head, n, scaling)
+    got, _ = rope_frequencies(n, scaling=scaling)
+    if scaling["rope_type"] == "default":
+        want = [500000.0 ** (-2 * i / n) for i in range(n // 2)]
+    else:
+        from transformers import LlamaConfig
+        from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+        cfg = LlamaConfig(hidden_size=head, num_attention_heads=1, head_dim=head, max_position_embeddings=131072, rope_parameters=scaling)
+        want = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")[0].tolist()
+    assert len(want) == len(got) == n // 2
+    for a, b in zip(got, want):
+        assert a == pytest.approx(b, rel=16 * 2.0 ** -24)
+    for other in (n - 2, n + 2):
+        with pytest.raises(_lib.StarKVError):
+            rope.Rope(head, rotary_dim=other, scaling=scaling)
+
+
+@pytest.mark.parametrize("part", [0.0, -0.5, 1.5, float("nan"), 0.02, 0.4])
+def test_part_of_a_head_refusals(part):
+    """Outside 0 to 1, or no even number of channels (1 and 25 of 64)."""
+    with pytest.raises(_lib.StarKVError):
+        rope.Rope(64, scaling=dict(rope_type="default", partial_rotary_factor=part))
