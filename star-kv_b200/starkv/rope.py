@@ -26,6 +26,12 @@ _STRIDES, _REST = struct.Struct("12q"), struct.Struct("2qPf10i4x")
 _ROPE = struct.Struct(f"4P{_STRIDES.size}sP{_REST.size}s")
 _MAX_PLANS = 64
 
+# What a scaling may hold: read below, or without a say in the angles of the types that are taken
+_SCALING_KEYS = frozenset((
+    "rope_type", "type", "rope_theta", "partial_rotary_factor", "factor", "low_freq_factor", "high_freq_factor",
+    "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim",
+    "short_factor", "long_factor", "max_position_embeddings", "finetuned"))
+
 
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None) -> Tuple[List[float], float]:
     """The angle per position of each of rotary_dim / 2 channel pairs, in 64 bits, and the factor of
@@ -36,8 +42,12 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
     high_freq_factor, original_max_position_embeddings) or "yarn" (factor,
     original_max_position_embeddings, beta_fast, beta_slow, truncate, attention_factor); a
     ``rope_theta`` in it is the base; of a ``partial_rotary_factor`` rotary_dim is the outcome (``Rope``
-    works it out)."""
-    s = dict(scaling or {})
+    works it out).  Entries of None count as absent, unknown ones (sections of several positions, a
+    dictionary for each kind of layer) are refused."""
+    s = {name: value for name, value in (scaling or {}).items() if value is not None or name == "truncate"}
+    unknown = sorted(map(str, s.keys() - _SCALING_KEYS))
+    if unknown:
+        raise StarKVError(f"scaling entries that are not understood: {', '.join(unknown)}")
     base = float(s.get("rope_theta", base))
     kind = s.get("rope_type", s.get("type", "default"))
     if rotary_dim <= 0 or rotary_dim % 2 or not base > 0 or base == 1.0 or not math.isfinite(base):
@@ -51,7 +61,7 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
         return float(value)
 
     f = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-    if kind in ("default", None):
+    if kind == "default":
         return f, 1.0
     factor = number("factor")
     if kind == "linear":

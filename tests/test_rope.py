@@ -137,3 +137,22 @@ def test_part_of_a_head_refusals(part):
     """Outside 0 to 1, or no even number of channels (1 and 25 of 64)."""
     with pytest.raises(_lib.StarKVError):
         rope.Rope(64, scaling=dict(rope_type="default", partial_rotary_factor=part))
+
+
+@pytest.mark.parametrize("extra", [dict(mrope_section=[8, 12, 12]), dict(llama_4_scaling_beta=0.1), dict(some_new_factor=2.0)])
+@pytest.mark.parametrize("scaling", [dict(rope_type="default"), LLAMA3, YARN])
+def test_unknown_entries_are_refused(scaling, extra):
+    with pytest.raises(_lib.StarKVError):
+        rope_frequencies(64, 10000.0, dict(scaling, **extra))
+    # a dictionary for each kind of layer is not one
+    with pytest.raises(_lib.StarKVError):
+        rope_frequencies(64, 10000.0, dict(full_attention=scaling, sliding_attention=dict(rope_type="default")))
+
+
+def test_entries_without_a_say():
+    """None counts as absent; what other types read, and notes, change nothing (nor do they in transformers)."""
+    plain = rope_frequencies(64, 10000.0, YARN)
+    assert rope_frequencies(64, 10000.0, dict(YARN, finetuned=True, max_position_embeddings=131072, low_freq_factor=2.0, some_new_factor=None,
+                                              rope_theta=None, attention_factor=None, beta_fast=None)) == plain
+    assert rope_frequencies(64, 10000.0, dict({k: v for k, v in YARN.items() if k != "rope_type"}, rope_type=None, type="yarn")) == plain
+    assert rope_frequencies(64, 10000.0, dict(rope_type=None, factor=4.0)) == rope_frequencies(64)
