@@ -92,6 +92,26 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[d
     raise StarKVError(f"unknown rope_type {kind!r}")
 
 
+class _Turn(torch.autograd.Function):
+    """The turn is linear and its transpose is the inverse turn with the same factor, so the gradients
+    of q and k are those of the outputs turned back; recorded again where they need gradients."""
+
+    @staticmethod
+    def forward(ctx, rope, inverse, positions, q, k):
+        ctx.rope, ctx.inverse = rope, inverse
+        ctx.save_for_backward(positions)             # autograd refuses positions that were written since
+        return rope._turn(q, k, positions, inverse, None)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, = ctx.saved_tensors
+        # a gradient may be repeated elements (that of a sum); channels have to follow one another
+        sides = [g if g.stride(-1) == 1 else g.contiguous() for g, needed in zip(grads, ctx.needs_input_grad[3:]) if needed]
+        back = ctx.rope.apply(sides[0], sides[1] if len(sides) == 2 else None, positions, inverse=not ctx.inverse)
+        found = iter(back if len(sides) == 2 else (back,))
+        return (None, None, None, *(next(found) if needed else None for needed in ctx.needs_input_grad[3:]))
+
+
 def rotary_channels(head_dim: int, rotary_dim: Optional[int] = None, scaling: Optional[dict] = None) -> int:
     """How many channels of a head turn: ``rotary_dim``, or the part of head_dim that scaling's
     ``partial_rotary_factor`` says, or all."""
@@ -187,8 +207,19 @@ class Rope:
         head_dim) for packed prompts, fp32, fp16 or bf16, any strides whose channels are
         contiguous; positions int32 or int64 of the leading shape, or (T,) for every
         sequence, on the GPU.  ``inverse`` turns back (what was turned by the same
-        positions; nothing is recorded for autograd, whose backward is this of the gradients).  Returns new tensors, or writes ``out`` (a tensor, or a
-        pair with k), which may be the inputs themselves.  Without k (None) one tensor."""
+        positions).  Returns new tensors, or writes ``out`` (a tensor, or a
+        pair with k), which may be the inputs themselves.  Without k (None) one tensor.
+        Where q or k needs a gradient autograd records the call, and ``out`` is refused."""
+        if torch.is_grad_enabled():
+            needs = q.requires_grad or k is not None and k.requires_grad
+            if out is None:
+                if needs:
+                    return _Turn.apply(self, inverse, positions, q, k)
+            elif needs or any(o.requires_grad for o in (out if isinstance(out, (tuple, list)) else (out,))):
+                raise StarKVError("out is for tensors without a gradient; without it new ones are recorded")
+        return self._turn(q, k, positions, inverse, out)
+
+    def _turn(self, q, k, positions, inverse, out):
         key = None
         if k is not None and (out is None or type(out) is tuple and len(out) == 2 and out[0] is q and out[1] is k):
             key = (q.shape, q.stride(), k.shape, k.stride(), positions.shape, positions.stride(), q.dtype, k.dtype,
@@ -260,7 +291,6 @@ class Rope:
                 rc = self._fn(a, _stream_of(self._index))
         if rc:
             check(rc, "starkv_rope")
-
 
     def _new(self, x: torch.Tensor, lead):
         """A contiguous tensor of x's shape and its strides (empty_like, which is cheaper, keeps x's order)."""

@@ -236,3 +236,69 @@ def test_part_of_a_head_from_the_scaling(cuda):
     got = rope.apply(q, None, pos)
     close(got, *reference(rope, q, pos))
     assert torch.equal(got[..., 32:], q[..., 32:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("needs", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("kw", [dict(), dict(interleaved=True, rotary_dim=64, scaling=YARN)])
+def test_gradients(cuda, dtype, needs, kw):
+    """Against the formula: the transposed map, that is the inverse turn, with one rounding."""
+    rope = Rope(128, **kw)
+    x = [make((2, 5, h, 128), dtype, h).requires_grad_(n) for h, n in zip((4, 2), needs)]
+    pos = torch.tensor([[0, 3, 77, 5, 9], [1, 2, 3, 4, 100000]], device=cuda)
+    for inverse in (False, True):
+        got = rope.apply(*x, pos, inverse=inverse)
+        with torch.no_grad():
+            plain = rope.apply(*x, pos, inverse=inverse)
+        assert all(torch.equal(a, b) for a, b in zip(got, plain)) and not any(b.requires_grad for b in plain)
+        assert got[0].grad_fn is not None and got[1].grad_fn is got[0].grad_fn
+        up = [make(t.shape, dtype, 7 + i) for i, t in enumerate(got)]
+        sides = [i for i in (0, 1) if needs[i]]
+        grads = torch.autograd.grad(got, [x[i] for i in sides], up)
+        for i, g in zip(sides, grads):
+            close(g, *reference(rope, up[i], pos, inverse=not inverse))
+    # one side, and a gradient that is one repeated number
+    if needs[0]:
+        g, = torch.autograd.grad(rope.apply(x[0], None, pos).sum(), x[0])
+        close(g, *reference(rope, torch.ones_like(g), pos, inverse=True))
+
+
+def test_gradients_by_differences(cuda):
+    """The map is linear: the difference of two calls is the derivative along their distance, but for
+    the calls' own errors (2^-20 of some values of one to eight, 9 * 3 * 128 of them times |up|)."""
+    rope = Rope(128, scaling=YARN)
+    x, d, up = (make((9, 3, 128), torch.float32, i) for i in range(3))
+    pos = torch.arange(9, device=cuda) * 311
+    x.requires_grad_()
+    y = rope.apply(x, None, pos)
+    g, = torch.autograd.grad(y, x, up, create_graph=True)
+    with torch.no_grad():
+        want = (up.double() * (rope.apply(x + d, None, pos).double() - y.double())).sum()
+    assert abs(float((g.detach().double() * d.double()).sum() - want)) < 9 * 3 * 128 * 2.0 ** -18
+    # the gradient's gradient: of <g, d> by up, the turned d
+    up2 = up.clone().requires_grad_()
+    g, = torch.autograd.grad(rope.apply(x, None, pos), x, up2, create_graph=True)
+    back, = torch.autograd.grad(g, up2, d)
+    close(back, *reference(rope, d, pos))
+
+
+def test_gradient_refusals(cuda):
+    rope = Rope(128)
+    q, k, pos = make((3, 4, 128), torch.float32), make((3, 2, 128), torch.float32, 1), torch.arange(3, device=cuda)
+    leaf = q.clone().requires_grad_()
+    before = k.clone()
+    for bad in (lambda: rope.apply(leaf, k, pos, out=(leaf, k)), lambda: rope.apply(k, leaf, pos, out=(k, leaf)),
+                lambda: rope.apply(leaf, None, pos, out=torch.empty_like(q)), lambda: rope.apply(q, None, pos, out=torch.empty_like(leaf).requires_grad_()),
+                lambda: rope.apply(k, leaf * 1, pos, out=[k, torch.empty_like(q)])):
+        with pytest.raises(StarKVError):
+            bad()
+    assert torch.equal(k, before) and torch.equal(leaf.detach(), q)
+    with torch.no_grad():                                                  # nothing is recorded: in place as asked
+        want = rope.apply(leaf, None, pos)
+        assert torch.equal(rope.apply(leaf, None, pos, out=leaf), want)
+    # positions that were written in between are not those of the call
+    leaf = q.clone().requires_grad_()
+    y = rope.apply(leaf, k, pos)
+    pos.add_(1)
+    with pytest.raises(RuntimeError):
+        y[0].sum().backward()
