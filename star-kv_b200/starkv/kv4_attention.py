@@ -251,7 +251,8 @@ class KV4Attention(nn.Module):
         if self.rope is not None:
             q = self.q_proj(x).view(B, T, self.num_heads, 128)
             k = self.k_proj(x).view(B, T, self.num_key_value_heads, 128)
-            q, k = self.rope.apply(q, k, positions, out=None if q.requires_grad else (q, k))
+            # into new tensors: a projection's output may be held by others (a forward hook, autograd)
+            q, k = self.rope.apply(q, k, positions)
             return q, k, self.v_proj(x).view(B, T, self.num_key_value_heads, 128)
         q = self.q_proj(x).view(B, T, self.num_heads, 128).transpose(1, 2)
         k = self.k_proj(x).view(B, T, self.num_key_value_heads, 128).transpose(1, 2)

@@ -210,3 +210,63 @@ def test_join_attention(cuda):
     got = join_attention(a, la, b, lb)
     for i, want in enumerate(((a[0] + b[0]) / 2, b[1], a[2], 0 * a[3], a[4])):
         assert torch.allclose(got[i], want, rtol=2.0 ** -20, atol=0)
+
+
+def module(dtype=torch.float16, seed=3, **kw):
+    torch.manual_seed(seed)
+    m = KV4Attention(Config(), layer_idx=0, **kw).to("cuda", dtype)
+    for p in m.parameters():
+        p.data.normal_(0, 0.05)
+    return m
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_projections_are_not_written_over(cuda, T):
+    """A forward hook that keeps a projection's output has it as it was."""
+    m = module(rope=Rope(128))
+    kept = []
+    for proj in (m.q_proj, m.k_proj):
+        proj.register_forward_hook(lambda mod, args, out: kept.append((out, out.clone())))
+    cache = StarKVCache(100)
+    m(make((2, 30, 1024), torch.float16, 1), None, None, past_key_values=cache)
+    m(make((2, T, 1024), torch.float16, 2), None, None, past_key_values=cache)
+    assert len(kept) == 4 and all(torch.equal(a, b) for a, b in kept)
+
+
+@pytest.mark.parametrize("train", ["all", "keys"])
+def test_projections_get_their_gradients(cuda, train):
+    """A piece behind a history (which goes through torch's attention) with the kernel's positions,
+    against the same in 64 bits from the history that the cache reads back."""
+    m = module(rope=Rope(128))
+    for name, p in m.named_parameters():
+        p.requires_grad_(train == "all" or name.startswith("k_proj"))
+    B, P, T = 2, 37, 20
+    cache = StarKVCache(P + T)
+    with torch.no_grad():
+        m(make((B, P, 1024), torch.float16, 1), None, None, past_key_values=cache)
+    x, up = make((B, T, 1024), torch.float16, 2), make((B, T, 1024), torch.float16, 4)
+    hk, hv = (t.double() for t in cache.kv4_states[0].history(torch.float32))
+    y, _ = m(x, None, None, past_key_values=cache)
+    y.backward(up)
+    w = {n: p.detach().double().requires_grad_() for n, p in m.named_parameters()}
+    heads = lambda n: (x.double() @ w[n + ".weight"].T).view(B, T, -1, 128)  # noqa: E731
+    f = torch.tensor(m.rope.frequencies, dtype=torch.float64, device=cuda)
+    angle = (torch.arange(P, P + T, device=cuda).double()[:, None] * f)[:, None]
+
+    def turn(t):
+        a, b = t[..., :64], t[..., 64:]
+        return torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1)
+
+    k, v = torch.cat([hk, turn(heads("k_proj"))], 1), torch.cat([hv, heads("v_proj")], 1)
+    s = torch.einsum("bihd,bjhd->bhij", turn(heads("q_proj")), k.repeat_interleave(4, 2)) * m.scaling
+    s = s.masked_fill(~torch.ones(T, P + T, dtype=torch.bool, device=cuda).tril(P), -math.inf)
+    o = torch.einsum("bhij,bjhd->bihd", s.softmax(-1), v.repeat_interleave(4, 2)).reshape(B, T, -1)
+    (o @ w["o_proj.weight"].T).backward(up.double())
+    for n, p in m.named_parameters():
+        if p.requires_grad:
+            # eight roundings of 2^-11 one after the other (projections, turn, scores, weights, outputs, gradients of
+            # each); they are independent over the sums that a gradient is, so of its norm at most that
+            assert rel(p.grad, w[n].grad) <= 8 * 2.0 ** -11, n
+        else:
+            assert p.grad is None
