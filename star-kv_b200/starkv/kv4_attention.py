@@ -51,6 +51,16 @@ def causal_rows(mask: torch.Tensor, n: int) -> bool:
     return bool(torch.where(seen, rows == rows[:, -1:], rows <= low).all())
 
 
+def only_causal(mask: torch.Tensor, T: int, n: int) -> bool:
+    """Whether mask (B or 1, 1, T, >= n), of several tokens, drops the positions behind each token and
+    does nothing else, as what a model makes for tokens behind a history.  Synchronises; under graph
+    capture, which cannot ask what a mask holds, none counts as such."""
+    if mask.dim() != 4 or mask.shape[1] != 1 or not mask.shape[2] == T > 1 or mask.shape[3] < n or \
+            torch.cuda.is_current_stream_capturing():
+        return False
+    return causal_rows(mask, n) and not bool(additive_mask(mask[:, 0, -1, :n]).any())
+
+
 class KV4State:
     """One layer's pages of a fixed batch: sequence b owns ``pages_per_sequence``
     consecutive pages of the pool.  ``lengths`` (int32, on the GPU) is what the kernels
@@ -272,8 +282,8 @@ class KV4Attention(nn.Module):
             position_ids = torch.arange(before, before + T, device=hidden_states.device)
         q, k, v = self.heads(hidden_states, *(position_embeddings or (None, None)), position_ids)
         if isinstance(st, KV4Branches):
-            if attention_mask is not None:
-                raise NotImplementedError("branches take no mask")
+            if attention_mask is not None and not only_causal(attention_mask, T, before + T):
+                raise NotImplementedError("branches take no mask but one that says no more than causality")
             if T > MAX_DRAFT:
                 out = st.attend_piece(q, k, v, self.scaling)
                 st.append(k, v)

@@ -270,3 +270,66 @@ def test_projections_get_their_gradients(cuda, train):
             assert rel(p.grad, w[n].grad) <= 8 * 2.0 ** -11, n
         else:
             assert p.grad is None
+
+
+def masks_of(B, T, n):
+    """A causal mask of the newest T of n tokens in the forms that models make."""
+    seen = torch.ones(T, n, dtype=torch.bool, device="cuda").tril(n - T).expand(B, 1, T, n)
+    for low in (-math.inf, torch.finfo(torch.float16).min):
+        yield torch.zeros(seen.shape, dtype=torch.float16, device="cuda").masked_fill(~seen, low)
+    yield seen
+    yield torch.nn.functional.pad(seen[:1].long(), (0, 5))                  # wider than what is held
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("T", [2, 16, 17, 40])
+def test_branches_take_causal_masks(cuda, T):
+    m, B, P = module(rope=Rope(128)), 3, 90
+    one = StarKVCache(P)
+    m(make((1, P, 1024), torch.float16, 1), None, None, past_key_values=one)
+    x, first = make((B, T, 1024), torch.float16, 2), make((B, 1, 1024), torch.float16, 5)
+
+    def run(mask):
+        cache = one.branch(B, 60)
+        m(first, None, None, past_key_values=cache)
+        return m(x, None, mask, past_key_values=cache)[0]
+
+    want = run(None)
+    for mask in masks_of(B, T, P + 1 + T):
+        assert torch.equal(run(mask), want)
+    # what a mask says beyond causality is refused, and nothing is written
+    for at, value in (((0, 0, T - 1, 3), False), ((1, 0, 0, P), False), ((2, 0, 0, P + 2), True)):
+        mask = torch.ones(T, P + 1 + T, dtype=torch.bool, device=cuda).tril(P + 1).expand(B, 1, -1, -1).clone()
+        mask[at] = value
+        cache = one.branch(B, 60)
+        m(first, None, None, past_key_values=cache)
+        for bad in (mask, mask[..., :-1], torch.cat([mask, mask], 1), mask[:, :, 1:]):
+            with pytest.raises(NotImplementedError):
+                m(x, None, bad, past_key_values=cache)
+        assert cache.get_seq_length() == P + 1 and torch.equal(m(x, None, None, past_key_values=cache)[0], want)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("attention", ["sdpa", "eager"])
+def test_branches_through_a_transformers_model(cuda, attention):
+    """Tokens, drafts and longer pieces of branches by the model's own forward, which makes the masks,
+    against the layers called one by one."""
+    kw = dict(num_layers=2, hidden=512, heads=4, kv_heads=2, mlp=1024, vocab=1000, v_block_kv=2, quantized=False, seed=3, device=cuda,
+              max_positions=1024, kv4_layers=range(2), kernel_rope=True)
+    model = build_model(**kw)
+    model.config._attn_implementation = attention
+    g = torch.Generator(device=cuda).manual_seed(1)
+    prompt = torch.randint(0, 1000, (1, 300), generator=g, device=cuda)
+    one = StarKVCache(300, quantized=False)
+    forward_tokens(model, prompt, 0, one)
+    by_hand, by_model = one.branch(4, 70), one.branch(4, 70)
+    at = 300
+    for T in (3, 40, 5) if attention == "eager" else (1, 3, 40, 1, 16):
+        ids = torch.randint(0, 1000, (4, T), generator=g, device=cuda)
+        want = forward_tokens(model, ids, at, by_hand)
+        pos = torch.arange(at, at + T, device=cuda)[None]
+        got = model(input_ids=ids, position_ids=pos, past_key_values=by_model, use_cache=True).logits[:, -1]
+        # the same kernels on the same numbers, but for the model's own fp16 tables of sines, which are not used
+        assert torch.equal(got, want), T
+        at += T
+        assert by_model.get_seq_length() == by_hand.get_seq_length() == at
