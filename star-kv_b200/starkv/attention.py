@@ -127,7 +127,11 @@ class StarKVCache(_HFCache):
                 st.crop(keep)
 
     def reset(self) -> None:
-        self.crop(0)
+        """Forgets all tokens; of branches the shared ones too."""
+        for st in self.states.values():
+            st.crop(0)
+        for st in self.kv4_states.values():
+            st.reset()
 
     def branch(self, branches: int, capacity: int) -> "StarKVCache":
         """A cache of ``branches`` sequences that continue the one this holds, each with room for

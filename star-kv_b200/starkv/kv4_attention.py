@@ -86,6 +86,10 @@ class KV4State:
         self.lengths.fill_(length)
         self.length = length
 
+    def reset(self) -> None:
+        """Forgets all tokens."""
+        self.crop(0)
+
     def select(self, q: torch.Tensor, keep_pages: int, mask: Optional[torch.Tensor] = None,
                newest: Optional[int] = None) -> torch.Tensor:
         """The pages (``KV4Cache.select``) of queries q (B, T, Hq, 128) among the ``newest``
@@ -176,6 +180,12 @@ class KV4Branches(KV4State):
             raise ValueError("the shared prefix stays")
         self.lengths.fill_(length - self.shared)
         self.length = length
+
+    def reset(self) -> None:
+        """Forgets all tokens, the prefix too: sequences of ``capacity`` tokens that share none."""
+        self.prefix_length.zero_()
+        self.lengths.zero_()
+        self.shared = self.length = 0
 
     def select(self, *args, **kwargs):
         raise NotImplementedError("branches attend to all pages")

@@ -333,3 +333,33 @@ def test_branches_through_a_transformers_model(cuda, attention):
         assert torch.equal(got, want), T
         at += T
         assert by_model.get_seq_length() == by_hand.get_seq_length() == at
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("first", [1, 16, 40])
+def test_reset_of_branches(cuda, first):
+    """After reset branches are sequences that share nothing: as a new cache of theirs, from the first
+    token on."""
+    m, B = module(rope=Rope(128)), 3
+    one = StarKVCache(70)
+    m(make((1, 70, 1024), torch.float16, 1), None, None, past_key_values=one)
+    cache = one.branch(B, 64)
+    m(make((B, 5, 1024), torch.float16, 2), None, None, past_key_values=cache)
+    for _ in range(2):
+        cache.reset()
+        assert cache.get_seq_length() == 0
+        new = StarKVCache(64)
+        for i, T in enumerate((first, 1, 7, 1)):
+            x = make((B, T, 1024), torch.float16, 10 + i)
+            got, want = (m(x, None, None, past_key_values=c)[0] for c in (cache, new))
+            # (of a first piece of up to 16 tokens, one attends to its own tokens' 4-bit heads and the other to exact ones)
+            assert i == 0 and 1 < first <= 16 or rel(got, want) < 5e-3, T
+            assert cache.get_seq_length() == new.get_seq_length()
+        cache.crop(first + 1)
+        assert cache.get_seq_length() == first + 1
+        with pytest.raises(ValueError):
+            m(make((B, 64, 1024), torch.float16, 9), None, None, past_key_values=cache)
+    # the cache it came from is as it was
+    assert one.get_seq_length() == 70
+    one.reset()
+    assert one.get_seq_length() == 0
