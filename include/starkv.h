@@ -544,7 +544,8 @@ typedef struct starkv_packed_args {
   void* workspace;            /* starkv_packed_workspace_size bytes, 16-byte aligned, the first 4096 zeroed before its first
                                  use (each call leaves them zero).  One call at a time may use it. */
   size_t workspace_bytes;
-  int* error_word;            /* device int that a bad range or a timed-out wait sets, or NULL */
+  int* error_word;            /* device int that a bad range or a timed-out wait sets; NULL: the current device's own word,
+                                 which starkv_packed_read_error reads */
   int64_t total_q;
   int64_t total_k;
   float scaling;              /* positive */
@@ -558,6 +559,9 @@ typedef struct starkv_packed_args {
 
 int starkv_packed_workspace_size(size_t* bytes);
 int starkv_packed_attention(const starkv_packed_args* args, starkv_stream_t stream);
+/* Reads and clears the current device's word of calls without an error_word (synchronises the stream, which
+ * is to come after theirs); *out_code = 0 means that none of them failed. */
+int starkv_packed_read_error(int* out_code, starkv_stream_t stream);
 
 /* sizeof of starkv_rope_args (0) and starkv_packed_args (1) (ABI check for bindings). */
 size_t starkv_args_size(int32_t which);

@@ -30,6 +30,22 @@ int rows_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int he
   return rc == CUDA_SUCCESS ? STARKV_OK : host_error(STARKV_ERR_INVALID, "q / k / v cannot be described by a tensor map");
 }
 
+// Where calls without an error word of their own report: one word a device, looked up once with that
+// device current.
+__device__ int g_packed_error;
+int packed_error(int** word) {
+  static std::atomic<int*> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return host_launch_status();
+  *word = dev < 64 ? known[dev].load(std::memory_order_relaxed) : nullptr;
+  if (*word) return STARKV_OK;
+  void* found = nullptr;
+  if (cudaGetSymbolAddress(&found, g_packed_error) != cudaSuccess) return host_launch_status();
+  *word = reinterpret_cast<int*>(found);
+  if (dev < 64) known[dev].store(*word, std::memory_order_relaxed);
+  return STARKV_OK;
+}
+
 template <typename T>
 int launch_packed(const PackedParams& p, int grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
                   cudaStream_t st) {
@@ -62,6 +78,14 @@ int starkv_packed_workspace_size(size_t* bytes) {
   if (!bytes) return host_error(STARKV_ERR_INVALID, "null argument");
   *bytes = kPkWorkspaceBytes;
   return STARKV_OK;
+}
+
+int starkv_packed_read_error(int* out_code, starkv_stream_t stream) {
+  if (!out_code) return host_error(STARKV_ERR_INVALID, "null argument");
+  int* word = nullptr;
+  int rc = host_device(nullptr);
+  if (rc || (rc = packed_error(&word))) return rc;
+  return starkv_read_device_error(word, out_code, stream);
 }
 
 int starkv_packed_attention(const starkv_packed_args* a, starkv_stream_t stream) {
@@ -119,7 +143,7 @@ int starkv_packed_attention(const starkv_packed_args* a, starkv_stream_t stream)
   const double pieces = ((double)a->total_q / (2 * p.tokens) + a->batch) * a->num_kv_heads;
   if (pieces > 1e8) return host_error(STARKV_ERR_UNSUPPORTED, "too many rows in one call");
   int sms = 0, rc = host_device(&sms);
-  if (rc) return rc;
+  if (rc || (!p.err && (rc = packed_error(&p.err)))) return rc;
   CUtensorMap tq, tk, tv;
   memset(&tk, 0, sizeof(tk));
   memset(&tv, 0, sizeof(tv));

@@ -189,6 +189,7 @@ SIGNATURES = [
     ("starkv_rope", C.c_int, [C.c_void_p, C.c_void_p]),
     ("starkv_packed_workspace_size", C.c_int, [C.POINTER(C.c_size_t)]),
     ("starkv_packed_attention", C.c_int, [C.c_void_p, C.c_void_p]),
+    ("starkv_packed_read_error", C.c_int, [C.POINTER(C.c_int), C.c_void_p]),
     ("starkv_args_size", C.c_size_t, [C.c_int32]),
     ("starkv_last_error", C.c_char_p, []),
 ]

@@ -213,7 +213,8 @@ class KV4Branches(KV4State):
         flat = q.reshape(B * T, Hq, 128)
         ends = lambda *n: torch.tensor([0, *n], dtype=torch.int32).cumsum(0).to(q.device, torch.int32, non_blocking=True)  # noqa: E731
         run = lambda kk, vv, cq, ck, causal: prefill.packed_attention(  # noqa: E731
-            flat, kk, vv, cq, ck, scaling, causal=causal, out=torch.empty(flat.shape, device=q.device), return_lse=True)
+            flat, kk, vv, cq, ck, scaling, causal=causal, out=torch.empty(flat.shape, device=q.device), return_lse=True,
+            error_word=self.cache.error_word)
         held = self.length - self.shared
         if held:
             k, v = (torch.cat(x, 1) for x in zip(self.history(k.dtype), (k, v)))

@@ -119,7 +119,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Ra
     and -inf.  Rows of no sequence stay as they are in an ``out`` that is given; in a new one
     they are 0 (-inf) where ranges are pairs, and undefined before cu_q[0] and from cu_q[batch]
     on.  error_word: int32 (1,), set to a code of ``kv4.ERRORS`` where ranges leave the tensors
-    (they are cut off there) or a copy never lands.  ws: scratch of one's own,
+    (they are cut off there) or a copy never lands; without it the device has one, which
+    ``read_packed_error`` reads.  ws: scratch of one's own,
     ``starkv_packed_workspace_size`` bytes, its first 4096 zeroed before its first use (each
     call leaves them zero)."""
     index = q.get_device()
@@ -170,3 +171,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: Ra
     if rc:
         check(rc, "starkv_packed_attention")
     return (out, lse) if return_lse else out
+
+
+def read_packed_error(device="cuda") -> int:
+    """Read and clear the device's error word of ``packed_attention`` calls that were given none, behind
+    what the current stream holds (synchronises): 0, or a code of ``kv4.ERRORS``."""
+    code = C.c_int(0)
+    with torch.cuda.device(torch.device(device)):
+        check(load().starkv_packed_read_error(C.byref(code), torch.cuda.current_stream().cuda_stream), "starkv_packed_read_error")
+    return int(code.value)

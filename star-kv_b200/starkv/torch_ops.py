@@ -8,7 +8,8 @@
     torch.ops.starkv.kv4_read      4-bit pages back to whole heads (starkv_kv4_read)
     torch.ops.starkv.kv4_attn      attention over 4-bit pages, with its log-sum-exp (starkv_kv4_attention)
     torch.ops.starkv.kv4_attn_shared   the same behind one prefix (starkv_kv4_shared_attention)
-    torch.ops.starkv.packed_attn   attention of packed sequences, with its log-sum-exp (starkv_packed_attention)
+    torch.ops.starkv.packed_attn   attention of packed sequences, with its log-sum-exp (starkv_packed_attention;
+                                   errors to prefill.read_packed_error)
     torch.ops.starkv.rope          rotary positions of queries and keys (starkv_rope)
     torch.ops.starkv.kv4_select    the pages a score bound keeps (starkv_kv4_select)
 

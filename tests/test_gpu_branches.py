@@ -363,3 +363,36 @@ def test_reset_of_branches(cuda, first):
     assert one.get_seq_length() == 70
     one.reset()
     assert one.get_seq_length() == 0
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("own", [0, 3])
+def test_pieces_of_branches_report_errors(cuda, own):
+    """A wait that runs out in a longer piece's attention, behind the prompt or among the own tokens, is in
+    the layer's error word; the next piece is what it was."""
+    from starkv import ops
+    m, B, P, T = module(rope=Rope(128)), 3, 2000, 40
+    one = StarKVCache(P)
+    m(make((1, P, 1024), torch.float16, 1), None, None, past_key_values=one)
+    x = make((B, T, 1024), torch.float16, 2)
+
+    def run():
+        cache = one.branch(B, 60)
+        if own:
+            m(make((B, own, 1024), torch.float16, 3), None, None, past_key_values=cache)
+        return cache.kv4_states[0].cache, m(x, None, None, past_key_values=cache)[0]
+
+    pool, want = run()
+    assert pool.read_error() == 0
+    try:
+        cache = one.branch(B, 60)
+        if own:
+            m(make((B, own, 1024), torch.float16, 3), None, None, past_key_values=cache)
+        ops.set_test_hooks(wait_limit_ns=20_000_000, skip_copy_unit=1)
+        m(x, None, None, past_key_values=cache)
+        assert cache.kv4_states[0].cache.read_error() in (0x101, 0x102)
+    finally:
+        ops.set_test_hooks()
+    for _ in range(2):
+        pool, got = run()
+        assert pool.read_error() == 0 and torch.equal(got, want)

@@ -346,3 +346,34 @@ def test_ends_far_below_zero(cuda, batch):
             close(out[live], None, want, torch.float16, 2)
             # without queries rows are left alone, without keys they are 0
             assert bool((out[~live] == (7.0 if which == "q" else 0.0)).all())
+
+
+def test_errors_of_calls_without_a_word(cuda):
+    """They are in the device's word: of the entry point, the torch.library op and a replayed graph; calls
+    with a word of their own leave it alone."""
+    from starkv import ops, torch_ops  # noqa: F401
+    from starkv.prefill import read_packed_error
+    q, k = make((20, 2, 128), torch.float16, 1), make((20, 1, 128), torch.float16, 2)
+    good, bad = cumulated([20]), cumulated([21])
+    read_packed_error()
+    want = packed_attention(q, k, k, good, good, SCALE)
+    assert read_packed_error() == 0
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for run in (lambda: packed_attention(q, k, k, bad, bad, SCALE), lambda: torch.ops.starkv.packed_attn(q, k, k, bad, bad, SCALE)[0]):
+        assert torch.equal(run(), want) and read_packed_error(q.device) == 0x203 and read_packed_error() == 0
+    packed_attention(q, k, k, bad, bad, SCALE, error_word=err)
+    assert int(err) == 0x203 and read_packed_error() == 0
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = packed_attention(q, k, k, good, good, SCALE)
+    for cu, code in (([20], 0), ([21], 0x203), ([20], 0)):
+        good.copy_(cumulated(cu))
+        g.replay()
+        assert torch.equal(out, want) and read_packed_error() == code
+    try:
+        ops.set_test_hooks(wait_limit_ns=20_000_000, skip_copy_unit=1)
+        packed_attention(q, k, k, good, good, SCALE)
+        assert read_packed_error() in (0x101, 0x102)
+    finally:
+        ops.set_test_hooks()
+    assert torch.equal(packed_attention(q, k, k, good, good, SCALE), want) and read_packed_error() == 0

@@ -48,6 +48,10 @@ def test_c_null():
     assert _lib.load().starkv_packed_workspace_size(None) == 1
 
 
+def test_c_read_error_null():
+    assert _lib.load().starkv_packed_read_error(None, None) == 1
+
+
 def test_no_cpu_path():
     q, cu = torch.zeros(4, 2, 128, dtype=torch.float16), torch.tensor([0, 4], dtype=torch.int32)
     with pytest.raises(StarKVError):
