@@ -377,3 +377,18 @@ def test_errors_of_calls_without_a_word(cuda):
     finally:
         ops.set_test_hooks()
     assert torch.equal(packed_attention(q, k, k, good, good, SCALE), want) and read_packed_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk", [([300, 40], [100, 0]), ([5, 700, 1], [0, 257, 3]), ([600], [599]), ([3], [0])])
+def test_rows_that_see_nothing_are_zero(cuda, dtype, causal, nq, nk):
+    """Exactly 0 and -inf, also into memory that held NaN."""
+    q, k, v = make((sum(nq), 4, 128), dtype), make((sum(nk), 2, 128), dtype, 1), make((sum(nk), 2, 128), dtype, 2)
+    for out_dtype in (dtype, torch.float32):
+        out = torch.full(q.shape, math.nan, dtype=out_dtype, device="cuda")
+        _, lse = packed_attention(q, k, v, cumulated(nq), cumulated(nk), SCALE, causal=causal, out=out, return_lse=True)
+        idle = torch.cat([torch.arange(n, device="cuda") < (n - m if causal else n if m == 0 else 0) for n, m in zip(nq, nk)])
+        assert bool(idle.any()) or not causal
+        assert torch.equal(out[idle], torch.zeros_like(out[idle])) and bool((lse[idle] == -math.inf).all())
+        assert bool(out[~idle].isfinite().all()) and bool(lse[~idle].isfinite().all())
