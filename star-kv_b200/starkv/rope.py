@@ -258,6 +258,9 @@ class Rope:
                 for a, b in ((oq, k), (ok, q), (oq, ok)):
                     if a.numel() and a.data_ptr() == b.data_ptr():
                         raise StarKVError("the two sides must be apart")
+                # (in place the two may lie between one another, as heads of a joint projection do)
+                if oq.data_ptr() != q.data_ptr() and _overlap(oq, k) or ok.data_ptr() != k.data_ptr() and _overlap(ok, q):
+                    raise StarKVError("an output that is not its input must be apart from the other side's too")
         wide = positions.dtype == torch.int64
         if positions.get_device() != self._index or not (wide or positions.dtype == torch.int32):
             raise StarKVError(f"positions must be int32 or int64 on {self.device}")

@@ -302,3 +302,27 @@ def test_gradient_refusals(cuda):
     pos.add_(1)
     with pytest.raises(RuntimeError):
         y[0].sum().backward()
+
+
+def test_an_output_over_the_other_side_is_refused(cuda):
+    rope = Rope(128)
+    buf = make((2, 6, 8, 128), torch.float16)
+    pos = torch.arange(6, device=cuda)
+    q, k = buf[0], make((6, 8, 128), torch.float16, 1)
+    for oq, ok in ((torch.empty_like(q), buf.view(-1)[128:128 + k.numel()].view(k.shape)),             # ok over q, a head on
+                   (torch.empty_like(q), buf.view(12, 8, 128)[5:11])):                                              # and by its last token
+        with pytest.raises(StarKVError):
+            rope.apply(q, k, pos, out=(oq, ok))
+        with pytest.raises(StarKVError):
+            rope.apply(k, q, pos, out=(ok, oq))
+    # behind the other side's input, into the two halves of one buffer, and in place between one another
+    a, b = rope.apply(q, k, pos)
+    ok = buf[1]
+    rope.apply(q, k, pos, out=(torch.empty_like(q), ok))
+    assert torch.equal(ok, b)
+    both = torch.empty(6, 16, 128, dtype=torch.float16, device=cuda)
+    rope.apply(q, k, pos, out=(both[:, :8], both[:, 8:]))
+    assert torch.equal(both[:, :8], a) and torch.equal(both[:, 8:], b)
+    both = torch.cat([q, k], 1)
+    rope.apply(both[:, :8], both[:, 8:], pos, out=(both[:, :8], both[:, 8:]))
+    assert torch.equal(both[:, :8], a) and torch.equal(both[:, 8:], b)
