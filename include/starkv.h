@@ -525,7 +525,8 @@ int starkv_rope(const starkv_rope_args* args, starkv_stream_t stream);
  * gets 0 and -inf.  Rows of out and lse that belong to no sequence are left as they were; a
  * row must not belong to two.  What k and v hold at keys that a query does not attend to, NaN
  * included, does not matter to it.  A query with a score that is NaN or +inf gets NaN.
- * Ranges that leave the tensors are cut off there and set the error word.
+ * Ranges that leave the tensors are cut off there and set the error word.  Where the same rows of q are
+ * given to so many sequences that pieces of work cannot be numbered, it is set too and nothing is done.
  */
 typedef struct starkv_packed_args {
   const void* q;

@@ -52,6 +52,9 @@ constexpr int kPkPartFloats = 2 * kPkTilePart;
 constexpr int kPkMaxCut = kPkMaxSlots / 2;       // cut pairs: each has two slots at least
 constexpr int kPkMinPiece = 4;                   // key tiles
 constexpr int kPkMost = 64;                     // keys whose weights go to the products ahead of the rest
+constexpr float kPkMaxThreadPieces = 5e6f;       // that a thread counts for the table of sequences
+static_assert(kPkMaxThreadPieces * kPkThreads < 2147483648.f, "the sum over threads");
+constexpr int kPkTooMany = 0x7fffffff;           // more: in the place of the longest sequence, which is below 2^30
 constexpr float kPkLazy = 5.f;
 // p is up to 2^(kPkBias + kPkLazy): the least fp16 weight is 2^-34 of the largest then.
 constexpr float kPkBias = 10.f;
@@ -600,12 +603,18 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     int s[3], before[3], most = 0;
     float units = 0.f;
     auto sums = [&](int limit) {
-      s[0] = s[1] = s[2] = 0;
+      s[0] = s[1] = s[2] = most = 0;
       units = 0.f;
       for (int e = e0; e < e1; ++e)
         for (int i = 0; i < in_entry(e); ++i) {
           const PkSeq q = sequence(e, i);
           const PkShape h = pk_shape(p, q, limit);
+          // Rows of one sequence each fit a GPU's memory a hundred times before a thread has this many pieces:
+          // the same rows were given to many.  The sums of 384 threads stay within 31 bits.
+          if ((float)s[0] + (float)h.tiles * h.splits * p.kv_heads > kPkMaxThreadPieces) {
+            most = kPkTooMany;
+            continue;
+          }
           s[0] += h.tiles * h.splits * p.kv_heads;
           if (h.splits > 1) s[1] += h.live * h.splits * p.kv_heads, s[2] += h.live * p.kv_heads;
           units += h.units * p.kv_heads;
@@ -649,14 +658,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     // pieces of half a CTA's share at most (four new pieces behind up to 16 K tokens and two single
     // tokens: 102 us with whole shares, 88 with two thirds, 84 with halves and thirds)
     int limit = max((int)fminf(units / (2.f * gridDim.x), 1e9f) + 1, kPkMinPiece);
-    if ((most + kPkKeys - 1) / kPkKeys > limit)
+    const bool crowded = most == kPkTooMany;
+    if (!crowded && (most + kPkKeys - 1) / kPkKeys > limit)
       for (;;) {
         sums(limit);
         scan();
-        if (s[1] <= kPkMaxSlots) break;
-        limit = limit < (1 << 28) ? limit + limit / 4 + 1 : limit;   // one piece each from 2^24 key tiles on, so this ends
+        if (s[1] <= kPkMaxSlots && most != kPkTooMany) break;
+        // one piece each from 2^24 key tiles on, so this ends; at once where cuts of idle tiles are too many
+        limit = most == kPkTooMany ? 1 << 28 : limit < (1 << 28) ? limit + limit / 4 + 1 : limit;
       }
-    for (int e = e0; e < e1; ++e) {
+    if (crowded) {                                     // nothing is done
+      if (tid == 0) record_error(p.err, kDevBadRange);
+      s[0] = s[2] = 0;
+    }
+    for (int e = crowded ? e1 : e0; e < e1; ++e) {
       sm.pre[e] = before[0], sm.slot_pre[e] = before[1], sm.counter_pre[e] = before[2];
       for (int i = 0; i < in_entry(e); ++i) {
         const PkShape h = pk_shape(p, sequence(e, i), limit);

@@ -392,3 +392,31 @@ def test_rows_that_see_nothing_are_zero(cuda, dtype, causal, nq, nk):
         assert bool(idle.any()) or not causal
         assert torch.equal(out[idle], torch.zeros_like(out[idle])) and bool((lse[idle] == -math.inf).all())
         assert bool(out[~idle].isfinite().all()) and bool(lse[~idle].isfinite().all())
+
+
+@pytest.mark.parametrize("kv_heads,batch", [(8, 4_000_000), (1, 30_000_000)])
+def test_rows_given_to_too_many_sequences(cuda, kv_heads, batch):
+    """All rows to every sequence: 128 pairs of tiles a KV head, 4e9 pieces of work, which 31 bits do not
+    number.  The call says so and leaves its outputs alone; the next one is as before."""
+    n = 128 * 256
+    q, k = make((n, kv_heads, 128), torch.float16), make((5, kv_heads, 128), torch.float16, 1)
+    good = packed_attention(q, k, k, cumulated([n]), cumulated([5]), SCALE, causal=False)
+    i = lambda x: torch.full((batch,), x, dtype=torch.int32, device="cuda")  # noqa: E731
+    out, err = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    packed_attention(q, k, k, (i(0), i(n)), (i(0), i(5)), SCALE, causal=False, out=out, error_word=err)
+    assert int(err) == 0x203 and bool((out == 7.0).all())
+    assert torch.equal(packed_attention(q, k, k, cumulated([n]), cumulated([5]), SCALE, causal=False, error_word=err), good)
+
+
+def test_many_idle_rows_beside_a_long_history(cuda):
+    """Two million queries with nothing to see beside cut histories."""
+    nq, nk = [2_000_000, 3, 1], [700, 40_000, 30_000]
+    q, k, v = make((sum(nq), 1, 128), torch.float16), make((sum(nk), 1, 128), torch.float16, 1), make((sum(nk), 1, 128), torch.float16, 2)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got, lse = packed_attention(q, k, v, cumulated(nq), cumulated(nk), SCALE, return_lse=True, error_word=err)
+    assert int(err) == 0
+    idle = nq[0] - nk[0]
+    assert not bool(got[:idle].any()) and bool((lse[:idle] == -math.inf).all())
+    live = torch.arange(idle, sum(nq), device="cuda")
+    want = reference(q[live], k, v, [(0, 700), (700, 703), (703, 704)], [(0, 700), (700, 40_700), (40_700, 70_700)])
+    close(got[live], lse[live], want, torch.float16, 40_000)
