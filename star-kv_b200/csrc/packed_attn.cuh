@@ -605,21 +605,20 @@ __global__ void __launch_bounds__(kPkThreads, 1)
     auto sums = [&](int limit) {
       s[0] = s[1] = s[2] = most = 0;
       units = 0.f;
+      float all = 0.f;
       for (int e = e0; e < e1; ++e)
         for (int i = 0; i < in_entry(e); ++i) {
           const PkSeq q = sequence(e, i);
           const PkShape h = pk_shape(p, q, limit);
-          // Rows of one sequence each fit a GPU's memory a hundred times before a thread has this many pieces:
-          // the same rows were given to many.  The sums of 384 threads stay within 31 bits.
-          if ((float)s[0] + (float)h.tiles * h.splits * p.kv_heads > kPkMaxThreadPieces) {
-            most = kPkTooMany;
-            continue;
-          }
           s[0] += h.tiles * h.splits * p.kv_heads;
+          all += (float)h.tiles * h.splits;
           if (h.splits > 1) s[1] += h.live * h.splits * p.kv_heads, s[2] += h.live * p.kv_heads;
           units += h.units * p.kv_heads;
           most = max(most, h.live ? q.kn : 0);
         }
+      // A thread has this many pieces only where the same rows were given to many sequences (rows of
+      // one sequence each would not fit a GPU's memory); up to there the sum of 384 threads has 31 bits.
+      if (all * p.kv_heads > kPkMaxThreadPieces) most = kPkTooMany;
     };
     auto scan = [&]() {
 #pragma unroll
