@@ -24,13 +24,16 @@
 // Rows.  Up to 128 rows a KV head: both tiles hold them, and take the even and the odd steps of 128
 // tokens.  More: tiles of 128 rows each, 256 a CTA, each block of 256 reads the prefix.
 // Bound: a step of 256 rows takes about 6100 cycles, of which the products need 3200.  Of a tile's turn
-// the rows' softmax is 3400 (S read twice, 80 registers, short loops), what is left its products
-// behind the other tile's; the codes are turned in less.  The warps share one instruction cache, so
+// the rows' softmax is 3600 (S read twice in short loops, as registers are few: the 25 warps are allotted
+// as 28, which leaves 72 a thread, and 204 bytes are spilled), the wait for its products behind the other
+// tile's 1700; the codes are turned in less.  Beside the steps a CTA takes about 46000 cycles: 3000 to
+// start, 27000 to lay out the queries (a thread reads a row of its own, twice), 9000 to the first
+// weights (instructions come in), 7000 for the parts and the end.  256 rows of 8 KV heads, 32769
+// tokens, 15 steps at most: 143000 cycles, 82 us, 404 TFLOP/s of products over 128 channels, 630 with the
+// parts of the exact keys.  The warps share one instruction cache, so
 // code is kept short rather than unrolled.  Measured and slower: seven warps for the codes and 192
 // registers for a row's softmax, bulk copies of the codes into shared memory, the next tile's codes in
-// registers ahead, a row's S in 64 registers (28 warps), loads of S ahead (spills: 127 us).  256 rows
-// of 8 KV heads, 32769 tokens: 85 us for this kernel, 404 TFLOP/s of products over 128 channels, 630
-// with the parts of the exact keys.
+// registers ahead, a row's S in 64 registers (28 warps), loads of S ahead (spills: 127 us).
 // Work.  A KV head and block of rows is cut into equal ranges of the prefix so that there is a piece
 // for every SM; a second kernel adds the parts in order, the own tokens' part last.
 #pragma once
@@ -39,7 +42,7 @@
 
 namespace starkv {
 
-constexpr int kKvpThreads = 25 * 32;                         // of 80 registers
+constexpr int kKvpThreads = 25 * 32;                         // of 72 registers
 constexpr int kKvpMaxParts = 2 * kKv4MaxGrid;                // tile parts in the workspace
 constexpr int kKvpMinPiece = 2;                              // steps of 128 tokens a piece has at least
 constexpr size_t kKvpPartBytes = (size_t)kKvpMaxParts * kPkTilePart * sizeof(float);

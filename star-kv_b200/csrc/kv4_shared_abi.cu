@@ -12,9 +12,16 @@ using namespace starkv;
 
 namespace {
 
-// Rows a KV head up to which the decode kernel takes the prefix (its columns are 16).  Both ways, back to
-// back, 16 rows: 32 KV heads, 16384 tokens 72 us and on the tensor cores 107; 8 KV heads, 777 tokens 35
-// and 37.
+// Rows a KV head up to which the decode kernel takes the prefix (its columns are 16).  Both ways, us in a
+// graph, decode kernel and tensor cores, own 40:
+//                      777 tokens   4096        16384       65536       131072
+//    4 rows,  1 head    25  31     27  33      31  45      35  66      37  70
+//    4 rows,  8 heads   29  36     31  37      35  47      46  92      66  158
+//   16 rows,  1 head    35  35     37  35      46  47      58  68      62  74
+//   16 rows,  4 heads   36  36     39  37      49  45      60  66      71  98
+//   16 rows,  8 heads   37  37     39  37      49  47      70  98      98  156
+//   16 rows, 32 heads   41  41     45  49      67  102
+// The tensor cores gain up to 4 us in between and lose far more at both ends.
 constexpr int kDecodeRows = 16;
 
 size_t up(size_t n) { return (n + 255) & ~(size_t)255; }

@@ -66,7 +66,7 @@ int launch_packed(const PackedParams& p, int grid, const CUtensorMap& q, const C
   const int rc = host_launch_status();
   // too few keys for any to be cut
   if (rc || p.total_k <= kPkMinPiece * kPkKeys) return rc;
-  packed_join_kernel<<<4 * grid, 128, 0, st>>>(p);
+  packed_join_kernel<8><<<4 * grid, 128, 0, st>>>(p);
   return host_launch_status();
 }
 

@@ -382,8 +382,8 @@ __device__ __forceinline__ void pk_store16x64(void* base, const int64_t* dst, in
 // Whole rows of a warp: out = O / l.  Sixteen rows at a time, four lanes a row: lane l holds rows l / 4
 // (the first two values of four) and l / 4 + 8, so that a store writes 64 bytes in eight places (16 in
 // 32 with a lane a row).  About 5600 cycles for a pair of tiles, in which no products run: what most
-// of the gap to the floor is where a piece has few key tiles (24 mixed prompts: 247 us; 262 with a
-// lane's conversions to both types and exchanges of one row after the other).  Values that are not
+// of the gap to the floor is where a piece has few key tiles (24 mixed prompts, in a graph: 246 us; 262
+// with a lane's conversions to both types and exchanges of one row after the other).  Values that are not
 // finite are added first, a lane a row, into tensor memory (the 0 that stands for them made them 0).
 template <typename T>
 __device__ __noinline__ void pk_finish(const PackedParams& p, const PkItem& it, PkPlace at, uint32_t o_col, int nx, int border0, int upto,
@@ -470,7 +470,9 @@ __device__ __noinline__ void pk_put_part(const PackedParams& p, const PkItem& it
 // The parts of rows whose keys were cut, in order: out = sum 2^(m_k - m) O_k / sum 2^(m_k - m) l_k.  A
 // CTA takes eight channels of a tile's 128 rows at a time, a thread a row, so that parts are read in
 // lines and by all SMs (the last arriver of a pair alone, 1.8 MB: 18 us).
-static __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant__ PackedParams p) {
+// kAhead parts are read before the first is used.
+template <int kAhead>
+__global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant__ PackedParams p) {
   const int count = min(p.cuts->count, kPkMaxCut), r = threadIdx.x, tok_in = r / p.group;
   if (tok_in >= p.tokens) return;
   for (int unit = blockIdx.x; unit < count * 32; unit += gridDim.x) {
@@ -485,7 +487,6 @@ static __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_co
     float m = -INFINITY, l = 0.f, v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    constexpr int kAhead = 8;
 #pragma unroll 1
     for (int k0 = 0; k0 < cut.splits; k0 += kAhead) {
       float2 a[kAhead];
