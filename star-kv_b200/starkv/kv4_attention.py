@@ -295,6 +295,8 @@ class KV4Attention(nn.Module):
         if isinstance(st, KV4Branches):
             if attention_mask is not None and not only_causal(attention_mask, T, before + T):
                 raise NotImplementedError("branches take no mask but one that says no more than causality")
+            if T <= MAX_DRAFT and self.keep_pages:       # ahead of the append: a call that raises leaves no token behind
+                st.select()
             if T > MAX_DRAFT:
                 out = st.attend_piece(q, k, v, self.scaling)
                 st.append(k, v)

@@ -396,3 +396,22 @@ def test_pieces_of_branches_report_errors(cuda, own):
     for _ in range(2):
         pool, got = run()
         assert pool.read_error() == 0 and torch.equal(got, want)
+
+
+@torch.no_grad()
+def test_refused_calls_of_branches_leave_no_token(cuda):
+    m, B = module(rope=Rope(128)), 2
+    one = StarKVCache(30)
+    m(make((1, 30, 1024), torch.float16, 1), None, None, past_key_values=one)
+    cache, x = one.branch(B, 40), make((B, 3, 1024), torch.float16, 2)
+    want = m(x, None, None, past_key_values=cache)[0]
+    for n, bad in enumerate((dict(keep_pages=4), dict(mask=torch.zeros(B, 1, 3, 5, device=cuda)), dict(batch=B + 1), dict(tokens=70))):
+        cache = one.branch(B, 40)
+        st = cache.kv4_states[0]
+        m.keep_pages = bad.get("keep_pages", 0)
+        y = make((bad.get("batch", B), bad.get("tokens", 3), 1024), torch.float16, 3)
+        with pytest.raises((NotImplementedError, ValueError, StarKVError)):
+            m(y, None, bad.get("mask"), past_key_values=cache)
+        m.keep_pages = 0
+        assert cache.get_seq_length() == 30 and not bool(st.lengths.any()), n
+        assert torch.equal(m(x, None, None, past_key_values=cache)[0], want), n
